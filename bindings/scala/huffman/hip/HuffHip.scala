@@ -168,6 +168,20 @@ trait HuffHip extends Library {
   // AdaptiveThreshold's register sets (adaptive_threshold.scala:41-79); out = {mode, threshold Q16,
   // depth limit, reserved: 4 x u32, then min_freq_threshold: u64}
   def hf_adaptive_threshold(entropyQ16: Int, depth: Int, wtWidth: Int, out: Pointer): Int
+  // quantised KV cache: rows into pages, pages into rows, attention over them, accepted drafts kept.
+  // cache, batch and query point at the structs of include/huffhip.h (hf_kv_cache, hf_kv_batch,
+  // hf_kv_query), laid out by the caller
+  def hf_kv_write(ctx: Pointer, cache: Pointer, batch: Pointer, dK: Pointer, dV: Pointer,
+                  kRowStride: Long, kHeadStride: Long, vRowStride: Long, vHeadStride: Long,
+                  dtype: Int): Int
+  def hf_kv_read(ctx: Pointer, cache: Pointer, batch: Pointer, dK: Pointer, dV: Pointer,
+                 kRowStride: Long, kHeadStride: Long, vRowStride: Long, vHeadStride: Long,
+                 dtype: Int): Int
+  def hf_kv_attend_work_bytes(ctx: Pointer, cache: Pointer, batch: Pointer, qHeads: Int): Long
+  def hf_kv_attend(ctx: Pointer, cache: Pointer, batch: Pointer, query: Pointer, dWork: Pointer,
+                   workBytes: Long): Int
+  def hf_kv_keep(ctx: Pointer, cache: Pointer, batch: Pointer, dPath: Pointer, pathStride: Long,
+                 pathWidth: Int, dPathLen: Pointer, dNewLen: Pointer): Int
   // TreeQualityAnalyzer.io (tree_q_analyser.scala:11-19)
   def hf_quality(ctx: Pointer, hFreq: Array[Long], hLen: Array[Byte], depth: Int, wtWidth: Int,
                  avgLenQ8: ShortByReference, efficiency: ShortByReference,

@@ -36,6 +36,8 @@ HF_CODEBOOK_STREAM, HF_CODEBOOK_PER_CHUNK = 0, 1
 HF_PLACEMENT_DENSE, HF_PLACEMENT_SLOTTED, HF_PLACEMENT_PAGED = 0, 1, 2
 HF_RESERVE_ENCODE, HF_RESERVE_CODEBOOKS, HF_RESERVE_PLACED, HF_RESERVE_ALL = 1, 2, 4, 7
 HF_PAGE_HDR_WORDS, HF_PAGE_GAP_WORDS = 10, 48
+HF_KV_BF16, HF_KV_FP16, HF_KV_FP8_E4M3, HF_KV_FP8_E5M2, HF_KV_FP4_E2M1 = 0, 1, 2, 3, 4
+HF_DT_BF16, HF_DT_FP16, HF_DT_FP32 = 0, 1, 2
 
 
 def HF_SLOT_WORDS(bits: int) -> int:
@@ -69,6 +71,33 @@ class hf_container_info(C.Structure):
         ("n", C.c_uint64), ("nchunks", C.c_uint64), ("payload_words", C.c_uint64),
         ("off_codebook", C.c_uint64), ("off_chunk_off", C.c_uint64), ("off_side", C.c_uint64),
         ("off_payload", C.c_uint64), ("total_bytes", C.c_uint64), ("off_chunk_words", C.c_uint64),
+    ]
+
+
+class hf_kv_cache(C.Structure):
+    _fields_ = [
+        ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("d_k_scale", C.c_void_p),
+        ("d_v_scale", C.c_void_p), ("n_pages", C.c_uint64), ("page_stride", C.c_int64),
+        ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("page_size", C.c_uint32),
+        ("heads", C.c_uint32), ("head_dim", C.c_uint32), ("group", C.c_uint32),
+        ("format", C.c_uint32), ("reserved", C.c_uint32),
+    ]
+
+
+class hf_kv_batch(C.Structure):
+    _fields_ = [
+        ("d_cu_rows", C.c_void_p), ("d_kv_len", C.c_void_p), ("d_table", C.c_void_p),
+        ("table_stride", C.c_int64), ("table_width", C.c_uint32), ("batch", C.c_uint32),
+        ("rows", C.c_uint32), ("max_rows", C.c_uint32),
+    ]
+
+
+class hf_kv_query(C.Structure):
+    _fields_ = [
+        ("d_q", C.c_void_p), ("d_out", C.c_void_p), ("d_lse", C.c_void_p), ("d_mask", C.c_void_p),
+        ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64), ("out_row_stride", C.c_int64),
+        ("out_head_stride", C.c_int64), ("q_heads", C.c_uint32), ("mask_words", C.c_uint32),
+        ("dtype", C.c_uint32), ("scale", C.c_float),
     ]
 
 
@@ -155,6 +184,15 @@ SIGNATURES = {
                                            _vp, _vp, C.c_uint64]),
     "hf_container_open": (C.c_int, [_vp, _vp, C.c_uint64, C.POINTER(hf_container_info)]),
     "hf_container_codebook": (C.c_int, [_vp, _vp, C.POINTER(hf_container_info), _vp]),
+    # (the hf_kv_* structs are passed as raw memory, as the Scala binding passes them; strides are
+    # int64_t)
+    "hf_kv_write": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64,
+                              C.c_int]),
+    "hf_kv_read": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64,
+                             C.c_int]),
+    "hf_kv_attend_work_bytes": (C.c_uint64, [_vp, _vp, _vp, C.c_uint32]),
+    "hf_kv_attend": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_uint64]),
+    "hf_kv_keep": (C.c_int, [_vp, _vp, _vp, _vp, C.c_uint64, C.c_uint32, _vp, _vp]),
     "hf_quality": (C.c_int, [_vp, _u64p, _u8p, C.c_int, C.c_int, _u16p, _u16p, _u16p]),
     "hf_last_kernel_ms": (C.c_int, [_vp, C.POINTER(C.c_float)]),
     "hf_set_timing": (C.c_int, [_vp, C.c_int]),

@@ -7,7 +7,7 @@
 #include <atomic>
 #include <new>
 
-#include "hf_common.h"
+#include "hf_kv.h"
 
 struct hf_ctx {
     int device;
@@ -1516,6 +1516,241 @@ int hf_container_codebook(hf_ctx* ctx, const void* d_blob, const hf_container_in
     HF_HIP(hipMemcpyAsync(ctx->h_ctl, ctx->d_ctl, 64, hipMemcpyDeviceToHost, ctx->stream));
     HF_HIP(hipStreamSynchronize(ctx->stream));
     return report_kernel_errors(ctx);
+}
+
+/* ---- quantised KV cache ----------------------------------------------------------------------- */
+namespace {
+
+inline int kv_code_bits(uint32_t format) {
+    return format == HF_KV_FP4_E2M1 ? 4 : format >= HF_KV_FP8_E4M3 ? 8 : 16;
+}
+
+int kv_check_cache(const hf_kv_cache* c, hf_kv_pools* p) {
+    if (!c || !c->d_k || !c->d_v || c->format > HF_KV_FP4_E2M1) return HF_ERR_ARG;
+    if (c->n_pages < 1 || c->n_pages > 0x7FFFFFFFull) return HF_ERR_ARG;
+    if (c->page_size < 8 || c->page_size > 65536 || !is_pow2((int)c->page_size)) return HF_ERR_ARG;
+    if (c->heads < 1 || c->heads > 1024) return HF_ERR_ARG;
+    if (c->head_dim < 32 || c->head_dim > 256 || c->head_dim % 32) return HF_ERR_ARG;
+    const int bits = kv_code_bits(c->format);
+    const int64_t row = (int64_t)c->head_dim * bits / 8;
+    if (c->page_stride < row || c->token_stride < row || c->head_stride < row) return HF_ERR_ARG;
+    if (bits < 16) {
+        if (!c->d_k_scale || !c->d_v_scale) return HF_ERR_ARG;
+        if (c->group < 32 || c->group > 256 || !is_pow2((int)c->group) || c->head_dim % c->group)
+            return HF_ERR_ARG;
+        if (!aligned16(c->d_k_scale) || !aligned16(c->d_v_scale)) return HF_ERR_ALIGN;
+    }
+    if (!aligned16(c->d_k) || !aligned16(c->d_v)) return HF_ERR_ALIGN;
+    if ((c->page_stride | c->token_stride | c->head_stride) & 15) return HF_ERR_ALIGN;
+    // (an offset inside a pool is computed in 63 bits)
+    if (c->page_stride > (1ll << 31) || c->token_stride > (1ll << 31) || c->head_stride > (1ll << 31))
+        return HF_ERR_RANGE;
+    p->k = (uint8_t*)c->d_k;
+    p->v = (uint8_t*)c->d_v;
+    p->k_scale = bits < 16 ? c->d_k_scale : nullptr;
+    p->v_scale = bits < 16 ? c->d_v_scale : nullptr;
+    p->page_stride = c->page_stride;
+    p->token_stride = c->token_stride;
+    p->head_stride = c->head_stride;
+    p->n_pages = (uint32_t)c->n_pages;
+    p->page_shift = (uint32_t)log2ceil_i((int)c->page_size);
+    p->heads = c->heads;
+    p->head_dim = c->head_dim;
+    p->group_shift = bits < 16 ? (uint32_t)log2ceil_i((int)c->group) : 8u;
+    p->groups = bits < 16 ? c->head_dim / c->group : 0u;
+    return HF_OK;
+}
+
+int kv_check_batch(const hf_kv_batch* b, hf_kv_seqs* s) {
+    if (!b) return HF_ERR_ARG;
+    if (b->batch > 0x7FFFFFFFu || b->rows > 0x7FFFFFFFu) return HF_ERR_RANGE;
+    if (b->batch && (!b->d_kv_len || !b->d_table || b->table_width < 1 || b->table_stride < b->table_width))
+        return HF_ERR_ARG;
+    if (!b->d_cu_rows && b->rows != b->batch) return HF_ERR_ARG;
+    s->cu = b->d_cu_rows;
+    s->kv_len = b->d_kv_len;
+    s->table = b->d_table;
+    s->table_stride = b->table_stride;
+    s->width = b->table_width;
+    s->batch = b->batch;
+    s->rows = b->rows;
+    s->most = b->rows;
+    return HF_OK;
+}
+
+// row tensors: whole 16-byte pieces wherever a row or a head starts
+int kv_check_rows(const void* p, int64_t row_stride, int64_t head_stride, int elem, hf_kv_rows* r) {
+    if (!p) return HF_ERR_ARG;
+    if (!aligned16(p) || (row_stride * elem) % 16 || (head_stride * elem) % 16) return HF_ERR_ALIGN;
+    if (row_stride < 0 || head_stride < 0) return HF_ERR_ARG;
+    if (row_stride > (1ll << 31) || head_stride > (1ll << 31)) return HF_ERR_RANGE;
+    r->p = const_cast<void*>(p);
+    r->row_stride = row_stride;
+    r->head_stride = head_stride;
+    return HF_OK;
+}
+
+int kv_move(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch, const void* d_k,
+            const void* d_v, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, int dtype,
+            bool write) {
+    hf_kv_pools p;
+    hf_kv_seqs s;
+    hf_kv_rows k, v;
+    if (!ctx) return HF_ERR_ARG;
+    if (int rc = kv_check_cache(cache, &p)) return rc;
+    if (int rc = kv_check_batch(batch, &s)) return rc;
+    if (dtype < HF_DT_BF16 || dtype > HF_DT_FP32) return HF_ERR_ARG;
+    if ((cache->format == HF_KV_BF16 && dtype == HF_DT_FP16) ||
+        (cache->format == HF_KV_FP16 && dtype == HF_DT_BF16))
+        return HF_ERR_ARG;
+    if (s.rows == 0 || s.batch == 0) return HF_OK;
+    const int elem = dtype == HF_DT_FP32 ? 4 : 2;
+    if (int rc = kv_check_rows(d_k, k_row, k_head, elem, &k)) return rc;
+    if (int rc = kv_check_rows(d_v, v_row, v_head, elem, &v)) return rc;
+    // (rows that are written must not lie on one another)
+    const int64_t row = p.head_dim;
+    if (!write && ((p.heads > 1 && (k_head < row || v_head < row)) || (s.rows > 1 && (k_row < row || v_row < row))))
+        return HF_ERR_ARG;
+    HF_USE_DEVICE(ctx);
+    tic(ctx);
+    if (write) hf_launch_kv_write(p, s, k, v, dtype, (int)cache->format, ctx->d_ctl + 1, ctx->num_cu, ctx->stream);
+    else hf_launch_kv_read(p, s, k, v, dtype, (int)cache->format, ctx->d_ctl + 1, ctx->num_cu, ctx->stream);
+    const hipError_t launch_err = hipGetLastError();
+    toc(ctx);
+    HF_HIP(launch_err);
+    return HF_OK;
+}
+
+// How a call of hf_kv_attend is cut: rows of a tile, workgroups, least range, and the scratch.
+struct kv_plan {
+    int tile_rows;
+    uint32_t target, min_steps, units;
+    bool join;
+    uint64_t part_floats, bytes;
+};
+int kv_plan_of(const hf_ctx* ctx, const hf_kv_pools& p, const hf_kv_seqs& s, uint32_t per, kv_plan* o) {
+    o->tile_rows = hf_kv_attend_tile_rows(s.most, per, p.head_dim);
+    o->target = (uint32_t)ctx->num_cu * (o->tile_rows == 64 ? 1u : 2u);
+    o->min_steps = 4;
+    const uint64_t rows = (uint64_t)s.rows * per;
+    const uint64_t by_rows = rows / o->tile_rows + s.batch;
+    const uint64_t by_most = (uint64_t)s.batch * (((uint64_t)s.most * per + o->tile_rows - 1) / o->tile_rows);
+    const uint64_t tiles = p.heads * (by_rows < by_most ? by_rows : by_most);
+    const uint64_t steps = (((uint64_t)s.width << p.page_shift) + 31) / 32;
+    const uint64_t most = (steps + o->min_steps - 1) / o->min_steps;  // ranges of a sequence, at most
+    o->join = most > 1;
+    uint64_t units = tiles + o->target;
+    if (most < units && tiles * most < units) units = tiles * most;
+    if (units > 0x7FFFFFFFull || (uint64_t)s.rows * p.heads * per > 0x7FFFFFFFull) return HF_ERR_RANGE;
+    o->units = (uint32_t)units;
+    const uint64_t pad = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
+    o->part_floats = o->join ? units * (uint64_t)o->tile_rows * pad : 0;
+    o->bytes = o->join ? 4 * o->part_floats + 8 * units * (uint64_t)o->tile_rows : 0;
+    return HF_OK;
+}
+
+int kv_check_attend(const hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
+                    uint32_t q_heads, hf_kv_pools* p, hf_kv_seqs* s, uint32_t* per) {
+    if (!ctx) return HF_ERR_ARG;
+    if (int rc = kv_check_cache(cache, p)) return rc;
+    if (int rc = kv_check_batch(batch, s)) return rc;
+    if (q_heads == 0 || q_heads % p->heads || q_heads > 65536) return HF_ERR_ARG;
+    *per = q_heads / p->heads;
+    if (s->cu == nullptr) {
+        s->most = 1;
+    } else {
+        if (batch->max_rows < 1 && s->rows) return HF_ERR_ARG;
+        s->most = batch->max_rows < s->rows ? batch->max_rows : s->rows;
+    }
+    if ((uint64_t)s->most * *per > 0x7FFFFFFFull) return HF_ERR_RANGE;
+    return HF_OK;
+}
+
+}  // namespace
+
+int hf_kv_write(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch, const void* d_k,
+                const void* d_v, int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                int64_t v_head_stride, int dtype) {
+    return kv_move(ctx, cache, batch, d_k, d_v, k_row_stride, k_head_stride, v_row_stride, v_head_stride,
+                   dtype, true);
+}
+
+int hf_kv_read(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch, void* d_k, void* d_v,
+               int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+               int64_t v_head_stride, int dtype) {
+    return kv_move(ctx, cache, batch, d_k, d_v, k_row_stride, k_head_stride, v_row_stride, v_head_stride,
+                   dtype, false);
+}
+
+uint64_t hf_kv_attend_work_bytes(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
+                                 uint32_t q_heads) {
+    hf_kv_pools p;
+    hf_kv_seqs s;
+    uint32_t per;
+    kv_plan plan;
+    if (kv_check_attend(ctx, cache, batch, q_heads, &p, &s, &per)) return 0;
+    if (s.rows == 0 || s.batch == 0 || kv_plan_of(ctx, p, s, per, &plan)) return 0;
+    return plan.bytes;
+}
+
+int hf_kv_attend(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
+                 const hf_kv_query* query, void* d_work, uint64_t work_bytes) {
+    hf_kv_attend_args a;
+    kv_plan plan;
+    if (!query) return HF_ERR_ARG;
+    if (int rc = kv_check_attend(ctx, cache, batch, query->q_heads, &a.c, &a.s, &a.per)) return rc;
+    if (query->dtype > HF_DT_FP16) return HF_ERR_ARG;
+    if (cache->format <= HF_KV_FP16 && query->dtype != cache->format) return HF_ERR_ARG;
+    if (!(query->scale > 0.0f) || query->scale > 3.0e38f) return HF_ERR_ARG;
+    if (a.s.rows == 0 || a.s.batch == 0) return HF_OK;
+    if (query->d_mask && (uint64_t)query->mask_words * 32u < a.s.most) return HF_ERR_ARG;
+    if (int rc = kv_check_rows(query->d_q, query->q_row_stride, query->q_head_stride, 2, &a.q)) return rc;
+    if (int rc = kv_check_rows(query->d_out, query->out_row_stride, query->out_head_stride, 2, &a.out)) return rc;
+    const int64_t row = a.c.head_dim;
+    if ((query->q_heads > 1 && query->out_head_stride < row) || (a.s.rows > 1 && query->out_row_stride < row))
+        return HF_ERR_ARG;
+    if (int rc = kv_plan_of(ctx, a.c, a.s, a.per, &plan)) return rc;
+    if (plan.bytes > work_bytes || (plan.bytes && !d_work)) return HF_ERR_ARG;
+    if (!aligned16(d_work)) return HF_ERR_ALIGN;
+    a.lse = query->d_lse;
+    a.mask = query->d_mask;
+    a.mask_words = query->mask_words;
+    a.scale_log2 = query->scale * 1.4426950408889634f;
+    a.part = (float*)d_work;
+    a.part_ml = (float*)d_work + plan.part_floats;
+    a.target = plan.target;
+    a.min_steps = plan.min_steps;
+    a.units = plan.units;
+    a.join = plan.join ? 1u : 0u;
+    a.err = ctx->d_ctl + 1;
+    HF_USE_DEVICE(ctx);
+    tic(ctx);
+    hf_launch_kv_attend(a, (int)query->dtype, (int)cache->format, plan.tile_rows, ctx->stream);
+    const hipError_t launch_err = hipGetLastError();
+    toc(ctx);
+    HF_HIP(launch_err);
+    return HF_OK;
+}
+
+int hf_kv_keep(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
+               const int32_t* d_path, int64_t path_stride, uint32_t path_width,
+               const int32_t* d_path_len, int32_t* d_new_len) {
+    hf_kv_pools p;
+    hf_kv_seqs s;
+    if (!ctx) return HF_ERR_ARG;
+    if (int rc = kv_check_cache(cache, &p)) return rc;
+    if (int rc = kv_check_batch(batch, &s)) return rc;
+    if (s.batch == 0) return HF_OK;
+    if (!d_path_len || !d_new_len || d_new_len == s.kv_len) return HF_ERR_ARG;
+    if ((path_width && !d_path) || path_stride < path_width || path_stride > (1ll << 31)) return HF_ERR_ARG;
+    HF_USE_DEVICE(ctx);
+    tic(ctx);
+    hf_launch_kv_keep(p, s, d_path, path_stride, path_width, d_path_len, d_new_len,
+                      p.head_dim * (uint32_t)kv_code_bits(cache->format) / 8u, ctx->d_ctl + 1, ctx->stream);
+    const hipError_t launch_err = hipGetLastError();
+    toc(ctx);
+    HF_HIP(launch_err);
+    return HF_OK;
 }
 
 /* ---- TreeQualityAnalyzer --------------------------------------------------------------------------

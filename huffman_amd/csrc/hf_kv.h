@@ -1,0 +1,108 @@
+// Shared by the KV-cache kernels: what a launch gets, formats, places of rows in the page pools.
+#pragma once
+
+#include "hf_common.h"
+
+// One cache as the kernels see it (hf_kv_cache, checked; strides in bytes).
+struct hf_kv_pools {
+    uint8_t* k;
+    uint8_t* v;
+    uint8_t* k_scale;  // [n_pages][heads][groups][page_size], NULL for the 16-bit formats
+    uint8_t* v_scale;
+    int64_t page_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+    uint32_t n_pages;
+    uint32_t page_shift;  // page_size = 1 << page_shift, at least 8 tokens
+    uint32_t heads;
+    uint32_t head_dim;    // multiple of 32, at most 256
+    uint32_t group_shift; // elements of a row that share a scale = 1 << group_shift
+    uint32_t groups;      // head_dim >> group_shift (0 for the 16-bit formats)
+};
+
+// The sequences of a call: rows cu[b] .. cu[b + 1] - 1 of the row tensors are the last rows of
+// sequence b, which has kv_len[b] tokens in the pages table[b][*].  cu == NULL: one row each.
+struct hf_kv_seqs {
+    const int32_t* cu;
+    const int32_t* kv_len;
+    const int32_t* table;
+    int64_t table_stride;
+    uint32_t width;  // pages in a row of the table
+    uint32_t batch;
+    uint32_t rows;   // rows of the row tensors
+    uint32_t most;   // rows a sequence has at most
+};
+
+// Row tensors [rows][heads][head_dim], strides in elements, head_dim contiguous.
+struct hf_kv_rows {
+    void* p;
+    int64_t row_stride;
+    int64_t head_stride;
+};
+
+struct hf_kv_attend_args {
+    hf_kv_pools c;
+    hf_kv_seqs s;
+    hf_kv_rows q;
+    hf_kv_rows out;
+    float* lse;            // [rows][q_heads], NULL: not wanted
+    const uint32_t* mask;  // [rows][mask_words], NULL: causal
+    uint32_t mask_words;
+    uint32_t per;          // query heads per cache head
+    float scale_log2;      // softmax scale x log2(e)
+    float* part;           // partial outputs of the units, [units][rows of a tile][padded head_dim]
+    float* part_ml;        // their maxima and sums, [units][rows of a tile][2]
+    uint32_t target;       // units the call is cut into, about
+    uint32_t min_steps;    // tokens / 32 a unit has at least
+    uint32_t units;        // workgroups of the call, and room of the partial buffers
+    uint32_t join;         // units may have to be joined (the partial buffers exist)
+    uint32_t* err;
+};
+
+int hf_kv_attend_tile_rows(uint32_t max_q, uint32_t per, uint32_t head_dim);
+void hf_launch_kv_write(const hf_kv_pools& c, const hf_kv_seqs& s, const hf_kv_rows& k,
+                        const hf_kv_rows& v, int dtype, int format, uint32_t* d_err, int num_cu,
+                        hipStream_t st);
+void hf_launch_kv_read(const hf_kv_pools& c, const hf_kv_seqs& s, const hf_kv_rows& k,
+                       const hf_kv_rows& v, int dtype, int format, uint32_t* d_err, int num_cu,
+                       hipStream_t st);
+void hf_launch_kv_keep(const hf_kv_pools& c, const hf_kv_seqs& s, const int32_t* path,
+                       int64_t path_stride, uint32_t path_width, const int32_t* path_len,
+                       int32_t* new_len, uint32_t row_bytes, uint32_t* d_err, hipStream_t st);
+void hf_launch_kv_attend(const hf_kv_attend_args& a, int dtype, int format, int tile_rows,
+                         hipStream_t st);
+
+#ifdef __HIPCC__
+typedef __attribute__((address_space(1))) uint8_t hf_g8;
+typedef __attribute__((address_space(1))) const int32_t hf_gi32;
+
+// Sequence b of a call, from the device's own lists.  Lists that do not describe rows of the call
+// (offsets that fall or leave the row tensors, more rows than tokens, more tokens than the table
+// holds) give n = 0 and bad = true: nothing of such a sequence is read or written.
+struct hf_kv_seq {
+    int32_t row0, n, past, len;
+    bool bad;
+};
+__device__ __forceinline__ hf_kv_seq hf_kv_sequence(const hf_kv_seqs& s, const uint32_t b,
+                                                    const uint32_t page_shift) {
+    hf_kv_seq q;
+    int32_t lo = (int32_t)b, hi = (int32_t)b + 1;
+    if (s.cu) {
+        lo = s.cu[b];
+        hi = s.cu[b + 1];
+    }
+    q.len = s.kv_len[b];
+    q.row0 = lo;
+    q.n = hi - lo;
+    q.past = q.len - q.n;
+    q.bad = lo < 0 || hi < lo || (uint32_t)hi > s.rows || (uint32_t)q.n > s.most || q.len < q.n ||
+            (uint64_t)(uint32_t)q.len > ((uint64_t)s.width << page_shift);
+    if (q.bad) {
+        q.row0 = 0;
+        q.n = 0;
+        q.past = 0;
+        q.len = 0;
+    }
+    return q;
+}
+#endif

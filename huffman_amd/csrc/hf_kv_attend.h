@@ -1,0 +1,771 @@
+// Attention of a sequence's last rows over its quantised pages: the kernel, as a template over the
+// type of the queries, the format of the cache, the padded head dimension DP and the row blocks R.
+//
+//   o_i = sum_t p_it v_t / sum_t p_it,   p_it = exp(scale q_i . k_t - m_i),   t over what i may see
+//
+// One unit = 16 R rows (tokens x query heads of one cache head of one sequence) against one range
+// of the sequence's tokens; a workgroup of four wavefronts takes a unit, its wavefronts taking the
+// unit's tokens 32 at a time in turn, each with its own running maximum and sum, and joins them
+// through LDS at the end.  There is no LDS and no barrier in the loop: the products are arranged so
+// that every operand is where it is needed,
+//
+//   S^T = K Q^T   A = 16 tokens of K, B = 16 rows of Q: a lane gets, of row lane % 16, four tokens
+//   O^T = V^T P^T B = P^T needs, of row lane % 16, eight tokens in the lane: those it has from two
+//                 products S^T, since the order of the tokens inside a product is free as long as A
+//                 and B agree; A = V^T needs eight tokens of one d in a lane: a lane loads its
+//                 DP / 16 neighbouring d of eight tokens and pairs them up with byte permutes
+//
+// and the d that a lane holds are free in the same way (any order that Q and K, or V and O, share).
+// Codes become 16-bit operands with the conversions that apply a power-of-two scale for nothing, so
+// scales may differ by token and by group of d.  The sums of S and O and the statistics are kept in
+// 32 bits; p is rounded to the type of the queries for the second product, as the codes' values are
+// exact in it (fp16: unless they leave its range, as reading the cache in fp16 would).
+#pragma once
+
+#include "hf_kv.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = 4;
+constexpr int kStep = 32;  // tokens a wavefront takes at a time
+
+template <int QT>
+struct kv_type;
+template <>
+struct kv_type<HF_DT_BF16> {
+    // bit patterns: exponent field of both halves, its lowest bit, infinity, one
+    static constexpr uint32_t expo = 0x7F807F80u, unit = 0x00800080u, inf = 0x7F80u, one = 0x3F80u;
+    static constexpr float off = 0.0f, rise = 8.0f;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+    }
+    static __device__ __forceinline__ f32x4 mma(hf_u32x4 a, hf_u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct kv_type<HF_DT_FP16> {
+    static constexpr uint32_t expo = 0x7C007C00u, unit = 0x04000400u, inf = 0x7C00u, one = 0x3C00u;
+    // p is held 2^7 up and may rise by 2^8 more, to 2^15: a p that fp16 flushes is below 2^-31 of
+    // the largest, so even a long row of such tokens beside one large one keeps its weight
+    static constexpr float off = 7.0f, rise = 8.0f;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+    }
+    static __device__ __forceinline__ f32x4 mma(hf_u32x4 a, hf_u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+
+// Two codes (elements 2i and 2i + 1 of the word) times the scale, as 16-bit values.
+template <int QT, int FMT, int I>
+__device__ __forceinline__ uint32_t kv_pair(const uint32_t w, const float s) {
+    if constexpr (FMT == HF_KV_FP8_E4M3) {
+        if constexpr (QT == HF_DT_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, I == 1));
+        else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, I == 1));
+    } else if constexpr (FMT == HF_KV_FP8_E5M2) {
+        if constexpr (QT == HF_DT_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, s, I == 1));
+        else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, s, I == 1));
+    } else if constexpr (FMT == HF_KV_FP4_E2M1) {
+        if constexpr (QT == HF_DT_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, I));
+        else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, I));
+    } else {
+        return w;  // two 16-bit values
+    }
+}
+
+// Bytes from global memory into consecutive 32-bit words (2 bytes: the low half of one).
+template <int BYTES>
+struct kv_raw {
+    uint32_t w[BYTES >= 4 ? BYTES / 4 : 1];
+    __device__ __forceinline__ void load(const hf_g8* p) {
+        if constexpr (BYTES == 2) {
+            w[0] = *(__attribute__((address_space(1))) const uint16_t*)p;
+        } else if constexpr (BYTES == 4) {
+            w[0] = *(__attribute__((address_space(1))) const uint32_t*)p;
+        } else if constexpr (BYTES == 8) {
+            const hf_u32x2 a = *(const hf_gmem_u32x2*)p;
+            w[0] = a.x;
+            w[1] = a.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) {
+                const hf_u32x4 a = *(const hf_gmem_u32x4*)(p + 16 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[4 * i + j] = a[j];
+            }
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < (BYTES >= 4 ? BYTES / 4 : 1); ++i) w[i] = 0;
+    }
+};
+
+template <int FMT>
+constexpr int kv_bits() {
+    return FMT == HF_KV_FP4_E2M1 ? 4 : (FMT == HF_KV_FP8_E4M3 || FMT == HF_KV_FP8_E5M2) ? 8 : 16;
+}
+
+__device__ __forceinline__ float kv_row_max(float a) {  // over the lanes of a row: l, l ^ 16, l ^ 32, l ^ 48
+    a = fmaxf(a, __shfl_xor(a, 16));
+    return fmaxf(a, __shfl_xor(a, 32));
+}
+__device__ __forceinline__ float kv_row_sum(float a) {
+    a += __shfl_xor(a, 16);
+    return a + __shfl_xor(a, 32);
+}
+
+// ---- the cut of a call into units ---------------------------------------------------------------
+// Every wavefront finds its unit from the device's own lengths, so a captured call follows lengths
+// that change between replays and a ragged batch is cut evenly: all sequences' steps (32 tokens)
+// times their row tiles are summed, divided by the units aimed at, and a sequence has as many
+// ranges of that many steps as it needs.  Units of a sequence are numbered range by range, in it by
+// cache head, in it by row tile, so that the tiles that read the same tokens are neighbours.
+struct kv_cut {
+    uint32_t b, n_before;  // sequence; units of the sequences before it
+    uint32_t tiles, ranges, steps_each;
+};
+
+__device__ __forceinline__ void kv_shape(const hf_kv_attend_args& a, const uint32_t tile_rows,
+                                         const uint32_t b, uint32_t& tiles, uint32_t& steps) {
+    const hf_kv_seq q = hf_kv_sequence(a.s, b, a.c.page_shift);
+    if (q.bad) atomicOr(a.err, HF_KERR_CORRUPT);
+    tiles = q.n > 0 ? a.c.heads * (((uint32_t)q.n * a.per + tile_rows - 1u) / tile_rows) : 0u;
+    steps = ((uint32_t)q.len + kStep - 1u) / kStep;
+}
+__device__ __forceinline__ uint32_t kv_steps_each(const hf_kv_attend_args& a, const uint32_t tile_rows) {
+    unsigned long long sum = 0;
+    for (uint32_t b0 = 0; b0 < a.s.batch; b0 += 64) {
+        const uint32_t b = b0 + hf_lane();
+        uint32_t tiles = 0, steps = 0;
+        if (b < a.s.batch) kv_shape(a, tile_rows, b, tiles, steps);
+        sum += (unsigned long long)tiles * steps;
+    }
+    sum = hf_wave_sum_u64(sum);
+    unsigned long long each = (sum + a.target - 1u) / a.target;
+    each = (each + kWaves - 1u) / kWaves * kWaves;
+    return (uint32_t)max(each, (unsigned long long)a.min_steps);
+}
+__device__ __forceinline__ uint32_t kv_ranges(const uint32_t steps, const uint32_t each) {
+    return max(1u, (steps + each - 1u) / each);
+}
+// The sequence that unit `unit` belongs to; false: there are fewer units.
+__device__ __forceinline__ bool kv_find(const hf_kv_attend_args& a, const uint32_t tile_rows,
+                                        const uint32_t unit, kv_cut& cut) {
+    cut.steps_each = kv_steps_each(a, tile_rows);
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < a.s.batch; b0 += 64) {
+        const uint32_t b = b0 + hf_lane();
+        uint32_t tiles = 0, steps = 0;
+        if (b < a.s.batch) kv_shape(a, tile_rows, b, tiles, steps);
+        const uint32_t ranges = kv_ranges(steps, cut.steps_each), own = tiles * ranges;
+        uint32_t incl = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t up = __shfl_up(incl, o);
+            if (hf_lane() >= o) incl += up;
+        }
+        const unsigned long long hit = __ballot(before + incl > unit);
+        if (hit) {
+            const int l = __ffsll((unsigned long long)hit) - 1;
+            cut.b = b0 + l;
+            cut.n_before = before + __builtin_amdgcn_readlane(incl - own, l);
+            cut.tiles = __builtin_amdgcn_readlane(tiles, l);
+            cut.ranges = __builtin_amdgcn_readlane(ranges, l);
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return false;
+}
+
+// ---- one unit ------------------------------------------------------------------------------------
+template <int QT, int FMT, int DP, int R>
+struct kv_unit {
+    typedef kv_type<QT> T;
+    static constexpr int bits = kv_bits<FMT>();
+    // K: a lane loads pieces of DPC consecutive d of a token: four lanes take 4 DPC of them
+    static constexpr int DPC = bits == 16 ? 8 : bits == 8 ? 16 : DP == 64 ? 16 : 32;
+    static constexpr int KP = DP / (4 * DPC);  // pieces per token and lane
+    static constexpr int KB = DPC * bits / 8;  // bytes of a piece
+    static constexpr int KS = DP / 32;         // products along d
+    // V: a lane loads VD consecutive d of eight tokens
+    static constexpr int VD = DP / 16;
+    static constexpr int VB = VD * bits / 8;
+
+    // what a wavefront holds of 32 tokens, as loaded
+    struct tile {
+        kv_raw<KB> k[2][KP];
+        kv_raw<VB> v[8];
+        hf_u32x2 ks[bits == 16 ? 1 : KP];  // scale bytes of the lane's eight tokens, by piece
+        hf_u32x2 vs;
+    };
+    struct pages {  // pages of the lane's tokens as a row of K and as eight columns of V
+        int32_t k, v;
+    };
+
+    const hf_kv_attend_args& a;
+    const int lane, m, g;
+    uint32_t head;
+    hf_kv_seq q;
+    const hf_gi32* table;
+    uint32_t groups_of_page;  // groups of eight tokens the table has pages for
+    f32x4 acc[R][VD];
+    float mx[R], sum[R];
+    hf_u32x4 qr[R][KS];
+    uint32_t bad;
+
+    __device__ __forceinline__ kv_unit(const hf_kv_attend_args& args)
+        : a(args), lane(hf_lane()), m(lane & 15), g(lane >> 4), bad(0) {}
+
+    // d of the lane's elements of product ks: first of eight
+    __device__ __forceinline__ int d_of(const int ks) const {
+        constexpr int per = DPC / 8;
+        return 4 * DPC * (ks / per) + DPC * g + 8 * (ks % per);
+    }
+
+    __device__ __forceinline__ void load_q(const int32_t row_lo, const int32_t rows) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int32_t i = row_lo + 16 * r + m;
+            const bool on = i < rows;
+            const int32_t tok = (on ? i : 0) / (int32_t)a.per, hq = (on ? i : 0) % (int32_t)a.per;
+            const hf_g8* p = (const hf_g8*)a.q.p + ((int64_t)(q.row0 + tok) * a.q.row_stride +
+                                                    (int64_t)(head * a.per + hq) * a.q.head_stride) * 2;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const int d = d_of(ks);
+                hf_u32x4 x = {0, 0, 0, 0};
+                if (on && d < (int)a.c.head_dim) x = *(const hf_gmem_u32x4*)(p + 2 * d);
+                qr[r][ks] = x;
+            }
+            mx[r] = -3.402823466e38f;
+            sum[r] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < VD; ++c) acc[r][c] = f32x4{0, 0, 0, 0};
+        }
+    }
+
+    // Tokens past the end of the sequence are taken from its last group of eight (a page holds
+    // whole groups, so all eight are inside it) and masked later.
+    __device__ __forceinline__ uint32_t group_at(const uint32_t t) const {
+        const uint32_t last = ((uint32_t)q.len - 1u) & ~7u;
+        return min(t, last);
+    }
+    __device__ __forceinline__ int32_t page_at(const uint32_t t) {
+        int32_t p = table[group_at(t) >> a.c.page_shift];
+        return p;
+    }
+    __device__ __forceinline__ pages find(const uint32_t t) {
+        pages p;
+        p.k = page_at(t + 8u * (m >> 2));
+        p.v = page_at(t + 8u * g);
+        return p;
+    }
+    __device__ __forceinline__ void load(const uint32_t t, pages p, tile& x) {
+        if ((uint32_t)p.k >= a.c.n_pages) { bad = 1; p.k = 0; }
+        if ((uint32_t)p.v >= a.c.n_pages) { bad = 1; p.v = 0; }
+        const uint32_t in_page = (1u << a.c.page_shift) - 1u;
+        const uint32_t ok = group_at(t + 8u * (m >> 2)) & in_page;
+        const uint32_t ov = group_at(t + 8u * g) & in_page;
+        const int64_t hk = (int64_t)head * a.c.head_stride;
+        const hf_g8* pk = (const hf_g8*)a.c.k + (int64_t)p.k * a.c.page_stride +
+                          (int64_t)(ok + (m & 3)) * a.c.token_stride + hk;
+        const hf_g8* pv = (const hf_g8*)a.c.v + (int64_t)p.v * a.c.page_stride +
+                          (int64_t)ov * a.c.token_stride + hk;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int h = 0; h < KP; ++h) {
+                const int d = 4 * DPC * h + DPC * g;
+                if (d < (int)a.c.head_dim) x.k[b][h].load(pk + d * bits / 8);
+                else x.k[b][h].clear();
+            }
+            pk += 4 * a.c.token_stride;
+        }
+        const bool on = VD * m < (int)a.c.head_dim;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (on) x.v[j].load(pv + VB * m);
+            else x.v[j].clear();
+            pv += a.c.token_stride;
+        }
+        if constexpr (bits != 16) {
+            const int64_t sk = (((int64_t)p.k * a.c.heads + head) * a.c.groups << a.c.page_shift) + ok;
+            const int64_t sv = (((int64_t)p.v * a.c.heads + head) * a.c.groups << a.c.page_shift) + ov;
+#pragma unroll
+            for (int h = 0; h < KP; ++h) {
+                const int d = 4 * DPC * h + DPC * g;
+                x.ks[h] = hf_u32x2{0, 0};
+                if (d < (int)a.c.head_dim)
+                    x.ks[h] = *(const hf_gmem_u32x2*)((const hf_g8*)a.c.k_scale + sk +
+                                                      ((int64_t)(d >> a.c.group_shift) << a.c.page_shift));
+            }
+            x.vs = hf_u32x2{0, 0};
+            if (on)
+                x.vs = *(const hf_gmem_u32x2*)((const hf_g8*)a.c.v_scale + sv +
+                                               ((int64_t)((VD * m) >> a.c.group_shift) << a.c.page_shift));
+        }
+    }
+
+    // Which of the lane's eight tokens t + 8 g + 0..7 row i (of the sequence's n rows) may see.
+    __device__ __forceinline__ uint32_t seen(const int32_t row, const uint32_t t, const bool on) const {
+        const int32_t j = (int32_t)(t + 8u * g) - q.past;  // draft number of the first of them
+        uint32_t bits8;
+        if (a.mask) {
+            const int32_t w = j >> 5;
+            const uint32_t* words = a.mask + (int64_t)(q.row0 + (on ? row : 0)) * a.mask_words;
+            const uint32_t lo = w < 0 ? ~0u : (uint32_t)w < a.mask_words ? words[w] : 0u;
+            const uint32_t hi = w + 1 < 0 ? ~0u : (uint32_t)(w + 1) < a.mask_words ? words[w + 1] : 0u;
+            bits8 = __builtin_amdgcn_alignbit(hi, lo, (uint32_t)j & 31u) & 0xFFu;
+        } else {
+            const int32_t can = min(max(row - j + 1, 0), 8);
+            bits8 = (1u << can) - 1u;
+        }
+        const int32_t left = min(max(q.n - j, 0), 8);  // tokens there are
+        return on ? bits8 & ((1u << left) - 1u) : 0u;
+    }
+
+    // The eight tokens of the lane as operand A of the product along tokens, for each of its d.
+    __device__ __forceinline__ void columns(const tile& x, const uint32_t there, hf_u32x4 (&av)[VD]) const {
+        uint32_t v[8][VD / 2];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // scale byte j of vs to the exponent of a float
+            const uint32_t w = j < 4 ? x.vs.x : x.vs.y;
+            const uint32_t sb = ((j & 3) == 3 ? w >> 1 : w << (23 - 8 * (j & 3))) & 0x7F800000u;
+            const float s = __uint_as_float(sb);
+            if constexpr (bits == 16) {
+#pragma unroll
+                for (int i = 0; i < VD / 2; ++i) v[j][i] = x.v[j].w[i];
+            } else if constexpr (bits == 8) {
+#pragma unroll
+                for (int i = 0; i < VD / 4; ++i) {
+                    v[j][2 * i] = kv_pair<QT, FMT, 0>(x.v[j].w[i], s);
+                    v[j][2 * i + 1] = kv_pair<QT, FMT, 1>(x.v[j].w[i], s);
+                }
+            } else {
+                v[j][0] = kv_pair<QT, FMT, 0>(x.v[j].w[0], s);
+                v[j][1] = kv_pair<QT, FMT, 1>(x.v[j].w[0], s);
+                if constexpr (VD >= 8) {
+                    v[j][2] = kv_pair<QT, FMT, 2>(x.v[j].w[0], s);
+                    v[j][3] = kv_pair<QT, FMT, 3>(x.v[j].w[0], s);
+                }
+                if constexpr (VD >= 16) {
+                    v[j][4] = kv_pair<QT, FMT, 0>(x.v[j].w[1], s);
+                    v[j][5] = kv_pair<QT, FMT, 1>(x.v[j].w[1], s);
+                    v[j][6] = kv_pair<QT, FMT, 2>(x.v[j].w[1], s);
+                    v[j][7] = kv_pair<QT, FMT, 3>(x.v[j].w[1], s);
+                }
+            }
+            if (!(there >> j & 1u)) {  // nothing is known of what the page holds behind the last token
+#pragma unroll
+                for (int i = 0; i < VD / 2; ++i) v[j][i] = 0;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VD / 2; ++i)
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+                av[2 * i][jj] = __builtin_amdgcn_perm(v[2 * jj + 1][i], v[2 * jj][i], 0x05040100u);
+                av[2 * i + 1][jj] = __builtin_amdgcn_perm(v[2 * jj + 1][i], v[2 * jj][i], 0x07060302u);
+            }
+    }
+
+    // A step: 32 tokens from t.  FULL: every row sees all of them.
+    template <bool FULL>
+    __device__ __forceinline__ void step(const uint32_t t, const tile& x, const int32_t row_lo,
+                                         const int32_t rows) {
+        f32x4 s[R][2];
+        {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                hf_u32x4 ka[KS];
+#pragma unroll
+                for (int h = 0; h < KP; ++h) {
+                    float f = 0.0f;
+                    if constexpr (bits != 16) {
+                        const uint32_t w = b ? x.ks[h].y : x.ks[h].x;
+                        f = __uint_as_float(__builtin_amdgcn_ubfe(w, 8u * (m & 3), 8u) << 23);
+                    }
+                    if constexpr (bits == 16) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) ka[h][i] = x.k[b][h].w[i];
+                    } else if constexpr (bits == 8) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            ka[2 * h + i / 2][2 * (i % 2)] = kv_pair<QT, FMT, 0>(x.k[b][h].w[i], f);
+                            ka[2 * h + i / 2][2 * (i % 2) + 1] = kv_pair<QT, FMT, 1>(x.k[b][h].w[i], f);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < KB / 4; ++i) {
+                            constexpr int per = DPC / 8;
+                            ka[per * h + i][0] = kv_pair<QT, FMT, 0>(x.k[b][h].w[i], f);
+                            ka[per * h + i][1] = kv_pair<QT, FMT, 1>(x.k[b][h].w[i], f);
+                            ka[per * h + i][2] = kv_pair<QT, FMT, 2>(x.k[b][h].w[i], f);
+                            ka[per * h + i][3] = kv_pair<QT, FMT, 3>(x.k[b][h].w[i], f);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    s[r][b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) s[r][b] = T::mma(ka[ks], qr[r][ks], s[r][b]);
+                }
+            }
+        }
+        uint32_t see[R];
+        float top[R];
+        bool up = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if constexpr (!FULL) {
+                const int32_t i = row_lo + 16 * r + m;
+                see[r] = seen((i < rows ? i : 0) / (int32_t)a.per, t, i < rows);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    s[r][e / 4][e % 4] = see[r] >> e & 1u ? s[r][e / 4][e % 4] : -__builtin_inff();
+            }
+            top[r] = s[r][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) top[r] = fmaxf(top[r], s[r][e / 4][e % 4]);
+            top[r] *= a.scale_log2;
+            up = up || top[r] > mx[r] + (T::off + T::rise);
+        }
+        if (__ballot(up)) {  // seldom after the first step: sums and outputs to a new maximum
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float was = mx[r];
+                mx[r] = fmaxf(was, kv_row_max(top[r]) - T::off);
+                const float f = __builtin_amdgcn_exp2f(was - mx[r]);
+                sum[r] *= f;
+#pragma unroll
+                for (int c = 0; c < VD; ++c) acc[r][c] *= f;
+            }
+        }
+        hf_u32x4 p[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i / 4][i % 4], a.scale_log2, -mx[r]));
+                sum[r] += e[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[r][i] = T::pack(e[2 * i], e[2 * i + 1]);
+        }
+        hf_u32x4 av[VD];
+        uint32_t there = 0xFFu;
+        if constexpr (!FULL) {
+            const int32_t left = min(max(q.len - (int32_t)(t + 8u * g), 0), 8);
+            there = (1u << left) - 1u;
+        }
+        columns(x, there, av);
+        if constexpr (!FULL) {
+            // A token that some rows may not see must not reach them as 0 x infinity or NaN.
+            uint32_t odd = 0;
+#pragma unroll
+            for (int c = 0; c < VD; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) odd |= ((av[c][i] & T::expo) + T::unit) & 0x80008000u;
+            if (__ballot(odd != 0)) not_finite(av, see);
+        }
+#pragma unroll
+        for (int c = 0; c < VD; ++c)
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[r][c] = T::mma(av[c], p[r], acc[r][c]);
+    }
+
+    // Takes infinities and NaN out of the tokens' values and adds them to the outputs of the rows
+    // that see their token: how many a row sees of each kind is a product of ones.
+    __device__ __forceinline__ void not_finite(hf_u32x4 (&av)[VD], const uint32_t (&see)[R]) {
+#pragma unroll 1
+        for (int kind = 0; kind < 3; ++kind) {
+            const float add = kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
+#pragma unroll
+            for (int c = 0; c < VD; ++c) {
+                hf_u32x4 is;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    is[i] = 0;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t x = av[c][i] >> (16 * h) & 0xFFFFu, mag = x & 0x7FFFu;
+                        const bool hit = kind == 0 ? mag > T::inf : x == (kind == 1 ? T::inf : T::inf | 0x8000u);
+                        if (hit) is[i] |= T::one << (16 * h);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    hf_u32x4 ones;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        ones[i] = (see[r] >> (2 * i) & 1u ? T::one : 0u) | (see[r] >> (2 * i + 1) & 1u ? T::one << 16 : 0u);
+                    const f32x4 count = T::mma(is, ones, f32x4{0, 0, 0, 0});
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (count[i] > 0.0f) acc[r][c][i] += add;
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < VD; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if ((av[c][i] & 0x7FFFu) >= T::inf) av[c][i] &= 0xFFFF0000u;
+                if ((av[c][i] >> 16 & 0x7FFFu) >= T::inf) av[c][i] &= 0xFFFFu;
+            }
+    }
+};
+
+// Scratch of a workgroup: what two wavefronts hand to the other two.
+template <int DP, int R>
+struct kv_lds {
+    f32x4 acc[2][R][DP / 16][64];
+    float mx[2][R][64], sum[2][R][64];
+};
+
+template <int QT, int FMT, int DP, int R>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(R == 4 || DP * R > 256 ? 1 : 2)))
+void hf_k_kv_attend(const hf_kv_attend_args a) {
+    typedef kv_unit<QT, FMT, DP, R> U;
+    constexpr uint32_t tile_rows = 16 * R;
+    __shared__ kv_lds<DP, R> lds;
+    kv_cut cut;
+    if (!kv_find(a, tile_rows, blockIdx.x, cut)) return;
+    U u(a);
+    u.q = hf_kv_sequence(a.s, cut.b, a.c.page_shift);
+    const uint32_t in_seq = blockIdx.x - cut.n_before;
+    const uint32_t row_tiles = cut.tiles / a.c.heads;
+    const uint32_t range = in_seq / cut.tiles, tile = in_seq % cut.tiles;
+    u.head = tile / row_tiles;
+    const int32_t rows = u.q.n * (int32_t)a.per;
+    const int32_t row_lo = (int32_t)(tile % row_tiles * tile_rows);
+    u.table = (const hf_gi32*)(a.s.table + (int64_t)cut.b * a.s.table_stride);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+
+    // tokens of the unit, and how far every row of the tile sees all of them
+    const int32_t tok_lo = row_lo / (int32_t)a.per;
+    const int32_t tok_hi = (min(row_lo + (int32_t)tile_rows, rows) - 1) / (int32_t)a.per;
+    const uint32_t whole = (uint32_t)(a.mask ? u.q.past : u.q.past + tok_lo + 1);
+    uint32_t end = (uint32_t)(a.mask ? u.q.len : u.q.past + tok_hi + 1);
+    const uint32_t t_lo = range * cut.steps_each * kStep;
+    end = min(end, t_lo + cut.steps_each * kStep);
+
+    u.load_q(row_lo, rows);
+    uint32_t t = t_lo + kStep * (uint32_t)wave;
+    if (t < end) {
+        constexpr uint32_t stride = kStep * kWaves;
+        typename U::tile x0, x1;
+        typename U::pages p = u.find(t);
+        u.load(t, p, x0);
+        p = u.find(t + stride);
+        auto one = [&](typename U::tile& now, typename U::tile& next) {
+            // the next tokens' bytes and the pages of those after them are under way meanwhile
+            if (t + stride < end) {
+                u.load(t + stride, p, next);
+                p = u.find(t + 2 * stride);
+            }
+            if (t + kStep <= whole && t + kStep <= end) u.template step<true>(t, now, row_lo, rows);
+            else u.template step<false>(t, now, row_lo, rows);
+            t += stride;
+        };
+        while (true) {
+            one(x0, x1);
+            if (t >= end) break;
+            one(x1, x0);
+            if (t >= end) break;
+        }
+    }
+    if (u.bad) atomicOr(a.err, HF_KERR_CORRUPT);
+
+    // join the wavefronts: 2 and 3 hand to 0 and 1, then 1 to 0
+#pragma unroll
+    for (int r = 0; r < R; ++r) u.sum[r] = kv_row_sum(u.sum[r]);
+#pragma unroll 1
+    for (int half = 2; half >= 1; half >>= 1) {
+        if (wave >= half && wave < 2 * half) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                lds.mx[wave - half][r][u.lane] = u.mx[r];
+                lds.sum[wave - half][r][u.lane] = u.sum[r];
+#pragma unroll
+                for (int c = 0; c < U::VD; ++c) lds.acc[wave - half][r][c][u.lane] = u.acc[r][c];
+            }
+        }
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float om = lds.mx[wave][r][u.lane];
+                const float top = fmaxf(u.mx[r], om);
+                const float f = __builtin_amdgcn_exp2f(u.mx[r] - top), h = __builtin_amdgcn_exp2f(om - top);
+                u.mx[r] = top;
+                u.sum[r] = u.sum[r] * f + lds.sum[wave][r][u.lane] * h;
+#pragma unroll
+                for (int c = 0; c < U::VD; ++c) u.acc[r][c] = u.acc[r][c] * f + lds.acc[wave][r][c][u.lane] * h;
+            }
+        }
+        __syncthreads();
+    }
+    if (wave != 0) return;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int32_t i = row_lo + 16 * r + u.m;
+        if (cut.ranges > 1) {  // to be joined with the other ranges
+            const int64_t row = (int64_t)blockIdx.x * tile_rows + 16 * r + u.m;
+            float* dst = a.part + row * DP;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < U::VD; c += 4)
+                    *(f32x4*)(dst + U::VD * (4 * u.g + e) + c) =
+                        f32x4{u.acc[r][c][e], u.acc[r][c + 1][e], u.acc[r][c + 2][e], u.acc[r][c + 3][e]};
+            if (u.g == 0) {
+                a.part_ml[2 * row] = u.mx[r];
+                a.part_ml[2 * row + 1] = u.sum[r];
+            }
+        } else if (i < rows) {
+            const int32_t tok = i / (int32_t)a.per, hq = i % (int32_t)a.per;
+            const uint32_t out_head = u.head * a.per + hq;
+            const float l = u.sum[r], f = l == 0.0f ? 0.0f : 1.0f / l;  // no token seen: zeros
+            hf_g8* dst = (hf_g8*)a.out.p + ((int64_t)(u.q.row0 + tok) * a.out.row_stride +
+                                            (int64_t)out_head * a.out.head_stride) * 2;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = U::VD * (4 * u.g + e);
+                if (d < (int)a.c.head_dim) {
+#pragma unroll
+                    for (int c = 0; c < U::VD; c += 4)
+                        *(hf_gmem_u32x2*)(dst + 2 * (d + c)) =
+                            hf_u32x2{U::T::pack(u.acc[r][c][e] * f, u.acc[r][c + 1][e] * f),
+                                     U::T::pack(u.acc[r][c + 2][e] * f, u.acc[r][c + 3][e] * f)};
+                }
+            }
+            if (a.lse && u.g == 0)
+                a.lse[(int64_t)(u.q.row0 + tok) * a.c.heads * a.per + out_head] =
+                    l == 0.0f ? -__builtin_inff() : 0.6931471805599453f * (u.mx[r] + __builtin_amdgcn_logf(l));
+        }
+    }
+}
+
+// Joins the ranges of a row: a wavefront per row, DP / 4 lanes along the row and the ranges dealt to
+// the groups of lanes that are left.
+template <int QT, int DP, int R>
+__global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a) {
+    typedef kv_type<QT> T;
+    constexpr uint32_t tile_rows = 16 * R;
+    constexpr uint32_t cols = DP / 4, deal = 64 / cols;
+    const uint32_t each = kv_steps_each(a, tile_rows);
+    const uint32_t q_heads = a.c.heads * a.per;
+    const uint32_t id = blockIdx.x * 4u + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int32_t row = (int32_t)(id / q_heads);
+    const uint32_t out_head = id % q_heads;
+    if ((uint32_t)row >= a.s.rows) return;
+    // the sequence of the row, and the units before it
+    uint32_t before = 0;
+    bool found = false;
+    hf_kv_seq q;
+    uint32_t tiles = 0, ranges = 0;
+    for (uint32_t b0 = 0; b0 < a.s.batch && !found; b0 += 64) {
+        const uint32_t b = b0 + hf_lane();
+        uint32_t nt = 0, steps = 0;
+        bool mine = false;
+        if (b < a.s.batch) {
+            const hf_kv_seq s = hf_kv_sequence(a.s, b, a.c.page_shift);
+            nt = s.n > 0 ? a.c.heads * (((uint32_t)s.n * a.per + tile_rows - 1u) / tile_rows) : 0u;
+            steps = ((uint32_t)s.len + kStep - 1u) / kStep;
+            mine = row >= s.row0 && row < s.row0 + s.n;
+        }
+        const uint32_t nr = kv_ranges(steps, each);
+        uint32_t units = nt * nr, incl = units;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t up = __shfl_up(incl, o);
+            if (hf_lane() >= o) incl += up;
+        }
+        const unsigned long long hit = __ballot(mine);
+        if (hit) {
+            const int l = __ffsll((unsigned long long)hit) - 1;
+            found = true;
+            q = hf_kv_sequence(a.s, b0 + l, a.c.page_shift);
+            before += __builtin_amdgcn_readlane(incl - units, l);
+            tiles = __builtin_amdgcn_readlane(nt, l);
+            ranges = __builtin_amdgcn_readlane(nr, l);
+        } else {
+            before += __builtin_amdgcn_readlane(incl, 63);
+        }
+    }
+    if (!found || ranges < 2) return;
+    const uint32_t i = (uint32_t)(row - q.row0) * a.per + out_head % a.per;
+    const uint32_t tile = out_head / a.per * (tiles / a.c.heads) + i / tile_rows;
+    // (offsets that cover a row twice, which the attending kernel reports, can count more units
+    // than there are)
+    if ((uint64_t)before + (uint64_t)tiles * ranges > a.units) return;
+    const int64_t first = (int64_t)(before + tile) * tile_rows + i % tile_rows;
+    const int64_t jump = (int64_t)tiles * tile_rows;
+    const uint32_t col = (uint32_t)hf_lane() % cols, part = (uint32_t)hf_lane() / cols;
+    float top = -3.402823466e38f;
+    for (uint32_t s = hf_lane(); s < ranges; s += 64) top = fmaxf(top, a.part_ml[2 * (first + s * jump)]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    f32x4 acc = {0, 0, 0, 0};
+    float sum = 0.0f;
+#pragma unroll 4
+    for (uint32_t s = part; s < ranges; s += deal) {
+        const int64_t at = first + s * jump;
+        const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - top);
+        sum += w * a.part_ml[2 * at + 1];
+        acc += w * *(const f32x4*)(a.part + at * DP + 4 * col);
+    }
+#pragma unroll
+    for (int o = cols; o < 64; o <<= 1) {
+        sum += __shfl_xor(sum, o);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
+    }
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (part == 0 && 4 * col < a.c.head_dim) {
+        hf_g8* dst = (hf_g8*)a.out.p + ((int64_t)row * a.out.row_stride + (int64_t)out_head * a.out.head_stride) * 2;
+        *(hf_gmem_u32x2*)(dst + 8 * col) =
+            hf_u32x2{T::pack(acc[0] * f, acc[1] * f), T::pack(acc[2] * f, acc[3] * f)};
+    }
+    if (a.lse && hf_lane() == 0)
+        a.lse[(int64_t)row * q_heads + out_head] =
+            sum == 0.0f ? -__builtin_inff() : 0.6931471805599453f * (top + __builtin_amdgcn_logf(sum));
+}
+
+template <int QT, int FMT, int DP, int R>
+void kv_launch(const hf_kv_attend_args& a, hipStream_t st) {
+    hipLaunchKernelGGL((hf_k_kv_attend<QT, FMT, DP, R>), dim3(a.units), dim3(64 * kWaves), 0, st, a);
+    if (a.join) {
+        const uint64_t rows = (uint64_t)a.s.rows * a.c.heads * a.per;
+        hipLaunchKernelGGL((hf_k_kv_join<QT, DP, R>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, st, a);
+    }
+}
+template <int QT, int FMT, int DP>
+void kv_launch_rows(const hf_kv_attend_args& a, const int tile_rows, hipStream_t st) {
+    if (tile_rows == 16) kv_launch<QT, FMT, DP, 1>(a, st);
+    else if (tile_rows == 32 || DP == 256) kv_launch<QT, FMT, DP, 2>(a, st);
+    else if constexpr (DP < 256) kv_launch<QT, FMT, DP, 4>(a, st);
+}
+template <int QT, int FMT>
+void kv_launch_dim(const hf_kv_attend_args& a, const int tile_rows, hipStream_t st) {
+    if (a.c.head_dim <= 64) kv_launch_rows<QT, FMT, 64>(a, tile_rows, st);
+    else if (a.c.head_dim <= 128) kv_launch_rows<QT, FMT, 128>(a, tile_rows, st);
+    else kv_launch_rows<QT, FMT, 256>(a, tile_rows, st);
+}
+
+}  // namespace

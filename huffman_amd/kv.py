@@ -1,0 +1,230 @@
+"""The quantised KV cache over the C ABI: rows written into pages of 8- or 4-bit codes (or 16-bit
+values), read back, attended to, and the accepted drafts of a tree kept.
+
+The pages are what the codec takes: a dense pool of fp8 pages is a run of 16384-symbol blocks for
+``EntropyAwareHuffmanSystem.encode_blocks``, and ``ParrallelHuffmanDecoder.decode_blocks_to``
+decodes stored pages straight into a pool.  The reference names the operand formats
+(reports/spec.md:22) and has no counterpart of these calls.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib as L
+from ._lib import check
+from .api import Context, _Module, default_context
+
+_DTYPES = {torch.bfloat16: L.HF_DT_BF16, torch.float16: L.HF_DT_FP16, torch.float32: L.HF_DT_FP32}
+_POOL_DTYPES = {
+    L.HF_KV_BF16: (torch.bfloat16,), L.HF_KV_FP16: (torch.float16,),
+    L.HF_KV_FP8_E4M3: (torch.uint8, torch.float8_e4m3fn),
+    L.HF_KV_FP8_E5M2: (torch.uint8, torch.float8_e5m2), L.HF_KV_FP4_E2M1: (torch.uint8,),
+}
+
+
+class KvCache(_Module):
+    """Two page pools and their scales (include/huffhip.h has the layout and the arithmetic).
+
+    ``k``, ``v``: [pages, page_size, heads, head_dim] of codes (uint8 or the float8 type; fp4: two
+    codes a byte, so the last dimension is head_dim / 2) or of the 16-bit type, any strides with a
+    contiguous last dimension, the same for both.  ``k_scale``, ``v_scale``: uint8 [pages, heads,
+    head_dim / group, page_size], contiguous; None for a 16-bit cache.  The pools stay the
+    caller's: the cache keeps them alive and never allocates, copies or clears them.
+
+    In every call ``table`` is int32 [batch, pages of a sequence], ``kv_len`` int32 [batch] (tokens
+    of a sequence, the call's rows included) and ``cu`` int32 [batch + 1], the first row of each
+    sequence; None: one row each.  They are read on the device, on the context's stream; what they
+    say wrongly is reported by ``Context.sync``.  No call synchronises or copies to the host.
+    """
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+                 v_scale: Optional[torch.Tensor] = None, fmt: int = L.HF_KV_FP8_E4M3,
+                 ctx: Optional[Context] = None):
+        super().__init__(ctx)
+        if fmt not in _POOL_DTYPES:
+            raise ValueError(f"unknown cache format {fmt}")
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.device != v.device:
+            raise ValueError("k and v: [pages, page_size, heads, head_dim], alike in shape, strides and device")
+        if k.dtype not in _POOL_DTYPES[fmt] or v.dtype != k.dtype:
+            raise TypeError(f"cache format {fmt} holds {_POOL_DTYPES[fmt]}, not {k.dtype}, {v.dtype}")
+        if not k.is_cuda or k.stride(3) != 1:
+            raise ValueError("the pools are device tensors with a contiguous last dimension")
+        pages, page_size, heads, width = k.shape
+        dim = 2 * width if fmt == L.HF_KV_FP4_E2M1 else width
+        group = 0
+        if fmt in (L.HF_KV_BF16, L.HF_KV_FP16):
+            if k_scale is not None or v_scale is not None:
+                raise ValueError("a 16-bit cache has no scales")
+        else:
+            for s in (k_scale, v_scale):
+                if s is None or s.dtype != torch.uint8 or s.device != k.device or not s.is_contiguous() \
+                        or s.dim() != 4 or s.shape[0] != pages or s.shape[1] != heads \
+                        or s.shape[2] < 1 or dim % s.shape[2] or s.shape[3] != page_size \
+                        or s.shape != k_scale.shape:
+                    raise ValueError("scales: contiguous uint8 [pages, heads, head_dim / group, page_size]")
+            group = dim // k_scale.shape[2]
+        self.k, self.v, self.k_scale, self.v_scale, self.fmt = k, v, k_scale, v_scale, fmt
+        self.heads, self.head_dim, self.group, self.page_size = heads, dim, group, page_size
+        size = k.element_size()
+        self._c = L.hf_kv_cache(
+            k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if group else 0,
+            v_scale.data_ptr() if group else 0, pages, k.stride(0) * size, k.stride(1) * size,
+            k.stride(2) * size, page_size, heads, dim, group, fmt, 0)
+        if pages < 2 or page_size < 2 or heads < 2:  # strides of a dimension of one say nothing
+            row = width * size
+            fix = self._c
+            fix.head_stride = max(fix.head_stride, row) if heads > 1 else row
+            fix.token_stride = max(fix.token_stride, row) if page_size > 1 else row
+            fix.page_stride = fix.page_stride if pages > 1 else max(fix.token_stride, fix.head_stride, row)
+
+    @staticmethod
+    def empty(pages: int, page_size: int, heads: int, head_dim: int, fmt: int = L.HF_KV_FP8_E4M3,
+              group: Optional[int] = None, ctx: Optional[Context] = None) -> "KvCache":
+        """A cache with dense pools of its own, cleared.  ``group``: elements of a row that share a
+        scale (default: the largest power of two that divides head_dim)."""
+        ctx = ctx if ctx is not None else default_context()
+        dev = f"cuda:{ctx.device}"
+        wide = fmt in (L.HF_KV_BF16, L.HF_KV_FP16)
+        dtype = {L.HF_KV_BF16: torch.bfloat16, L.HF_KV_FP16: torch.float16}.get(fmt, torch.uint8)
+        width = head_dim // 2 if fmt == L.HF_KV_FP4_E2M1 else head_dim
+        if group is None:
+            group = head_dim & -head_dim
+        with torch.cuda.stream(ctx.stream):
+            pools = [torch.zeros(pages, page_size, heads, width, dtype=dtype, device=dev) for _ in range(2)]
+            scales = [None, None] if wide else [
+                torch.full((pages, heads, head_dim // group, page_size), 127, dtype=torch.uint8, device=dev)
+                for _ in range(2)]
+        return KvCache(*pools, *scales, fmt=fmt, ctx=ctx)
+
+    # -- arguments -------------------------------------------------------------------------------
+    def _ints(self, name: str, t: torch.Tensor, dim: int) -> torch.Tensor:
+        if t.dtype != torch.int32 or t.dim() != dim or t.device != self.k.device or \
+                (t.numel() and t.stride(-1) != 1):
+            raise ValueError(f"{name}: int32, {dim} dimension(s), contiguous rows, on the pools' device")
+        return t
+
+    def _batch(self, table, kv_len, cu, rows: int, max_rows: int) -> L.hf_kv_batch:
+        if self.k.device.index != self.ctx.device:
+            raise ValueError(f"the pools are on {self.k.device}, the context on cuda:{self.ctx.device}")
+        self._ints("table", table, 2)
+        self._ints("kv_len", kv_len, 1)
+        batch = table.shape[0]
+        if kv_len.shape[0] != batch:
+            raise ValueError("kv_len: one length for every row of the table")
+        if cu is None:
+            if rows != batch:
+                raise ValueError("without cu there is one row for each sequence")
+        elif self._ints("cu", cu, 1).shape[0] != batch + 1:
+            raise ValueError("cu: batch + 1 row offsets")
+        return L.hf_kv_batch(cu.data_ptr() if cu is not None else 0, kv_len.data_ptr(), table.data_ptr(),
+                             table.stride(0) if batch > 1 else table.shape[1], table.shape[1], batch,
+                             rows, max_rows)
+
+    def _rows(self, name: str, t: torch.Tensor, heads: int) -> Tuple[int, int, int]:
+        """Pointer and strides of a row tensor."""
+        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim or t.device != self.k.device \
+                or (t.numel() and t.stride(2) != 1):
+            raise ValueError(f"{name}: [rows, {heads}, {self.head_dim}] on the pools' device, last dimension contiguous")
+        if t.dtype not in _DTYPES:
+            raise TypeError(f"{name}: bf16, fp16 or fp32, not {t.dtype}")
+        # (a stride of a dimension of one says nothing)
+        head = t.stride(1) if heads > 1 else self.head_dim
+        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else heads * head, head
+
+    # -- calls -----------------------------------------------------------------------------------
+    def write(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor,
+              cu: Optional[torch.Tensor] = None) -> None:
+        """``hf_kv_write``: quantise rows [rows, heads, head_dim] into the last places of their
+        sequences.  Rows outside every sequence are not looked at."""
+        if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
+            raise ValueError("k and v: as many rows of the same type")
+        pk, kr, kh = self._rows("k", k, self.heads)
+        pv, vr, vh = self._rows("v", v, self.heads)
+        b = self._batch(table, kv_len, cu, k.shape[0], 0)
+        check(L.lib().hf_kv_write(self.ctx.handle, C.byref(self._c), C.byref(b), pk, pv, kr, kh, vr, vh,
+                                  _DTYPES[k.dtype]), "hf_kv_write")
+
+    def read(self, table: torch.Tensor, kv_len: torch.Tensor, cu: Optional[torch.Tensor] = None,
+             rows: Optional[int] = None, dtype: torch.dtype = torch.bfloat16,
+             out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``hf_kv_read``: the last rows of the sequences as (keys, values) of ``dtype``, [rows,
+        heads, head_dim] (whole sequences: offsets that count their tokens).  ``rows`` is needed
+        with ``cu``; rows outside every sequence are left as they are (``out``) or undefined."""
+        if out is None:
+            n = table.shape[0] if cu is None and rows is None else rows
+            if n is None:
+                raise ValueError("rows: how many the offsets of cu cover")
+            with torch.cuda.stream(self.ctx.stream):
+                out = tuple(torch.empty(n, self.heads, self.head_dim, dtype=dtype, device=self.k.device)
+                            for _ in range(2))
+        k, v = out
+        if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
+            raise ValueError("out: as many rows of the same type")
+        pk, kr, kh = self._rows("out[0]", k, self.heads)
+        pv, vr, vh = self._rows("out[1]", v, self.heads)
+        b = self._batch(table, kv_len, cu, k.shape[0], 0)
+        check(L.lib().hf_kv_read(self.ctx.handle, C.byref(self._c), C.byref(b), pk, pv, kr, kh, vr, vh,
+                                 _DTYPES[k.dtype]), "hf_kv_read")
+        return k, v
+
+    def attend(self, q: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor,
+               cu: Optional[torch.Tensor] = None, max_q: int = 1, mask: Optional[torch.Tensor] = None,
+               scale: Optional[float] = None, lse: bool = False, out: Optional[torch.Tensor] = None):
+        """``hf_kv_attend``: attention of rows ``q`` [rows, query heads, head_dim] (bf16 or fp16),
+        whose keys and values are in the cache already, over their sequences.  ``max_q``: rows a
+        sequence has at most (host knowledge; with ``cu``).  ``mask``: int32 [rows, words], bit j of
+        a row: it sees row j of its sequence (a tree's ancestors); None: causal.  ``scale``: default
+        1 / sqrt(head_dim).  Returns the outputs, with ``lse`` (outputs, fp32 [rows, query heads]
+        logarithms of the softmax sums)."""
+        if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % self.heads or q.dtype == torch.float32:
+            raise ValueError(f"q: [rows, a multiple of {self.heads}, {self.head_dim}], bf16 or fp16")
+        rows, heads = q.shape[0], q.shape[1]
+        pq, qr, qh = self._rows("q", q, heads)
+        b = self._batch(table, kv_len, cu, rows, max_q if cu is not None else 1)
+        ctx, words = self.ctx, 0
+        if mask is not None:
+            if self._ints("mask", mask, 2).shape[0] != rows or not mask.is_contiguous():
+                raise ValueError("mask: contiguous int32 [rows, words]")
+            words = mask.shape[1]
+        with torch.cuda.stream(ctx.stream):
+            if out is None:
+                out = torch.empty(rows, heads, self.head_dim, dtype=q.dtype, device=q.device)
+            elif out.shape != q.shape or out.dtype != q.dtype:
+                raise ValueError("out: the shape and type of q")
+            sums = torch.empty(rows, heads, dtype=torch.float32, device=q.device) if lse else None
+            need = L.lib().hf_kv_attend_work_bytes(ctx.handle, C.byref(self._c), C.byref(b), heads)
+            # taken from torch's allocator for this call: another stream's call, or a captured
+            # graph, has its own
+            work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        po, orow, oh = self._rows("out", out, heads)
+        query = L.hf_kv_query(pq, po, sums.data_ptr() if lse else 0, mask.data_ptr() if mask is not None else 0,
+                              qr, qh, orow, oh, heads, words, _DTYPES[q.dtype],
+                              self.head_dim ** -0.5 if scale is None else scale)
+        check(L.lib().hf_kv_attend(ctx.handle, C.byref(self._c), C.byref(b), C.byref(query),
+                                   work.data_ptr() if need else None, need), "hf_kv_attend")
+        return (out, sums) if lse else out
+
+    def keep(self, table: torch.Tensor, kv_len: torch.Tensor, cu: Optional[torch.Tensor],
+             path: torch.Tensor, path_len: torch.Tensor, rows: Optional[int] = None,
+             new_len: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``hf_kv_keep``: of the sequences' last rows (drafts), keep those that ``path`` int32
+        [batch, width] names in ascending order, ``path_len`` int32 [batch] of them; returns the
+        sequences' new lengths.  ``rows``: rows that ``cu`` covers (default: any number)."""
+        self._ints("path", path, 2)
+        self._ints("path_len", path_len, 1)
+        batch = table.shape[0]
+        if path.shape[0] != batch or path_len.shape[0] != batch:
+            raise ValueError("path and path_len: one row for each sequence")
+        b = self._batch(table, kv_len, cu, batch if cu is None else 0x7FFFFFFF if rows is None else rows, 0)
+        if new_len is None:
+            with torch.cuda.stream(self.ctx.stream):
+                new_len = torch.empty(batch, dtype=torch.int32, device=self.k.device)
+        elif self._ints("new_len", new_len, 1).shape[0] != batch:
+            raise ValueError("new_len: one length for each sequence")
+        check(L.lib().hf_kv_keep(self.ctx.handle, C.byref(self._c), C.byref(b), path.data_ptr(),
+                                 path.stride(0) if batch > 1 else path.shape[1], path.shape[1],
+                                 path_len.data_ptr(), new_len.data_ptr()), "hf_kv_keep")
+        return new_len

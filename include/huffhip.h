@@ -564,6 +564,128 @@ int hf_container_open(hf_ctx* ctx, const void* d_blob, uint64_t blob_bytes,
 int hf_container_codebook(hf_ctx* ctx, const void* d_blob, const hf_container_info* info,
                           void* d_codebook_out);
 
+/* ---- quantised KV cache -----------------------------------------------------------------------
+ * The reference names FP16, FP8 and FP4 operands of LLM inference (reports/spec.md:22) and codes
+ * bytes; it has nothing that makes such bytes from keys and values or uses them.  These calls are
+ * both sides of the page coder (hf_encode_pages / hf_decode_pages with d_out_slots decode straight
+ * into a pool): rows are quantised as they are written into pages, read back, and attended to.
+ *
+ * A cache is two page pools, keys and values, of codes [n_pages][page_size][heads][head_dim] with
+ * any page, token and head stride (in bytes, the same for both; head_dim is contiguous), so a pool
+ * of fp8 pages whose strides are dense is also a run of HF_CHUNK_SYMS-symbol pages for the coder.
+ * The 8- and 4-bit formats have two pools of scale bytes [n_pages][heads][head_dim / group]
+ * [page_size], dense: byte e scales the `group` consecutive elements of a row by 2^(e - 127), 255
+ * is NaN.  HF_KV_FP4_E2M1 holds elements 2i and 2i + 1 in the low and high half of byte i.
+ *
+ * Sequence b owns the pages d_table[b][0 ..]; position t of it is token t % page_size of page
+ * t / page_size.  It has d_kv_len[b] tokens, and rows d_cu_rows[b] .. d_cu_rows[b + 1] - 1 of a
+ * call's row tensors are its LAST rows: a row's position is kv_len - (rows of the sequence) + i.
+ * d_cu_rows NULL: one row per sequence (rows = batch).  Rows in front of the first sequence and
+ * behind the last are left as they are.  These lists stay on the device, so a captured call
+ * follows their contents; lists that do not fit the call (offsets that fall or leave the row
+ * tensors, a sequence of more rows than tokens, or than max_rows in hf_kv_attend, more tokens than
+ * the table's row holds, a page number >= n_pages where a page is needed) are reported as
+ * HF_ERR_CORRUPT by the next call that synchronises (hf_sync); memory outside the buffers is
+ * neither read nor written, and what such a sequence's rows hold afterwards is not defined.
+ * A page may belong to several sequences (a shared prefix) as long as no call writes it for two.
+ *
+ * All calls only enqueue work, allocate nothing and can be captured.  Row tensors are 16-byte
+ * aligned with strides in elements that are multiples of 8 (fp32: of 4); pools, scales and byte
+ * strides are 16-byte aligned (HF_ERR_ALIGN).  heads <= 1024, 32 <= head_dim <= 256 in steps of 32,
+ * group a power of two from 32 that divides head_dim, page_size a power of two in 8 .. 65536
+ * (HF_ERR_ARG). */
+#define HF_KV_BF16 0
+#define HF_KV_FP16 1
+#define HF_KV_FP8_E4M3 2
+#define HF_KV_FP8_E5M2 3
+#define HF_KV_FP4_E2M1 4
+/* element types of row tensors */
+#define HF_DT_BF16 0
+#define HF_DT_FP16 1
+#define HF_DT_FP32 2
+
+typedef struct hf_kv_cache {
+    void* d_k;
+    void* d_v;
+    uint8_t* d_k_scale; /* NULL for HF_KV_BF16 / HF_KV_FP16 */
+    uint8_t* d_v_scale;
+    uint64_t n_pages;
+    int64_t page_stride; /* bytes, each at least a row of codes */
+    int64_t token_stride;
+    int64_t head_stride;
+    uint32_t page_size;
+    uint32_t heads;
+    uint32_t head_dim;
+    uint32_t group; /* not used for the 16-bit formats */
+    uint32_t format; /* HF_KV_* */
+    uint32_t reserved;
+} hf_kv_cache;
+
+typedef struct hf_kv_batch {
+    const int32_t* d_cu_rows; /* [batch + 1], or NULL */
+    const int32_t* d_kv_len;  /* [batch] */
+    const int32_t* d_table;   /* [batch][table_width], rows table_stride entries apart */
+    int64_t table_stride;
+    uint32_t table_width;
+    uint32_t batch;
+    uint32_t rows;     /* rows of the row tensors */
+    uint32_t max_rows; /* hf_kv_attend: rows of a sequence, at most (a larger bound costs speed) */
+} hf_kv_batch;
+
+/* Quantises the rows d_k, d_v [rows][heads][head_dim] into their places.  A group's scale exponent
+ * is the least e >= -126 for which the largest finite magnitude of the group is at most the
+ * format's largest value (448, 57344, 6) times 2^e, and 0 for a group of zeros; a code is x * 2^-e
+ * rounded to nearest even.  Infinities take the largest code of their sign; NaN stays NaN (e2m1:
+ * the group's scale byte is 255 and reads back as NaN).  A 16-bit cache takes rows of its own type
+ * (kept bit for bit) or fp32 (rounded). */
+int hf_kv_write(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch, const void* d_k,
+                const void* d_v, int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                int64_t v_head_stride, int dtype);
+/* The last rows of the sequences out of the cache, code * 2^(e - 127) rounded to dtype (a whole
+ * sequence: as many rows as it has tokens).  A 16-bit cache gives its own type or fp32. */
+int hf_kv_read(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch, void* d_k, void* d_v,
+               int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+               int64_t v_head_stride, int dtype);
+
+/* Attention of the sequences' last rows (which hf_kv_write has put into the cache) over everything
+ * in front of them and over those of themselves that the mask names:
+ *   o_i = sum_t p_it v_t / sum_t p_it,  p_it = exp(scale q_i . k_t), t < kv_len - n or draft bit set
+ * d_mask [rows][mask_words] (32 mask_words >= max_rows): bit j % 32 of word j / 32 of a row says
+ * whether it sees row j of its own sequence -- the ancestors, itself among them, of a node in a
+ * tree of drafted tokens, stored in any order.  NULL: rows 0 .. i (causal).  A row that sees nothing
+ * gives zeros and d_lse = -inf; what a row does not see does not reach it, infinities and NaN
+ * included.  Query heads h * (q_heads / heads) .. belong to cache head h.  d_lse [rows][q_heads]
+ * (optional) = log sum_t p_it.  Sums and statistics are held in 32 bits; p is rounded to the type of
+ * the queries in front of the second product.  fp16 queries take the cache's values as hf_kv_read
+ * gives them in fp16.  dtype is HF_DT_BF16 or HF_DT_FP16 and a 16-bit cache's own type.  d_work:
+ * hf_kv_attend_work_bytes bytes, 16-byte aligned, of no other call in flight (may be NULL if 0). */
+typedef struct hf_kv_query {
+    const void* d_q;
+    void* d_out;
+    float* d_lse;
+    const uint32_t* d_mask;
+    int64_t q_row_stride; /* elements */
+    int64_t q_head_stride;
+    int64_t out_row_stride;
+    int64_t out_head_stride;
+    uint32_t q_heads; /* a multiple of heads */
+    uint32_t mask_words;
+    uint32_t dtype;
+    float scale; /* finite, above 0 */
+} hf_kv_query;
+uint64_t hf_kv_attend_work_bytes(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
+                                 uint32_t q_heads);
+int hf_kv_attend(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
+                 const hf_kv_query* query, void* d_work, uint64_t work_bytes);
+/* After a tree of drafts is judged: rows d_path[b][0 .. d_path_len[b] - 1] (ascending numbers of
+ * the sequence's last rows) move, codes and scales, to the first places behind the tokens in front
+ * of the drafts, and d_new_len[b] (not d_kv_len itself) = those tokens + d_path_len[b].  A path that
+ * does not ascend or leaves the sequence's rows is reported as HF_ERR_CORRUPT, moves nothing and
+ * gives d_new_len = d_kv_len. */
+int hf_kv_keep(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
+               const int32_t* d_path, int64_t path_stride, uint32_t path_width,
+               const int32_t* d_path_len, int32_t* d_new_len);
+
 /* ---- TreeQualityAnalyzer (tree_q_analyser.scala:10-47) ------------------------------------- */
 int hf_quality(hf_ctx* ctx, const uint64_t* h_freq, const uint8_t* h_len, int N, int wt_width,
                uint16_t* avg_len_q8, uint16_t* efficiency, uint16_t* compression_ratio);
