@@ -1595,22 +1595,25 @@ int kv_move(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch, con
             bool write) {
     hf_kv_pools p;
     hf_kv_seqs s;
-    hf_kv_rows k, v;
-    if (!ctx) return HF_ERR_ARG;
+    hf_kv_rows k = {nullptr, 0, 0}, v = {nullptr, 0, 0};
     if (int rc = kv_check_cache(cache, &p)) return rc;
     if (int rc = kv_check_batch(batch, &s)) return rc;
     if (dtype < HF_DT_BF16 || dtype > HF_DT_FP32) return HF_ERR_ARG;
     if ((cache->format == HF_KV_BF16 && dtype == HF_DT_FP16) ||
         (cache->format == HF_KV_FP16 && dtype == HF_DT_BF16))
         return HF_ERR_ARG;
-    if (s.rows == 0 || s.batch == 0) return HF_OK;
+    const bool none = s.rows == 0 || s.batch == 0;
     const int elem = dtype == HF_DT_FP32 ? 4 : 2;
-    if (int rc = kv_check_rows(d_k, k_row, k_head, elem, &k)) return rc;
-    if (int rc = kv_check_rows(d_v, v_row, v_head, elem, &v)) return rc;
+    if (!none) {
+        if (int rc = kv_check_rows(d_k, k_row, k_head, elem, &k)) return rc;
+        if (int rc = kv_check_rows(d_v, v_row, v_head, elem, &v)) return rc;
+    }
     // (rows that are written must not lie on one another)
     const int64_t row = p.head_dim;
     if (!write && ((p.heads > 1 && (k_head < row || v_head < row)) || (s.rows > 1 && (k_row < row || v_row < row))))
         return HF_ERR_ARG;
+    if (!ctx) return HF_ERR_ARG;
+    if (none) return HF_OK;
     HF_USE_DEVICE(ctx);
     tic(ctx);
     if (write) hf_launch_kv_write(p, s, k, v, dtype, (int)cache->format, ctx->d_ctl + 1, ctx->num_cu, ctx->stream);
@@ -1645,13 +1648,12 @@ int kv_plan_of(const hf_ctx* ctx, const hf_kv_pools& p, const hf_kv_seqs& s, uin
     o->units = (uint32_t)units;
     const uint64_t pad = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
     o->part_floats = o->join ? units * (uint64_t)o->tile_rows * pad : 0;
-    o->bytes = o->join ? 4 * o->part_floats + 8 * units * (uint64_t)o->tile_rows : 0;
+    o->bytes = o->join ? 4 * o->part_floats + 16 * units * (uint64_t)o->tile_rows : 0;
     return HF_OK;
 }
 
-int kv_check_attend(const hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
-                    uint32_t q_heads, hf_kv_pools* p, hf_kv_seqs* s, uint32_t* per) {
-    if (!ctx) return HF_ERR_ARG;
+int kv_check_attend(const hf_kv_cache* cache, const hf_kv_batch* batch, uint32_t q_heads,
+                    hf_kv_pools* p, hf_kv_seqs* s, uint32_t* per) {
     if (int rc = kv_check_cache(cache, p)) return rc;
     if (int rc = kv_check_batch(batch, s)) return rc;
     if (q_heads == 0 || q_heads % p->heads || q_heads > 65536) return HF_ERR_ARG;
@@ -1688,7 +1690,7 @@ uint64_t hf_kv_attend_work_bytes(hf_ctx* ctx, const hf_kv_cache* cache, const hf
     hf_kv_seqs s;
     uint32_t per;
     kv_plan plan;
-    if (kv_check_attend(ctx, cache, batch, q_heads, &p, &s, &per)) return 0;
+    if (!ctx || kv_check_attend(cache, batch, q_heads, &p, &s, &per)) return 0;
     if (s.rows == 0 || s.batch == 0 || kv_plan_of(ctx, p, s, per, &plan)) return 0;
     return plan.bytes;
 }
@@ -1698,17 +1700,18 @@ int hf_kv_attend(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch
     hf_kv_attend_args a;
     kv_plan plan;
     if (!query) return HF_ERR_ARG;
-    if (int rc = kv_check_attend(ctx, cache, batch, query->q_heads, &a.c, &a.s, &a.per)) return rc;
+    if (int rc = kv_check_attend(cache, batch, query->q_heads, &a.c, &a.s, &a.per)) return rc;
     if (query->dtype > HF_DT_FP16) return HF_ERR_ARG;
     if (cache->format <= HF_KV_FP16 && query->dtype != cache->format) return HF_ERR_ARG;
     if (!(query->scale > 0.0f) || query->scale > 3.0e38f) return HF_ERR_ARG;
-    if (a.s.rows == 0 || a.s.batch == 0) return HF_OK;
+    if (a.s.rows == 0 || a.s.batch == 0) return ctx ? HF_OK : HF_ERR_ARG;
     if (query->d_mask && (uint64_t)query->mask_words * 32u < a.s.most) return HF_ERR_ARG;
     if (int rc = kv_check_rows(query->d_q, query->q_row_stride, query->q_head_stride, 2, &a.q)) return rc;
     if (int rc = kv_check_rows(query->d_out, query->out_row_stride, query->out_head_stride, 2, &a.out)) return rc;
     const int64_t row = a.c.head_dim;
     if ((query->q_heads > 1 && query->out_head_stride < row) || (a.s.rows > 1 && query->out_row_stride < row))
         return HF_ERR_ARG;
+    if (!ctx) return HF_ERR_ARG;
     if (int rc = kv_plan_of(ctx, a.c, a.s, a.per, &plan)) return rc;
     if (plan.bytes > work_bytes || (plan.bytes && !d_work)) return HF_ERR_ARG;
     if (!aligned16(d_work)) return HF_ERR_ALIGN;
@@ -1737,12 +1740,13 @@ int hf_kv_keep(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
                const int32_t* d_path_len, int32_t* d_new_len) {
     hf_kv_pools p;
     hf_kv_seqs s;
-    if (!ctx) return HF_ERR_ARG;
     if (int rc = kv_check_cache(cache, &p)) return rc;
     if (int rc = kv_check_batch(batch, &s)) return rc;
+    if (s.batch && (!d_path_len || !d_new_len || d_new_len == s.kv_len)) return HF_ERR_ARG;
+    if (s.batch && ((path_width && !d_path) || path_stride < path_width)) return HF_ERR_ARG;
+    if (path_stride > (1ll << 31)) return HF_ERR_RANGE;
+    if (!ctx) return HF_ERR_ARG;
     if (s.batch == 0) return HF_OK;
-    if (!d_path_len || !d_new_len || d_new_len == s.kv_len) return HF_ERR_ARG;
-    if ((path_width && !d_path) || path_stride < path_width || path_stride > (1ll << 31)) return HF_ERR_ARG;
     HF_USE_DEVICE(ctx);
     tic(ctx);
     hf_launch_kv_keep(p, s, d_path, path_stride, path_width, d_path_len, d_new_len,

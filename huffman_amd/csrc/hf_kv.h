@@ -51,7 +51,7 @@ struct hf_kv_attend_args {
     uint32_t per;          // query heads per cache head
     float scale_log2;      // softmax scale x log2(e)
     float* part;           // partial outputs of the units, [units][rows of a tile][padded head_dim]
-    float* part_ml;        // their maxima and sums, [units][rows of a tile][2]
+    float* part_ml;        // their maxima and two sums, [units][rows of a tile][4]
     uint32_t target;       // units the call is cut into, about
     uint32_t min_steps;    // tokens / 32 a unit has at least
     uint32_t units;        // workgroups of the call, and room of the partial buffers
@@ -83,8 +83,8 @@ struct hf_kv_seq {
     int32_t row0, n, past, len;
     bool bad;
 };
-__device__ __forceinline__ hf_kv_seq hf_kv_sequence(const hf_kv_seqs& s, const uint32_t b,
-                                                    const uint32_t page_shift) {
+__host__ __device__ __forceinline__ hf_kv_seq hf_kv_sequence(const hf_kv_seqs& s, const uint32_t b,
+                                                             const uint32_t page_shift) {
     hf_kv_seq q;
     int32_t lo = (int32_t)b, hi = (int32_t)b + 1;
     if (s.cu) {
@@ -93,8 +93,8 @@ __device__ __forceinline__ hf_kv_seq hf_kv_sequence(const hf_kv_seqs& s, const u
     }
     q.len = s.kv_len[b];
     q.row0 = lo;
-    q.n = hi - lo;
-    q.past = q.len - q.n;
+    q.n = (int32_t)((uint32_t)hi - (uint32_t)lo);  // (may wrap: such lists are bad)
+    q.past = (int32_t)((uint32_t)q.len - (uint32_t)q.n);
     q.bad = lo < 0 || hi < lo || (uint32_t)hi > s.rows || (uint32_t)q.n > s.most || q.len < q.n ||
             (uint64_t)(uint32_t)q.len > ((uint64_t)s.width << page_shift);
     if (q.bad) {

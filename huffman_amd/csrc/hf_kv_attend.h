@@ -19,7 +19,10 @@
 // Codes become 16-bit operands with the conversions that apply a power-of-two scale for nothing, so
 // scales may differ by token and by group of d.  The sums of S and O and the statistics are kept in
 // 32 bits; p is rounded to the type of the queries for the second product, as the codes' values are
-// exact in it (fp16: unless they leave its range, as reading the cache in fp16 would).
+// exact in it (fp16: unless they leave its range, as reading the cache in fp16 would).  O is divided
+// by the sum of the p as rounded, one more product, with ones: what rounding p does to the weights
+// then cancels where few tokens carry a row (a row of one token gives that token's values exactly).
+// The logarithm of the sum is taken from the p in 32 bits.
 #pragma once
 
 #include "hf_kv.h"
@@ -220,7 +223,8 @@ struct kv_unit {
     const hf_gi32* table;
     uint32_t groups_of_page;  // groups of eight tokens the table has pages for
     f32x4 acc[R][VD];
-    float mx[R], sum[R];
+    f32x4 div[R];         // sums of the rounded p (all four alike)
+    float mx[R], sum[R];  // largest score (unscaled); the lane's share of the sum of p
     hf_u32x4 qr[R][KS];
     uint32_t bad;
 
@@ -250,6 +254,7 @@ struct kv_unit {
             }
             mx[r] = -3.402823466e38f;
             sum[r] = 0.0f;
+            div[r] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int c = 0; c < VD; ++c) acc[r][c] = f32x4{0, 0, 0, 0};
         }
@@ -440,16 +445,16 @@ struct kv_unit {
             top[r] = s[r][0][0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) top[r] = fmaxf(top[r], s[r][e / 4][e % 4]);
-            top[r] *= a.scale_log2;
-            up = up || top[r] > mx[r] + (T::off + T::rise);
+            up = up || (top[r] - mx[r]) * a.scale_log2 > T::rise;
         }
         if (__ballot(up)) {  // seldom after the first step: sums and outputs to a new maximum
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const float was = mx[r];
-                mx[r] = fmaxf(was, kv_row_max(top[r]) - T::off);
-                const float f = __builtin_amdgcn_exp2f(was - mx[r]);
+                mx[r] = fmaxf(was, kv_row_max(top[r]));
+                const float f = __builtin_amdgcn_exp2f((was - mx[r]) * a.scale_log2);
                 sum[r] *= f;
+                div[r] *= f;
 #pragma unroll
                 for (int c = 0; c < VD; ++c) acc[r][c] *= f;
             }
@@ -460,11 +465,17 @@ struct kv_unit {
             float e[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i / 4][i % 4], a.scale_log2, -mx[r]));
+                // (the difference first: it is exact near the maximum, however large the scores)
+                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i / 4][i % 4] - mx[r], a.scale_log2, T::off));
                 sum[r] += e[i];
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) p[r][i] = T::pack(e[2 * i], e[2 * i + 1]);
+        }
+        {
+            constexpr uint32_t two = T::one | T::one << 16;
+#pragma unroll
+            for (int r = 0; r < R; ++r) div[r] = T::mma(hf_u32x4{two, two, two, two}, p[r], div[r]);
         }
         hf_u32x4 av[VD];
         uint32_t there = 0xFFu;
@@ -530,11 +541,17 @@ struct kv_unit {
     }
 };
 
+// Logarithm of the sum of exp(scale s), from the largest s and the sum of p.
+template <typename T>
+__device__ __forceinline__ float kv_lse(const hf_kv_attend_args& a, const float top, const float sum) {
+    return 0.6931471805599453f * (__builtin_fmaf(top, a.scale_log2, -T::off) + __builtin_amdgcn_logf(sum));
+}
+
 // Scratch of a workgroup: what two wavefronts hand to the other two.
 template <int DP, int R>
 struct kv_lds {
     f32x4 acc[2][R][DP / 16][64];
-    float mx[2][R][64], sum[2][R][64];
+    float mx[2][R][64], sum[2][R][64], div[2][R][64];
 };
 
 template <int QT, int FMT, int DP, int R>
@@ -601,6 +618,7 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
             for (int r = 0; r < R; ++r) {
                 lds.mx[wave - half][r][u.lane] = u.mx[r];
                 lds.sum[wave - half][r][u.lane] = u.sum[r];
+                lds.div[wave - half][r][u.lane] = u.div[r][0];
 #pragma unroll
                 for (int c = 0; c < U::VD; ++c) lds.acc[wave - half][r][c][u.lane] = u.acc[r][c];
             }
@@ -611,9 +629,11 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
             for (int r = 0; r < R; ++r) {
                 const float om = lds.mx[wave][r][u.lane];
                 const float top = fmaxf(u.mx[r], om);
-                const float f = __builtin_amdgcn_exp2f(u.mx[r] - top), h = __builtin_amdgcn_exp2f(om - top);
+                const float f = __builtin_amdgcn_exp2f((u.mx[r] - top) * a.scale_log2);
+                const float h = __builtin_amdgcn_exp2f((om - top) * a.scale_log2);
                 u.mx[r] = top;
                 u.sum[r] = u.sum[r] * f + lds.sum[wave][r][u.lane] * h;
+                u.div[r][0] = u.div[r][0] * f + lds.div[wave][r][u.lane] * h;
 #pragma unroll
                 for (int c = 0; c < U::VD; ++c) u.acc[r][c] = u.acc[r][c] * f + lds.acc[wave][r][c][u.lane] * h;
             }
@@ -634,13 +654,13 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
                     *(f32x4*)(dst + U::VD * (4 * u.g + e) + c) =
                         f32x4{u.acc[r][c][e], u.acc[r][c + 1][e], u.acc[r][c + 2][e], u.acc[r][c + 3][e]};
             if (u.g == 0) {
-                a.part_ml[2 * row] = u.mx[r];
-                a.part_ml[2 * row + 1] = u.sum[r];
+                *(f32x4*)(a.part_ml + 4 * row) = f32x4{u.mx[r], u.sum[r], u.div[r][0], 0.0f};
             }
         } else if (i < rows) {
             const int32_t tok = i / (int32_t)a.per, hq = i % (int32_t)a.per;
             const uint32_t out_head = u.head * a.per + hq;
-            const float l = u.sum[r], f = l == 0.0f ? 0.0f : 1.0f / l;  // no token seen: zeros
+            const float l = u.sum[r], w = u.div[r][0];
+            const float f = w == 0.0f ? 0.0f : 1.0f / w;  // no token seen: zeros
             hf_g8* dst = (hf_g8*)a.out.p + ((int64_t)(u.q.row0 + tok) * a.out.row_stride +
                                             (int64_t)out_head * a.out.head_stride) * 2;
 #pragma unroll
@@ -656,7 +676,7 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
             }
             if (a.lse && u.g == 0)
                 a.lse[(int64_t)(u.q.row0 + tok) * a.c.heads * a.per + out_head] =
-                    l == 0.0f ? -__builtin_inff() : 0.6931471805599453f * (u.mx[r] + __builtin_amdgcn_logf(l));
+                    l == 0.0f ? -__builtin_inff() : kv_lse<typename U::T>(a, u.mx[r], l);
         }
     }
 }
@@ -718,25 +738,28 @@ __global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a) {
     const int64_t jump = (int64_t)tiles * tile_rows;
     const uint32_t col = (uint32_t)hf_lane() % cols, part = (uint32_t)hf_lane() / cols;
     float top = -3.402823466e38f;
-    for (uint32_t s = hf_lane(); s < ranges; s += 64) top = fmaxf(top, a.part_ml[2 * (first + s * jump)]);
+    for (uint32_t s = hf_lane(); s < ranges; s += 64) top = fmaxf(top, a.part_ml[4 * (first + s * jump)]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     f32x4 acc = {0, 0, 0, 0};
-    float sum = 0.0f;
+    float sum = 0.0f, div = 0.0f;
 #pragma unroll 4
     for (uint32_t s = part; s < ranges; s += deal) {
         const int64_t at = first + s * jump;
-        const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - top);
-        sum += w * a.part_ml[2 * at + 1];
+        const f32x4 ml = *(const f32x4*)(a.part_ml + 4 * at);
+        const float w = __builtin_amdgcn_exp2f((ml[0] - top) * a.scale_log2);
+        sum += w * ml[1];
+        div += w * ml[2];
         acc += w * *(const f32x4*)(a.part + at * DP + 4 * col);
     }
 #pragma unroll
     for (int o = cols; o < 64; o <<= 1) {
         sum += __shfl_xor(sum, o);
+        div += __shfl_xor(div, o);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
     }
-    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float f = div == 0.0f ? 0.0f : 1.0f / div;
     if (part == 0 && 4 * col < a.c.head_dim) {
         hf_g8* dst = (hf_g8*)a.out.p + ((int64_t)row * a.out.row_stride + (int64_t)out_head * a.out.head_stride) * 2;
         *(hf_gmem_u32x2*)(dst + 8 * col) =
@@ -744,7 +767,7 @@ __global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a) {
     }
     if (a.lse && hf_lane() == 0)
         a.lse[(int64_t)row * q_heads + out_head] =
-            sum == 0.0f ? -__builtin_inff() : 0.6931471805599453f * (top + __builtin_amdgcn_logf(sum));
+            sum == 0.0f ? -__builtin_inff() : kv_lse<T>(a, top, sum);
 }
 
 template <int QT, int FMT, int DP, int R>

@@ -189,6 +189,8 @@ class KvCache(_Module):
             if self._ints("mask", mask, 2).shape[0] != rows or not mask.is_contiguous():
                 raise ValueError("mask: contiguous int32 [rows, words]")
             words = mask.shape[1]
+            if 32 * words < min(b.max_rows, rows):
+                raise ValueError("mask: a bit for each of the max_q rows of a sequence")
         with torch.cuda.stream(ctx.stream):
             if out is None:
                 out = torch.empty(rows, heads, self.head_dim, dtype=q.dtype, device=q.device)

@@ -1,0 +1,661 @@
+"""GPU suite of the quantised KV cache against its definitions in 64 bits (tests/kv_reference.py)."""
+import numpy as np
+import pytest
+import torch
+
+from tests import kv_reference as R
+
+pytestmark = pytest.mark.gpu
+
+NAMES = {"bf16": R.BF16, "fp16": R.FP16, "e4m3": R.E4M3, "e5m2": R.E5M2, "e2m1": R.E2M1}
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+@pytest.fixture()
+def kv(hf):
+    from huffman_amd import kv as m
+    return m
+
+
+def make(kv, fmt, pages, page, heads, dim, group=None, order="thd", ctx=None):
+    """A cache with its pools in token-major or head-major order, filled with codes that a write never
+    leaves (NaN, or 16-bit NaN), so that whatever reads outside its rows shows."""
+    f = NAMES[fmt]
+    c = kv.KvCache.empty(pages, page, heads, dim, f, group, ctx=ctx)
+    fill = float("nan") if f in R.TORCH else 0x7F
+    if order == "hdt":  # [pages, heads, page, dim] in memory
+        k, v = (torch.empty(pages, heads, page, c.k.shape[3], dtype=c.k.dtype, device="cuda").transpose(1, 2)
+                for _ in range(2))
+        c = kv.KvCache(k, v, c.k_scale, c.v_scale, fmt=f, ctx=ctx)
+    c.k.fill_(fill)
+    c.v.fill_(fill)
+    return c
+
+
+def layout(rng, new, past, page, width=None, spare=3):
+    """Table (shuffled pages), lengths and row offsets of sequences; spare pages belong to nobody."""
+    total = np.array(new) + np.array(past)
+    need = -(-total // page)
+    count = int(need.sum()) + spare
+    order = rng.permutation(count)
+    table = np.full((len(new), width or max(1, int(need.max()))), -7, np.int32)  # unused entries lead nowhere
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += int(n)
+    cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    return table, total.astype(np.int32), cu, count
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def rows_of(rng, n, heads, dim, dtype, spread=1.0):
+    x = rng.standard_normal((n, heads, dim)) * np.exp(0.8 * rng.standard_normal((heads, dim))) * spread
+    return torch.from_numpy(x.astype(np.float32)).to(DT[dtype])
+
+
+def written(c, f):
+    return R.pool_values(c.k, c.k_scale, f), R.pool_values(c.v, c.v_scale, f)
+
+
+# ---- write and read -----------------------------------------------------------------------------
+SHAPES = [  # new, past, page, heads, dim, group, order
+    ([1], [0], 8, 1, 32, 32, "thd"),
+    ([1, 1, 1], [0, 7, 8], 8, 8, 128, 128, "thd"),
+    ([5, 0, 33], [3, 2, 95], 16, 3, 96, 32, "hdt"),
+    ([17, 70], [0, 61], 32, 2, 256, 64, "thd"),
+    ([130], [1], 64, 4, 64, 64, "hdt"),
+    ([3, 9], [40, 0], 16, 1, 256, 256, "thd"),
+    ([2, 1], [5, 6], 8, 5, 224, 32, "thd"),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("fmt", list(NAMES))
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_write_and_read(kv, fmt, dtype, shape):
+    f = NAMES[fmt]
+    if f in R.TORCH and dtype not in (fmt, "fp32"):
+        pytest.skip("a 16-bit cache takes its own type or fp32")
+    new, past, page, heads, dim, group, order = SHAPES[shape]
+    rng = np.random.default_rng(shape)
+    table, kv_len, cu, count = layout(rng, new, past, page)
+    c = make(kv, fmt, count, page, heads, dim, group, order)
+    n = int(cu[-1])
+    k, v = rows_of(rng, n + 2, heads, dim, dtype), rows_of(rng, n + 2, heads, dim, dtype)
+    if dtype != "fp16":
+        k[0, 0, :4] = torch.tensor([1e-40, -1e-39, 3e-38, 0.0]).to(k.dtype)
+    k[0, 0, -32:] = 0  # a group of zeros; v's first row: -0.0 and one value alone
+    v[0, 0] = -0.0
+    v[0, 0, 1] = 0.1
+    before = [t.clone() for t in (c.k, c.v) + (() if c.k_scale is None else (c.k_scale, c.v_scale))]
+    # (two rows behind the last sequence belong to nobody)
+    c.write(k.cuda(), v.cuda(), dev(table), dev(kv_len), dev(cu))
+    c.ctx.sync()
+    pages, offs = [], []
+    for b in range(len(new)):
+        pos = past[b] + np.arange(new[b])
+        pages.append(table[b][pos // page])
+        offs.append(pos % page)
+    pg, of = np.concatenate(pages), np.concatenate(offs)
+    touched = torch.zeros(count, page, dtype=torch.bool)
+    touched[pg, of] = True
+    for rows, pool, scales, i in ((k, c.k, c.k_scale, 0), (v, c.v, c.v_scale, 1)):
+        x = rows[:n].double().numpy()
+        if f in R.TORCH:
+            want = rows[:n].to(R.TORCH[f]).cuda()
+            assert torch.equal(pool[dev(pg), dev(of)].view(torch.int16), want.view(torch.int16))
+        else:
+            code, scale = R.quantise(x, f, group)
+            assert np.array_equal(scales.cpu().numpy()[pg, :, :, of], scale)
+            assert np.array_equal(R.unpack(pool, f)[pg, of], code)
+            assert torch.equal(scales.permute(0, 3, 1, 2)[~touched.cuda()], before[2 + i].permute(0, 3, 1, 2)[~touched.cuda()])
+        assert torch.equal(pool[~touched.cuda()].view(torch.uint8), before[i][~touched.cuda()].view(torch.uint8))
+    # and back, in every type the cache gives
+    for out in ("bf16", "fp16", "fp32"):
+        if f in R.TORCH and out not in (fmt, "fp32"):
+            continue
+        gk, gv = torch.full((2, n + 2, heads, dim), 7.0, dtype=DT[out], device="cuda")
+        c.read(dev(table), dev(kv_len), dev(cu), out=(gk, gv))
+        c.ctx.sync()
+        for got, values in ((gk, written(c, f)[0]), (gv, written(c, f)[1])):
+            want = torch.from_numpy(values[pg, of]).to(DT[out])  # one rounding, torch's on the host
+            assert torch.equal(got[:n].cpu(), want)
+            assert (got[n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2", "e2m1"])
+def test_write_of_what_is_not_finite(kv, fmt, dtype):
+    f, dim = NAMES[fmt], 64
+    x = torch.randn(6, 1, dim, generator=torch.Generator().manual_seed(1)).to(DT[dtype])
+    x[0, 0, 3], x[0, 0, 40] = float("inf"), float("-inf")
+    x[1, 0, 5] = float("nan")
+    x[2] = float("inf")
+    x[3, 0, 33], x[3, 0, 34] = float("nan"), float("inf")
+    x[4] = torch.finfo(x.dtype).max
+    x[5] = -torch.finfo(x.dtype).tiny
+    c = make(kv, fmt, 1, 8, 1, dim, 32)
+    table, kv_len, cu = dev(np.zeros((1, 1), np.int32)), dev(np.array([6], np.int32)), dev(np.array([0, 6], np.int32))
+    c.write(x.cuda(), x.cuda(), table, kv_len, cu)
+    got = c.read(table, kv_len, cu, rows=6, dtype=torch.float32)
+    c.ctx.sync()
+    code, scale = R.quantise(x.double().numpy(), f, 32)
+    assert np.array_equal(c.k_scale.cpu().numpy()[0, :, :, :6].transpose(2, 0, 1), scale)
+    want = torch.from_numpy(R.dequantise(code, scale, f, 32)).float()
+    for t in got:
+        assert torch.equal(t.cpu().nan_to_num(nan=12345.0), want.nan_to_num(nan=12345.0))
+        assert torch.isnan(t[1]).any() and torch.isnan(t[3]).any() and not torch.isnan(t[[0, 2, 4, 5]]).any()
+
+
+def test_write_from_slices_and_many_sequences(kv):
+    """Keys and values as slices of one projection's output; more sequences than the offsets that a
+    workgroup holds, most with no rows."""
+    rng = np.random.default_rng(11)
+    batch = 1500
+    new = (rng.random(batch) < 0.3).astype(int) * rng.integers(1, 4, batch)
+    past = rng.integers(0, 9, batch)
+    table, kv_len, cu, count = layout(rng, new, past, 8)
+    n = int(cu[-1])
+    both = rows_of(rng, n, 6, 64, "bf16").cuda()
+    c = make(kv, "e4m3", count, 8, 2, 64, 32)
+    c.write(both[:, 2:4], both[:, 4:6], dev(table), dev(kv_len), dev(cu))
+    c.ctx.sync()
+    wide = torch.empty(n, 2, 2, 64, dtype=torch.float32, device="cuda")
+    c.read(dev(table), dev(kv_len), dev(cu), out=(wide[:, 0], wide[:, 1]))
+    c.ctx.sync()
+    for i, lo in ((0, 2), (1, 4)):
+        code, scale = R.quantise(both[:, lo:lo + 2].cpu().double().numpy(), R.E4M3, 32)
+        assert torch.equal(wide[:, i].cpu(), torch.from_numpy(R.dequantise(code, scale, R.E4M3, 32)).float())
+
+
+# ---- attention ----------------------------------------------------------------------------------
+def tree_mask(rng, new, words):
+    mask = np.zeros((sum(new), words), np.uint32)
+    at = 0
+    for n in new:
+        for i in range(n):
+            p = int(rng.integers(-1, i)) if i else -1
+            if p >= 0:
+                mask[at + i] = mask[at + p]
+            mask[at + i, i // 32] |= np.uint32(1 << (i % 32))
+        at += n
+    return mask
+
+
+ATTEND = [  # new, past, page, heads, per, dim, group, order, mask
+    ([1], [0], 16, 1, 1, 64, 64, "thd", None),
+    ([1, 1, 1, 1], [0, 31, 32, 700], 16, 2, 4, 128, 128, "thd", None),
+    ([1, 1], [1999, 100], 8, 1, 16, 64, 32, "hdt", None),
+    ([1], [530], 64, 2, 20, 128, 32, "thd", None),
+    ([40, 3, 0, 7], [0, 90, 5, 33], 16, 2, 3, 96, 32, "thd", None),
+    ([29], [260], 32, 1, 4, 128, 64, "thd", "tree"),
+    ([70, 64, 1], [45, 0, 200], 16, 1, 2, 64, 32, "hdt", "tree"),
+    ([5, 33], [0, 300], 8, 2, 1, 256, 64, "thd", "tree"),
+    ([13, 2], [77, 1], 16, 1, 5, 256, 256, "thd", None),
+    ([9], [600], 128, 2, 2, 32, 32, "thd", "any"),
+    ([50], [111], 16, 1, 8, 224, 32, "thd", "any"),
+    ([1] * 70, [i * 7 % 130 for i in range(70)], 8, 1, 2, 64, 64, "thd", None),
+]
+
+
+def attend_case(kv, fmt, dtype, new, past, page, heads, per, dim, group, order, kind, seed, ctx=None):
+    f = NAMES[fmt]
+    rng = np.random.default_rng(seed)
+    table, kv_len, cu, count = layout(rng, new, past, page)
+    c = make(kv, fmt, count, page, heads, dim, group, order, ctx)
+    # all rows of the sequences written in one call
+    total = int(kv_len.sum())
+    cut = np.concatenate([[0], np.cumsum(kv_len)]).astype(np.int32)
+    c.write(rows_of(rng, total, heads, dim, dtype).cuda(), rows_of(rng, total, heads, dim, dtype).cuda(),
+            dev(table), dev(kv_len), dev(cut))
+    q = rows_of(rng, int(cu[-1]), heads * per, dim, dtype, 0.7)
+    words = -(-max(max(new), 1) // 32)
+    mask = None if kind is None else tree_mask(rng, new, words) if kind == "tree" else \
+        rng.integers(0, 1 << 32, (int(cu[-1]), words), dtype=np.uint32)
+    return c, f, q, table, kv_len, cu, mask
+
+
+def verify(c, f, q, table, kv_len, cu, mask, got, lse, scale, dtype):
+    k, v = written(c, f)
+    out, ref_lse, weight = R.attend(q.double().numpy(), k, v, table, kv_len, cu, mask, scale)
+    kmax = max(float(np.abs(k[table[b][np.arange(kv_len[b]) // k.shape[1]], np.arange(kv_len[b]) % k.shape[1]]).max(initial=0))
+               for b in range(len(kv_len)))
+    tol = R.tolerance(out, weight, q.double().numpy(), kmax, int(kv_len.max()), scale, DT[dtype])
+    err = np.abs(got.cpu().double().numpy() - out)
+    assert (err <= tol).all(), (err - tol).max()
+    lse = lse.cpu().double().numpy()
+    none = np.isinf(ref_lse)
+    assert np.array_equal(np.isinf(lse), none) and (got.cpu().numpy() if dtype == "fp16" else got.float().cpu().numpy())[none].any() == False  # noqa: E712
+    # the logarithm's error is the weights' relative one: the exponents' error, the sum's, the logarithm's own
+    d = q.shape[-1]
+    bound = 1.5 * (d + 8) * 2.0 ** -24 * scale * np.abs(q.double().numpy()).sum(-1) * kmax + 2.0 ** -19 + \
+        int(kv_len.max()) * 2.0 ** -24 + 2.0 ** -21 * np.abs(np.where(none, 0, ref_lse))
+    assert (np.abs(np.where(none, 0, lse) - np.where(none, 0, ref_lse)) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("fmt", list(NAMES))
+@pytest.mark.parametrize("case", range(len(ATTEND)))
+def test_attend(kv, fmt, dtype, case):
+    if NAMES[fmt] in R.TORCH and fmt != dtype:
+        pytest.skip("a 16-bit cache takes queries of its own type")
+    c, f, q, table, kv_len, cu, mask = attend_case(kv, fmt, dtype, *ATTEND[case], seed=case)
+    new = ATTEND[case][0]
+    one = max(new) == 1
+    args = dict(max_q=max(new), mask=None if mask is None else dev(mask.view(np.int32)), lse=True)
+    got, lse = c.attend(q.cuda(), dev(table), dev(kv_len), None if one else dev(cu), **args)
+    c.ctx.sync()
+    verify(c, f, q, table, kv_len, cu, mask, got, lse, q.shape[-1] ** -0.5, dtype)
+    # a looser bound on the rows chooses other tiles; the same call again gives the same bits
+    args["max_q"] = max(new) + 40
+    if mask is not None:
+        args["mask"] = dev(np.pad(mask, ((0, 0), (0, 2))).view(np.int32))
+    again, lse2 = c.attend(q.cuda(), dev(table), dev(kv_len), dev(cu), **args)
+    third, lse3 = c.attend(q.cuda(), dev(table), dev(kv_len), dev(cu), **args)
+    c.ctx.sync()
+    verify(c, f, q, table, kv_len, cu, mask, again, lse2, q.shape[-1] ** -0.5, dtype)
+    assert torch.equal(again.view(torch.int16), third.view(torch.int16)) and torch.equal(lse2, lse3)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", "bf16"), ("bf16", "bf16"), ("fp16", "fp16"), ("e5m2", "fp16")])
+@pytest.mark.parametrize("scale", [1e-3, 1.0, 40.0])
+def test_attend_scales_and_strides(kv, fmt, dtype, scale):
+    """Sharp and flat softmax; queries and outputs as slices of wider tensors, rows behind the last
+    sequence and columns beside the outputs left as they were."""
+    c, f, q, table, kv_len, cu, mask = attend_case(kv, fmt, dtype, [3, 20], [100, 37], 16, 2, 3, 128, 64, "thd", "tree", 5)
+    n = q.shape[0]
+    if scale > 1:
+        q = q * 0.1
+        q = q.to(DT[dtype])
+    wide = torch.full((n + 3, 2, 6, 128), 3.0, dtype=DT[dtype], device="cuda")
+    wide[:n, 0] = q.cuda()
+    out = wide[:, 1]
+    tall = torch.cat([mask, np.zeros((3, mask.shape[1]), np.uint32)]) if False else np.pad(mask, ((0, 3), (0, 0)))
+    got, lse = c.attend(wide[:, 0], dev(table), dev(kv_len), dev(cu), max_q=20, mask=dev(tall.view(np.int32)),
+                        scale=scale, lse=True, out=out)
+    c.ctx.sync()
+    assert got.data_ptr() == out.data_ptr() and (out[n:] == 3.0).all() and torch.equal(wide[:n, 0], q.cuda())
+    verify(c, f, q, table, kv_len, cu, mask, got[:n], lse[:n], scale, dtype)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", "bf16"), ("e4m3", "fp16"), ("e5m2", "bf16"), ("bf16", "bf16"), ("fp16", "fp16")])
+@pytest.mark.parametrize("mask_kind", [None, "tree"])
+@pytest.mark.parametrize("keys", [True, False])
+def test_attend_unseen_rows_do_not_reach(kv, fmt, dtype, mask_kind, keys):
+    """A draft whose keys and values are NaN and infinite reaches the rows that see it, and no other."""
+    new, past = [40], [50]
+    c, f, q, table, kv_len, cu, mask = attend_case(kv, fmt, dtype, new, past, 16, 1, 2, 128, 64, "thd", mask_kind, 9)
+    bad = {7: "k nan", 11: "v nan", 17: "v inf", 18: "v -inf", 30: "both inf"}
+    nan = float("nan") if f in R.TORCH else 0x7F
+    inf, ninf = (float("inf"), float("-inf")) if f in R.TORCH else (0x7C, 0xFC)
+    for j, what in bad.items():
+        pos = past[0] + j
+        p, o = int(table[0][pos // 16]), pos % 16
+        if what == "k nan":
+            if keys:
+                c.k[p, o] = nan
+        elif what == "v nan":
+            c.v[p, o, 0, 5:9] = nan
+        elif f != R.E4M3:  # e4m3 has no infinities
+            if what == "both inf":
+                c.v[p, o, 0, 64:66] = inf
+                c.v[p, o, 0, 66:68] = ninf
+            else:
+                c.v[p, o, 0, 64:70] = inf if what == "v inf" else ninf
+    got, lse = c.attend(q.cuda(), dev(table), dev(kv_len), dev(cu), max_q=40,
+                        mask=None if mask is None else dev(mask.view(np.int32)), lse=True)
+    c.ctx.sync()
+    k, v = written(c, f)
+    out, ref_lse, weight = R.attend(q.double().numpy(), k, v, table, kv_len, cu, mask, 128 ** -0.5)
+    got = got.cpu().double().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(out))
+    assert np.array_equal(got[np.isinf(out)], out[np.isinf(out)]) and np.array_equal(np.isinf(got), np.isinf(out))
+    fin = np.isfinite(out)
+    tol = R.tolerance(np.where(fin, out, 0), np.where(np.isfinite(weight), weight, 0), q.double().numpy(),
+                      float(np.nanmax(np.abs(k[np.isfinite(k)]))), 90, 128 ** -0.5, DT[dtype])
+    assert (np.abs(np.where(fin, got - out, 0)) <= tol).all()
+    assert np.array_equal(np.isnan(lse.cpu().numpy()), np.isnan(ref_lse))
+    assert fin.any() and np.isnan(out).any()
+    # (after a causal row of NaN keys every row is NaN, and no infinity is left to see)
+    assert f == R.E4M3 or (keys and mask_kind is None) or np.isinf(out).any()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1", "bf16"])
+def test_attend_rows_that_see_nothing(kv, fmt):
+    """No past and an empty mask row: zeros and -inf; scores of the type's lowest and of -inf."""
+    c, f, q, table, kv_len, cu, _ = attend_case(kv, fmt, "bf16", [6, 4], [0, 20], 8, 1, 2, 64, 32, "thd", None, 3)
+    mask = np.zeros((10, 1), np.uint32)
+    mask[1, 0], mask[4, 0], mask[5, 0] = 0b10, 0b100000, 0xFFFFFFFF  # (bits past the sixth name no row)
+    got, lse = c.attend(q.cuda(), dev(table), dev(kv_len), dev(cu), max_q=6, mask=dev(mask.view(np.int32)), lse=True)
+    c.ctx.sync()
+    assert (got[[0, 2, 3]] == 0).all() and (lse[[0, 2, 3]] == float("-inf")).all()
+    verify(c, f, q, table, kv_len, cu, mask, got, lse, 64 ** -0.5, "bf16")
+    if fmt == "bf16":  # scores of -1e38: far below where a maximum starts
+        c.k.fill_(-1.0)
+        q.fill_(0)
+        q[:, :, 0] = 3e38
+        got, lse = c.attend(q.cuda(), dev(table), dev(kv_len), dev(cu), max_q=6, mask=dev(mask.view(np.int32)), scale=0.5, lse=True)
+        c.ctx.sync()
+        verify(c, f, q, table, kv_len, cu, mask, got, lse, 0.5, "bf16")
+
+
+def test_attend_long_and_past_four_gigabytes(kv):
+    """A pool of more than 2^32 bytes, its last pages in use; a context cut into many ranges."""
+    pages, page, dim = 35000, 64, 128  # 35000 x 64 x 16 x 128 = 4.6 GB a pool
+    if torch.cuda.mem_get_info()[0] < 12e9:
+        pytest.skip("needs 12 GB")
+    c = kv.KvCache.empty(pages, page, 16, dim, R.E4M3, 128)
+    rng = np.random.default_rng(2)
+    new, past = [5], [20000]
+    need = -(-20005 // page)
+    table = (pages - 1 - rng.permutation(need)).astype(np.int32)[None]
+    kv_len, cu = np.array([20005], np.int32), np.array([0, 5], np.int32)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(20005, 16, dim, generator=g, device="cuda").bfloat16() for _ in range(2))
+    c.write(k, v, dev(table), dev(kv_len), dev(np.array([0, 20005], np.int32)))
+    back = c.read(dev(table), dev(kv_len), dev(np.array([0, 20005], np.int32)), rows=20005, dtype=torch.float32)
+    q = torch.randn(5, 32, dim, generator=g, device="cuda").bfloat16()
+    got, lse = c.attend(q, dev(table), dev(kv_len), dev(cu), max_q=5, lse=True)
+    c.ctx.sync()
+    for x, y in ((k, back[0]), (v, back[1])):
+        assert ((x.float() - y).abs() <= x.float().abs() * 2.0 ** -4 + x.float().abs().amax(-1, keepdim=True) / 448 * 2.0 ** -9).all()
+    kk, vv = (t.cpu().double().transpose(0, 1).numpy() for t in back)
+    qq = q.cpu().double().numpy()
+    for h in range(0, 32, 5):
+        s = qq[:, h] @ kk[h // 2].T * dim ** -0.5
+        s[np.arange(20005)[None] > 20000 + np.arange(5)[:, None]] = -np.inf
+        p = np.exp(s - s.max(-1, keepdims=True))
+        z = p.sum(-1, keepdims=True)
+        out, weight = p @ vv[h // 2] / z, p @ np.abs(vv[h // 2]) / z
+        tol = R.tolerance(out, weight, qq[:, h], float(np.abs(kk[h // 2]).max()), 20005, dim ** -0.5, torch.bfloat16)
+        assert (np.abs(got[:, h].cpu().double().numpy() - out) <= tol).all()
+
+
+# ---- keep ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", list(NAMES))
+@pytest.mark.parametrize("page,heads,dim,group,order", [(8, 2, 96, 32, "hdt"), (16, 8, 128, 128, "thd"), (64, 1, 256, 32, "thd")])
+def test_keep(kv, fmt, page, heads, dim, group, order):
+    f = NAMES[fmt]
+    rng = np.random.default_rng(7)
+    new, past = [1, 40, 0, 70, 300, 12], [0, 13, 9, 0, 5, 31]
+    table, kv_len, cu, count = layout(rng, new, past, page)
+    c = make(kv, fmt, count, page, heads, dim, group, order)
+    n = int(cu[-1])
+    dt = "fp32" if f not in R.TORCH else fmt
+    k, v = rows_of(rng, n, heads, dim, dt), rows_of(rng, n, heads, dim, dt)
+    c.write(k.cuda(), v.cuda(), dev(table), dev(kv_len), dev(cu))
+    read = dict(rows=n, dtype=torch.float32)
+    before = [t.cpu() for t in c.read(dev(table), dev(kv_len), dev(cu), **read)]
+    path, plen = np.full((6, 300), 10 ** 6, np.int32), np.zeros(6, np.int32)
+    for b, keep in enumerate(([0], sorted(rng.choice(40, 11, replace=False)), [], list(range(70)),
+                              sorted(rng.choice(300, 222, replace=False)), [])):
+        path[b, :len(keep)], plen[b] = keep, len(keep)
+    new_len = c.keep(dev(table), dev(kv_len), dev(cu), dev(path), dev(plen))
+    c.ctx.sync()
+    assert new_len.cpu().tolist() == [past[b] + int(plen[b]) for b in range(6)]
+    after = [t.cpu() for t in c.read(dev(table), dev(kv_len), dev(cu), **read)]
+    for x, y in zip(before, after):
+        for b in range(6):
+            want = x[cu[b]:cu[b + 1]].clone()
+            want[:plen[b]] = x[cu[b]:cu[b + 1]][path[b, :plen[b]]]
+            assert torch.equal(want, y[cu[b]:cu[b + 1]])
+
+
+def test_keep_of_one_row_each(kv):
+    c = make(kv, "e4m3", 4, 8, 2, 64, 32)
+    table, kv_len = dev(np.array([[1], [3]], np.int32)), dev(np.array([5, 8], np.int32))
+    x = torch.randn(2, 2, 64, device="cuda").bfloat16()
+    c.write(x, x, table, kv_len)
+    out = c.keep(table, kv_len, None, dev(np.zeros((2, 1), np.int32)), dev(np.array([1, 0], np.int32)))
+    c.ctx.sync()
+    assert out.cpu().tolist() == [5, 7]
+
+
+# ---- lists that do not fit -----------------------------------------------------------------------
+def test_bad_lists_are_reported_and_stay_inside(kv, hf):
+    """Offsets, lengths, pages and paths that lead nowhere: HF_ERR_CORRUPT from the next sync, the
+    other sequences' results as they should be, nothing else written."""
+    from huffman_amd import HuffhipError
+    rng = np.random.default_rng(1)
+    new, past, page = [3, 4, 2], [20, 9, 0], 8
+    good_table, good_len, good_cu, count = layout(rng, new, past, page, width=4)
+    ctx = hf.Context()
+    c = make(kv, "e4m3", count, page, 2, 64, 32, ctx=ctx)
+    total = np.concatenate([[0], np.cumsum(good_len)]).astype(np.int32)
+    rows = rows_of(rng, int(total[-1]), 2, 64, "bf16").cuda()
+    c.write(rows, rows, dev(good_table), dev(good_len), dev(total))
+    q = rows_of(rng, 9, 4, 64, "bf16").cuda()
+    want = c.attend(q, dev(good_table), dev(good_len), dev(good_cu), max_q=4)
+    ctx.sync()
+    kv_before, scale_before = c.k.clone(), c.k_scale.clone()
+    values_before = [t.clone() for t in (c.v, c.v_scale)]
+    x = rows_of(rng, 9, 2, 64, "bf16").cuda()
+
+    def variant(table=None, length=None, cu=None):
+        t, l, o = good_table.copy(), good_len.copy(), good_cu.copy()
+        for a, change in ((t, table), (l, length), (o, cu)):
+            if change:
+                a[change[0]] = change[1]
+        return dev(t), dev(l), dev(o)
+
+    # (what is wrong, whether sequence 0's results stand; a bad page is met where it is needed: the
+    # last rows of sequence 1 are all in its second page)
+    for args, first_ok in ((dict(table=((1, 0), count)), True), (dict(table=((1, 1), -1)), True),
+                           (dict(length=(1, 4 * page + 1)), True), (dict(length=(1, 3)), True),
+                           (dict(length=(1, -5)), True), (dict(cu=(2, 2)), True), (dict(cu=(3, 10)), True),
+                           (dict(cu=(1, 2 ** 31 - 1)), False), (dict(cu=(0, -1)), False)):
+        t, l, o = variant(**args)
+        got = c.attend(q, t, l, o, max_q=4)
+        with pytest.raises(HuffhipError):
+            ctx.sync()
+        if first_ok:
+            assert torch.equal(got[:3].view(torch.int16), want[:3].view(torch.int16))
+        for call in (lambda: c.write(x, x, t, l, o), lambda: c.read(t, l, o, rows=9)):
+            call()
+            if args == dict(table=((1, 0), count)):
+                ctx.sync()
+                continue
+            with pytest.raises(HuffhipError):
+                ctx.sync()
+        assert torch.equal(c.k[dev(np.setdiff1d(np.arange(count), good_table.ravel()))],
+                           kv_before[dev(np.setdiff1d(np.arange(count), good_table.ravel()))])
+        c.k.copy_(kv_before)
+        c.k_scale.copy_(scale_before)
+        c.v.copy_(values_before[0])
+        c.v_scale.copy_(values_before[1])
+        ctx.sync()
+    # more rows of a sequence than the call said
+    c.attend(q, dev(good_table), dev(good_len), dev(good_cu), max_q=3)
+    with pytest.raises(HuffhipError):
+        ctx.sync()
+    # paths that fall, repeat, leave the rows, or are longer than they can be
+    for p, n in (([2, 1], 2), ([1, 1], 2), ([0, 4], 2), ([-1, 0], 2), ([0, 1], 3), ([0, 1], -1)):
+        path = np.zeros((3, 2), np.int32)
+        path[1] = p
+        out = c.keep(dev(good_table), dev(good_len), dev(good_cu), dev(path), dev(np.array([1, n, 1], np.int32)))
+        with pytest.raises(HuffhipError):
+            ctx.sync()
+        assert out.cpu().tolist() == [21, 13, 1]
+        assert torch.equal(c.k, kv_before) and torch.equal(c.k_scale, scale_before)
+
+
+def test_refusals(kv, hf):
+    c = make(kv, "e4m3", 4, 16, 2, 64, 32)
+    t, l = dev(np.zeros((1, 1), np.int32)), dev(np.ones(1, np.int32))
+    x = torch.zeros(1, 2, 64, device="cuda", dtype=torch.bfloat16)
+    q = torch.zeros(1, 4, 64, device="cuda", dtype=torch.bfloat16)
+    from huffman_amd import HuffhipError, HF_KV_BF16
+    bad = [
+        lambda: c.write(x, x[:, :1], t, l), lambda: c.write(x, x.half(), t, l), lambda: c.write(x.int(), x.int(), t, l),
+        lambda: c.write(x.cpu(), x.cpu(), t, l), lambda: c.write(x, x, t.long(), l), lambda: c.write(x, x, t, l.cpu()),
+        lambda: c.write(x, x, t[0], l), lambda: c.write(x, x, t, l, dev(np.zeros(3, np.int32))),
+        lambda: c.write(torch.cat([x, x]), torch.cat([x, x]), t, l),
+        lambda: c.write(x.transpose(1, 2).contiguous().transpose(1, 2), x, t, l),
+        lambda: c.read(t, l, dev(np.array([0, 1], np.int32))), lambda: c.attend(q.float(), t, l),
+        lambda: c.attend(q[:, :3], t, l), lambda: c.attend(q, t, l, mask=dev(np.zeros((2, 1), np.int32))),
+        lambda: c.attend(q, t, l, dev(np.array([0, 1], np.int32)), max_q=1, mask=dev(np.zeros((1, 0), np.int32))),
+        lambda: c.attend(q, t, l, scale=0.0), lambda: c.attend(q, t, l, scale=float("nan")),
+        lambda: c.attend(q, t, l, scale=float("inf")), lambda: c.attend(q, t, l, out=q.half()),
+        lambda: c.keep(t, l, None, t[0], l), lambda: c.keep(t, l, None, t, l, new_len=l),
+        lambda: kv.KvCache.empty(2, 12, 1, 64), lambda: kv.KvCache.empty(2, 4, 1, 64).write(x[:, :1], x[:, :1], t, l),
+        lambda: kv.KvCache.empty(2, 8, 2, 48, HF_KV_BF16).write(x[..., :48].contiguous(), x[..., :48].contiguous(), t, l),
+        lambda: kv.KvCache.empty(2, 8, 2, 64, group=16).write(x, x, t, l),
+        lambda: kv.KvCache.empty(2, 8, 2, 64, HF_KV_BF16).write(x.half(), x.half(), t, l),
+        lambda: kv.KvCache.empty(2, 8, 2, 64, HF_KV_BF16).attend(q.half(), t, l),
+        lambda: kv.KvCache(c.k, c.v), lambda: kv.KvCache(c.k, c.v, c.k_scale, c.v_scale[:, :, :1]),
+        # rows that start between 16-byte pieces
+        lambda: c.write(torch.zeros(1, 2, 72, device="cuda", dtype=torch.bfloat16)[..., 4:68], x, t, l),
+        # outputs that lie on one another
+        lambda: c.read(t, l, out=(x.expand(1, 2, 64), torch.zeros(1, 1, 64, device="cuda", dtype=torch.bfloat16).expand(1, 2, 64))),
+        lambda: c.attend(q, t, l, out=torch.zeros(1, 1, 64, device="cuda", dtype=torch.bfloat16).expand(1, 4, 64)),
+    ]
+    for i, f in enumerate(bad):
+        if i == 21:  # a page size that is no power of two is refused when it is used
+            f = lambda: kv.KvCache.empty(2, 12, 1, 64).write(x[:, :1], x[:, :1], t, l)  # noqa: E731
+        try:
+            f()
+        except (ValueError, TypeError, HuffhipError):
+            continue
+        pytest.fail(f"call {i} was not refused")
+    c.ctx.sync()
+    # calls of nothing are calls
+    none = torch.zeros(0, 2, 64, device="cuda", dtype=torch.bfloat16)
+    t0, l0 = torch.zeros(0, 1, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
+    c.write(none, none, t0, l0)
+    assert c.read(t0, l0)[0].shape == (0, 2, 64)
+    assert c.attend(torch.zeros(0, 4, 64, device="cuda", dtype=torch.bfloat16), t0, l0).shape == (0, 4, 64)
+    assert c.keep(t0, l0, None, torch.zeros(0, 3, dtype=torch.int32, device="cuda"), l0).shape == (0,)
+    c.ctx.sync()
+
+
+# ---- streams, graphs -----------------------------------------------------------------------------
+def test_graphs_follow_lengths_and_do_not_share_scratch(kv, hf):
+    """Two captured decode steps (write, attend) of one context, replayed on two streams at once and
+    in turn with eager calls, while lengths, tables and rows change between the replays."""
+    rng = np.random.default_rng(4)
+    side = torch.cuda.Stream()
+    ctx = hf.Context(stream=side)
+    sets = []
+    for i in range(2):
+        new, past = [1, 1, 1], [900, 300, 40]
+        table, kv_len, cu, count = layout(rng, new, [p + 60 for p in past], 16)
+        c = make(kv, "e4m3", count, 16, 2, 128, 64, ctx=ctx)
+        full = kv_len.copy()
+        cut = np.concatenate([[0], np.cumsum(full)]).astype(np.int32)
+        rows = rows_of(rng, int(cut[-1]), 2, 128, "bf16").cuda()
+        x, q = rows_of(rng, 3, 2, 128, "bf16").cuda(), rows_of(rng, 3, 8, 128, "bf16").cuda()
+        t, l = dev(table), dev(np.array([p + 1 for p in past], np.int32))
+        torch.cuda.synchronize()
+        c.write(rows, rows, t, dev(full), dev(cut))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            c.write(x, x, t, l)
+            out, lse = c.attend(q, t, l, lse=True)
+        sets.append((c, g, x, q, t, l, out, lse, table))
+    other = torch.cuda.Stream()
+    for turn in range(4):
+        for c, g, x, q, t, l, out, lse, table in sets:
+            x.copy_(rows_of(rng, 3, 2, 128, "bf16"))
+            q.copy_(rows_of(rng, 3, 8, 128, "bf16"))
+            l.add_(turn * 7)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            sets[0][1].replay()
+        with torch.cuda.stream(other):
+            sets[1][1].replay()
+        torch.cuda.synchronize()
+        for c, g, x, q, t, l, out, lse, table in sets:
+            verify(c, R.E4M3, q.cpu(), table, l.cpu().numpy(), np.arange(4), None, out, lse, 128 ** -0.5, "bf16")
+            eager, eager_lse = c.attend(q, t, l, lse=True)
+            torch.cuda.synchronize()
+            assert torch.equal(eager.view(torch.int16), out.view(torch.int16)) and torch.equal(eager_lse, lse)
+
+
+def test_contexts_on_two_streams(kv, hf):
+    """The same call on two contexts at once, over and over, gives each its own results."""
+    cases = []
+    for i in range(2):
+        ctx = hf.Context(stream=torch.cuda.Stream())
+        args = attend_case(kv, "e2m1", "bf16", [30, 30], [3000, 1500], 16, 2, 4, 128, 32, "thd", "tree", 40 + i, ctx)
+        torch.cuda.synchronize()
+        cases.append((ctx, args, [args[2].cuda(), dev(args[3]), dev(args[4]), dev(args[5])], dev(args[6].view(np.int32))))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(6):
+        for i, (ctx, args, dv, mask) in enumerate(cases):
+            outs[i].append(args[0].attend(*dv, max_q=30, mask=mask, lse=True))
+    torch.cuda.synchronize()
+    for i, (ctx, (c, f, q, table, kv_len, cu, mask), _, _) in enumerate(cases):
+        ctx.sync()
+        verify(c, f, q, table, kv_len, cu, mask, *outs[i][0], 128 ** -0.5, "bf16")
+        for out, lse in outs[i][1:]:
+            assert torch.equal(out.view(torch.int16), outs[i][0][0].view(torch.int16)) and torch.equal(lse, outs[i][0][1])
+
+
+# ---- the way it is used --------------------------------------------------------------------------
+def test_speculative_steps_with_stored_pages(kv, hf):
+    """Prompts in; then, twice: a tree of drafts written, attended, the accepted path kept.  Then the
+    fp8 pages go through the page coder, are decoded into other places of another pool, and attention
+    over those is the same, bit for bit."""
+    rng = np.random.default_rng(8)
+    page, heads, dim, batch = 16, 8, 128, 3
+    lens = [100, 37, 5]
+    width = 16
+    order = rng.permutation(batch * width)
+    table = order.reshape(batch, width).astype(np.int32)
+    t = dev(table)
+    c = kv.KvCache.empty(batch * width, page, heads, dim, R.E4M3)
+    assert c.group == 128 and page * heads * dim == hf.HF_CHUNK_SYMS  # a cache page is a page of the coder
+    history = [rows_of(rng, n, heads, dim, "bf16") for n in lens]  # what each sequence should hold, keys = values / 2
+    cut = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    flat = torch.cat(history)
+    c.write((flat * 0.5).cuda(), flat.cuda(), t, dev(np.array(lens, np.int32)), dev(cut))
+    kv_len = np.array(lens, np.int32)
+    for step in range(2):
+        new = [12, 7, 20]
+        cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        drafts = rows_of(rng, int(cu[-1]), heads, dim, "bf16")
+        now = dev(kv_len + np.array(new, np.int32))
+        c.write((drafts * 0.5).cuda(), drafts.cuda(), t, now, dev(cu))
+        mask = tree_mask(rng, new, 1)
+        q = rows_of(rng, int(cu[-1]), 32, dim, "bf16", 0.7)
+        got, lse = c.attend(q.cuda(), t, now, dev(cu), max_q=20, mask=dev(mask.view(np.int32)), lse=True)
+        c.ctx.sync()
+        verify(c, R.E4M3, q, table, now.cpu().numpy(), cu, mask, got, lse, dim ** -0.5, "bf16")
+        # the deepest path of each tree is accepted
+        path, plen = np.zeros((batch, 20), np.int32), np.zeros(batch, np.int32)
+        for b in range(batch):
+            best = max(range(new[b]), key=lambda i: bin(int(mask[cu[b] + i, 0])).count("1"))
+            keep = [j for j in range(new[b]) if int(mask[cu[b] + best, 0]) >> j & 1]
+            path[b, :len(keep)], plen[b] = keep, len(keep)
+            history[b] = torch.cat([history[b], drafts[cu[b]:cu[b + 1]][keep]])
+        new_len = c.keep(t, now, dev(cu), dev(path), dev(plen))
+        c.ctx.sync()
+        kv_len = new_len.cpu().numpy().astype(np.int32)
+        assert kv_len.tolist() == [len(h) for h in history]
+    cut = np.concatenate([[0], np.cumsum(kv_len)]).astype(np.int32)
+    got = c.read(t, dev(kv_len), dev(cut), rows=int(cut[-1]), dtype=torch.float32)
+    c.ctx.sync()
+    code, scale = R.quantise(torch.cat(history).double().numpy(), R.E4M3, 128)
+    want = torch.from_numpy(R.dequantise(code, scale, R.E4M3, 128)).float()
+    assert torch.equal(got[1].cpu(), want) and torch.equal(got[0].cpu(), want * 0.5)
+    # stored and fetched: both pools through the coder, page by page, into another pool's pages
+    q = rows_of(rng, batch, 32, dim, "bf16", 0.7).cuda()
+    before = c.attend(q, t, dev(kv_len))
+    system, decoder = hf.EntropyAwareHuffmanSystem(), hf.ParrallelHuffmanDecoder()
+    moved = rng.permutation(batch * width).astype(np.int32)  # page p of the pool goes to page moved[p]
+    other = kv.KvCache.empty(batch * width, page, heads, dim, R.E4M3)
+    ids = dev(np.arange(batch * width, dtype=np.int32))
+    for src, dst in ((c.k, other.k), (c.v, other.v)):
+        s = system.encode_blocks(src.reshape(-1), paged=True)
+        decoder.decode_blocks_to(s, ids, dev(moved), dst.view(-1))
+    for src, dst in ((c.k_scale, other.k_scale), (c.v_scale, other.v_scale)):
+        s = system.encode(src.reshape(-1))
+        dst[dev(moved).long()] = decoder.decode(s).view(src.shape)
+    after = other.attend(q, dev(moved[table]), dev(kv_len))
+    torch.cuda.synchronize()
+    assert torch.equal(before.view(torch.int16), after.view(torch.int16))
