@@ -224,7 +224,7 @@ struct kv_unit {
     uint32_t groups_of_page;  // groups of eight tokens the table has pages for
     f32x4 acc[R][VD];
     f32x4 div[R];         // sums of the rounded p (all four alike)
-    float mx[R], sum[R];  // largest score (unscaled); the lane's share of the sum of p
+    float nm[R], sum[R];  // p = exp2(scale_log2 s + nm); the lane's share of the sum of p
     hf_u32x4 qr[R][KS];
     uint32_t bad;
 
@@ -252,7 +252,7 @@ struct kv_unit {
                 if (on && d < (int)a.c.head_dim) x = *(const hf_gmem_u32x4*)(p + 2 * d);
                 qr[r][ks] = x;
             }
-            mx[r] = -3.402823466e38f;
+            nm[r] = 3.402823466e38f;
             sum[r] = 0.0f;
             div[r] = f32x4{0, 0, 0, 0};
 #pragma unroll
@@ -324,7 +324,10 @@ struct kv_unit {
 
     // Which of the lane's eight tokens t + 8 g + 0..7 row i (of the sequence's n rows) may see.
     __device__ __forceinline__ uint32_t seen(const int32_t row, const uint32_t t, const bool on) const {
-        const int32_t j = (int32_t)(t + 8u * g) - q.past;  // draft number of the first of them
+        return seen_at(row, t + 8u * g, on);
+    }
+    __device__ __forceinline__ uint32_t seen_at(const int32_t row, const uint32_t t, const bool on) const {
+        const int32_t j = (int32_t)t - q.past;  // draft number of the first of them
         uint32_t bits8;
         if (a.mask) {
             const int32_t w = j >> 5;
@@ -445,14 +448,14 @@ struct kv_unit {
             top[r] = s[r][0][0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) top[r] = fmaxf(top[r], s[r][e / 4][e % 4]);
-            up = up || (top[r] - mx[r]) * a.scale_log2 > T::rise;
+            up = up || __builtin_fmaf(top[r], a.scale_log2, nm[r]) > T::off + T::rise;
         }
         if (__ballot(up)) {  // seldom after the first step: sums and outputs to a new maximum
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const float was = mx[r];
-                mx[r] = fmaxf(was, kv_row_max(top[r]));
-                const float f = __builtin_amdgcn_exp2f((was - mx[r]) * a.scale_log2);
+                const float was = nm[r];
+                nm[r] = fminf(was, T::off - kv_row_max(top[r]) * a.scale_log2);
+                const float f = __builtin_amdgcn_exp2f(nm[r] - was);
                 sum[r] *= f;
                 div[r] *= f;
 #pragma unroll
@@ -460,13 +463,25 @@ struct kv_unit {
             }
         }
         hf_u32x4 p[R];
+        // (fused: the error of scale x maximum is the same factor for the whole row; where it could
+        // pass 1 / 256 of a power of two, the products are rounded first, as the maximum's was)
+        bool far = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) far = far || (fabsf(nm[r]) > 65536.0f && nm[r] != 3.402823466e38f);
+        const bool huge = __ballot(far) != 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float e[8];
+            if (huge) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = s[r][i / 4][i % 4] * a.scale_log2 + nm[r];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = __builtin_fmaf(s[r][i / 4][i % 4], a.scale_log2, nm[r]);
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                // (the difference first: it is exact near the maximum, however large the scores)
-                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][i / 4][i % 4] - mx[r], a.scale_log2, T::off));
+                e[i] = __builtin_amdgcn_exp2f(e[i]);
                 sum[r] += e[i];
             }
 #pragma unroll
@@ -541,17 +556,16 @@ struct kv_unit {
     }
 };
 
-// Logarithm of the sum of exp(scale s), from the largest s and the sum of p.
-template <typename T>
-__device__ __forceinline__ float kv_lse(const hf_kv_attend_args& a, const float top, const float sum) {
-    return 0.6931471805599453f * (__builtin_fmaf(top, a.scale_log2, -T::off) + __builtin_amdgcn_logf(sum));
+// Logarithm of the sum of exp(scale s), from the sum of exp2(scale_log2 s + nm).
+__device__ __forceinline__ float kv_lse(const float nm, const float sum) {
+    return sum == 0.0f ? -__builtin_inff() : 0.6931471805599453f * (__builtin_amdgcn_logf(sum) - nm);
 }
 
 // Scratch of a workgroup: what two wavefronts hand to the other two.
 template <int DP, int R>
 struct kv_lds {
     f32x4 acc[2][R][DP / 16][64];
-    float mx[2][R][64], sum[2][R][64], div[2][R][64];
+    float nm[2][R][64], sum[2][R][64], div[2][R][64];
 };
 
 template <int QT, int FMT, int DP, int R>
@@ -616,7 +630,7 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
         if (wave >= half && wave < 2 * half) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                lds.mx[wave - half][r][u.lane] = u.mx[r];
+                lds.nm[wave - half][r][u.lane] = u.nm[r];
                 lds.sum[wave - half][r][u.lane] = u.sum[r];
                 lds.div[wave - half][r][u.lane] = u.div[r][0];
 #pragma unroll
@@ -627,11 +641,11 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
         if (wave < half) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const float om = lds.mx[wave][r][u.lane];
-                const float top = fmaxf(u.mx[r], om);
-                const float f = __builtin_amdgcn_exp2f((u.mx[r] - top) * a.scale_log2);
-                const float h = __builtin_amdgcn_exp2f((om - top) * a.scale_log2);
-                u.mx[r] = top;
+                const float other = lds.nm[wave][r][u.lane];
+                const float least = fminf(u.nm[r], other);
+                const float f = __builtin_amdgcn_exp2f(least - u.nm[r]);
+                const float h = __builtin_amdgcn_exp2f(least - other);
+                u.nm[r] = least;
                 u.sum[r] = u.sum[r] * f + lds.sum[wave][r][u.lane] * h;
                 u.div[r][0] = u.div[r][0] * f + lds.div[wave][r][u.lane] * h;
 #pragma unroll
@@ -645,6 +659,7 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
     for (int r = 0; r < R; ++r) {
         const int32_t i = row_lo + 16 * r + u.m;
         if (cut.ranges > 1) {  // to be joined with the other ranges
+            if (i >= rows) continue;
             const int64_t row = (int64_t)blockIdx.x * tile_rows + 16 * r + u.m;
             float* dst = a.part + row * DP;
 #pragma unroll
@@ -654,7 +669,7 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
                     *(f32x4*)(dst + U::VD * (4 * u.g + e) + c) =
                         f32x4{u.acc[r][c][e], u.acc[r][c + 1][e], u.acc[r][c + 2][e], u.acc[r][c + 3][e]};
             if (u.g == 0) {
-                *(f32x4*)(a.part_ml + 4 * row) = f32x4{u.mx[r], u.sum[r], u.div[r][0], 0.0f};
+                *(f32x4*)(a.part_ml + 4 * row) = f32x4{u.nm[r], u.sum[r], u.div[r][0], 0.0f};
             }
         } else if (i < rows) {
             const int32_t tok = i / (int32_t)a.per, hq = i % (int32_t)a.per;
@@ -676,17 +691,16 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
             }
             if (a.lse && u.g == 0)
                 a.lse[(int64_t)(u.q.row0 + tok) * a.c.heads * a.per + out_head] =
-                    l == 0.0f ? -__builtin_inff() : kv_lse<typename U::T>(a, u.mx[r], l);
+                    kv_lse(u.nm[r], l);
         }
     }
 }
 
 // Joins the ranges of a row: a wavefront per row, DP / 4 lanes along the row and the ranges dealt to
 // the groups of lanes that are left.
-template <int QT, int DP, int R>
-__global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a) {
+template <int QT, int DP>
+__global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a, const uint32_t tile_rows) {
     typedef kv_type<QT> T;
-    constexpr uint32_t tile_rows = 16 * R;
     constexpr uint32_t cols = DP / 4, deal = 64 / cols;
     const uint32_t each = kv_steps_each(a, tile_rows);
     const uint32_t q_heads = a.c.heads * a.per;
@@ -737,17 +751,17 @@ __global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a) {
     const int64_t first = (int64_t)(before + tile) * tile_rows + i % tile_rows;
     const int64_t jump = (int64_t)tiles * tile_rows;
     const uint32_t col = (uint32_t)hf_lane() % cols, part = (uint32_t)hf_lane() / cols;
-    float top = -3.402823466e38f;
-    for (uint32_t s = hf_lane(); s < ranges; s += 64) top = fmaxf(top, a.part_ml[4 * (first + s * jump)]);
+    float least = 3.402823466e38f;
+    for (uint32_t s = hf_lane(); s < ranges; s += 64) least = fminf(least, a.part_ml[4 * (first + s * jump)]);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    for (int o = 32; o > 0; o >>= 1) least = fminf(least, __shfl_xor(least, o));
     f32x4 acc = {0, 0, 0, 0};
     float sum = 0.0f, div = 0.0f;
 #pragma unroll 4
     for (uint32_t s = part; s < ranges; s += deal) {
         const int64_t at = first + s * jump;
         const f32x4 ml = *(const f32x4*)(a.part_ml + 4 * at);
-        const float w = __builtin_amdgcn_exp2f((ml[0] - top) * a.scale_log2);
+        const float w = __builtin_amdgcn_exp2f(least - ml[0]);
         sum += w * ml[1];
         div += w * ml[2];
         acc += w * *(const f32x4*)(a.part + at * DP + 4 * col);
@@ -766,29 +780,7 @@ __global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a) {
             hf_u32x2{T::pack(acc[0] * f, acc[1] * f), T::pack(acc[2] * f, acc[3] * f)};
     }
     if (a.lse && hf_lane() == 0)
-        a.lse[(int64_t)row * q_heads + out_head] =
-            sum == 0.0f ? -__builtin_inff() : kv_lse<T>(a, top, sum);
-}
-
-template <int QT, int FMT, int DP, int R>
-void kv_launch(const hf_kv_attend_args& a, hipStream_t st) {
-    hipLaunchKernelGGL((hf_k_kv_attend<QT, FMT, DP, R>), dim3(a.units), dim3(64 * kWaves), 0, st, a);
-    if (a.join) {
-        const uint64_t rows = (uint64_t)a.s.rows * a.c.heads * a.per;
-        hipLaunchKernelGGL((hf_k_kv_join<QT, DP, R>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, st, a);
-    }
-}
-template <int QT, int FMT, int DP>
-void kv_launch_rows(const hf_kv_attend_args& a, const int tile_rows, hipStream_t st) {
-    if (tile_rows == 16) kv_launch<QT, FMT, DP, 1>(a, st);
-    else if (tile_rows == 32 || DP == 256) kv_launch<QT, FMT, DP, 2>(a, st);
-    else if constexpr (DP < 256) kv_launch<QT, FMT, DP, 4>(a, st);
-}
-template <int QT, int FMT>
-void kv_launch_dim(const hf_kv_attend_args& a, const int tile_rows, hipStream_t st) {
-    if (a.c.head_dim <= 64) kv_launch_rows<QT, FMT, 64>(a, tile_rows, st);
-    else if (a.c.head_dim <= 128) kv_launch_rows<QT, FMT, 128>(a, tile_rows, st);
-    else kv_launch_rows<QT, FMT, 256>(a, tile_rows, st);
+        a.lse[(int64_t)row * q_heads + out_head] = kv_lse(least, sum);
 }
 
 }  // namespace

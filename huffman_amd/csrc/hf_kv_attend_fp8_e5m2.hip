@@ -1,5 +1,5 @@
-// Attention over a cache of fp8_e5m2 codes (kernel: hf_kv_attend.h).
-#include "hf_kv_attend.h"
+// Attention over a cache of fp8_e5m2 codes (kernels: hf_kv_attend.h, hf_kv_block.h).
+#include "hf_kv_block.h"
 
 void hf_launch_kv_attend_fp8_e5m2(const hf_kv_attend_args& a, int dtype, int tile_rows,
                                 hipStream_t st) {
