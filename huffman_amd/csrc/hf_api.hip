@@ -1633,9 +1633,9 @@ struct kv_plan {
 };
 int kv_plan_of(const hf_ctx* ctx, const hf_kv_pools& p, const hf_kv_seqs& s, uint32_t per, kv_plan* o) {
     o->tile_rows = hf_kv_attend_tile_rows(s.most, per, p.head_dim);
-    // (units per compute unit: short ones even out a ragged batch of single tokens, 198 -> 170 us from
+    // (units per compute unit: short ones even out a ragged batch of single tokens, 198 -> 163 us from
     // 2 to 6 for 64 sequences of up to 8000; larger tiles pay more for each unit they are cut into)
-    o->target = (uint32_t)ctx->num_cu * (o->tile_rows == 16 ? 6u : o->tile_rows == 128 ? 2u : 8u);
+    o->target = (uint32_t)ctx->num_cu * (o->tile_rows == 16 ? 6u : o->tile_rows == 32 ? 4u : 2u);
     o->min_steps = 4;
     const uint64_t rows = (uint64_t)s.rows * per;
     const uint64_t by_rows = rows / o->tile_rows + s.batch;
@@ -1644,8 +1644,10 @@ int kv_plan_of(const hf_ctx* ctx, const hf_kv_pools& p, const hf_kv_seqs& s, uin
     const uint64_t steps = (((uint64_t)s.width << p.page_shift) + 31) / 32;
     const uint64_t most = (steps + o->min_steps - 1) / o->min_steps;  // ranges of a sequence, at most
     o->join = most > 1;
-    uint64_t units = tiles + o->target;
-    if (most < units && tiles * most < units) units = tiles * most;
+    // (a tile has one range and one more for each time it reaches the steps aimed at; the kernels
+    // round the number up to eighths)
+    uint64_t units = tiles + o->target + 8;
+    if (most < units && tiles * most < units) units = (tiles * most + 7) / 8 * 8;
     if (units > 0x7FFFFFFFull || (uint64_t)s.rows * p.heads * per > 0x7FFFFFFFull) return HF_ERR_RANGE;
     o->units = (uint32_t)units;
     const uint64_t pad = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;

@@ -127,68 +127,112 @@ __device__ __forceinline__ float kv_row_sum(float a) {
     return a + __shfl_xor(a, 32);
 }
 
+// Has the values' loads waited for here: left to their first use, which is in a loop that issues
+// loads of its own, the wait there would be for those too, in every turn.
+template <int N>
+__device__ __forceinline__ void kv_arrived(hf_u32x4 (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
+}
+
 // ---- the cut of a call into units ---------------------------------------------------------------
 // Every wavefront finds its unit from the device's own lengths, so a captured call follows lengths
 // that change between replays and a ragged batch is cut evenly: all sequences' steps (32 tokens)
-// times their row tiles are summed, divided by the units aimed at, and a sequence has as many
-// ranges of that many steps as it needs.  Units of a sequence are numbered range by range, in it by
-// cache head, in it by row tile, so that the tiles that read the same tokens are neighbours.
+// times their row tiles are summed and divided by the units aimed at, and a sequence has as many
+// equal ranges as it needs for about that many steps (a quarter more is let pass: a range costs its
+// partial outputs).  Units of a sequence are numbered range by range, in it by cache head, in it by
+// row tile, so that the tiles that read the same tokens are neighbours; and since consecutive
+// workgroups go to the eight XCDs in turn, each with an L2 of its own, XCD x takes the x-th eighth of
+// the units.
 struct kv_cut {
-    uint32_t b, n_before;  // sequence; units of the sequences before it
+    uint32_t unit, b, n_before;  // unit; its sequence; units of the sequences before that
     uint32_t tiles, ranges, steps_each;
 };
-
-__device__ __forceinline__ void kv_shape(const hf_kv_attend_args& a, const uint32_t tile_rows,
-                                         const uint32_t b, uint32_t& tiles, uint32_t& steps) {
-    const hf_kv_seq q = hf_kv_sequence(a.s, b, a.c.page_shift);
-    if (q.bad) atomicOr(a.err, HF_KERR_CORRUPT);
-    tiles = q.n > 0 ? a.c.heads * (((uint32_t)q.n * a.per + tile_rows - 1u) / tile_rows) : 0u;
-    steps = ((uint32_t)q.len + kStep - 1u) / kStep;
+struct kv_shape {
+    uint32_t tiles, steps, ranges;
+};
+__device__ __forceinline__ kv_shape kv_shape_of(const hf_kv_attend_args& a, const uint32_t tile_rows, const uint32_t b) {
+    kv_shape s = {0, 0, 1};
+    if (b < a.s.batch) {
+        const hf_kv_seq q = hf_kv_sequence(a.s, b, a.c.page_shift);
+        if (q.bad) atomicOr(a.err, HF_KERR_CORRUPT);
+        s.tiles = q.n > 0 ? a.c.heads * (((uint32_t)q.n * a.per + tile_rows - 1u) / tile_rows) : 0u;
+        s.steps = ((uint32_t)q.len + kStep - 1u) / kStep;
+    }
+    return s;
 }
-__device__ __forceinline__ uint32_t kv_steps_each(const hf_kv_attend_args& a, const uint32_t tile_rows) {
-    unsigned long long sum = 0;
-    for (uint32_t b0 = 0; b0 < a.s.batch; b0 += 64) {
-        const uint32_t b = b0 + hf_lane();
-        uint32_t tiles = 0, steps = 0;
-        if (b < a.s.batch) kv_shape(a, tile_rows, b, tiles, steps);
-        sum += (unsigned long long)tiles * steps;
+__device__ __forceinline__ uint32_t kv_ranges(const kv_shape& s, const uint32_t each) {
+    return max(1u, (s.steps + each - 1u - each / 4u) / each);
+}
+__device__ __forceinline__ uint32_t kv_wave_scan(const uint32_t v) {  // inclusive
+    uint32_t incl = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = __shfl_up(incl, o);
+        if (hf_lane() >= o) incl += up;
+    }
+    return incl;
+}
+// What the whole call comes to: steps of a range, units.
+struct kv_plan_dev {
+    uint32_t each, total;
+    kv_shape first;  // of the lane's sequence among the first 64: most calls have no more
+};
+__device__ __forceinline__ kv_plan_dev kv_plan_now(const hf_kv_attend_args& a, const uint32_t tile_rows) {
+    kv_plan_dev p;
+    p.first = kv_shape_of(a, tile_rows, hf_lane());
+    unsigned long long sum = (unsigned long long)p.first.tiles * p.first.steps;
+    for (uint32_t b0 = 64; b0 < a.s.batch; b0 += 64) {
+        const kv_shape s = kv_shape_of(a, tile_rows, b0 + hf_lane());
+        sum += (unsigned long long)s.tiles * s.steps;
     }
     sum = hf_wave_sum_u64(sum);
-    unsigned long long each = (sum + a.target - 1u) / a.target;
-    each = (each + kWaves - 1u) / kWaves * kWaves;
-    return (uint32_t)max(each, (unsigned long long)a.min_steps);
+    const unsigned long long each = (sum + a.target - 1u) / a.target;
+    p.each = (uint32_t)max(each, (unsigned long long)a.min_steps);
+    p.first.ranges = kv_ranges(p.first, p.each);
+    uint32_t total = p.first.tiles * p.first.ranges;
+    for (uint32_t b0 = 64; b0 < a.s.batch; b0 += 64) {
+        const kv_shape s = kv_shape_of(a, tile_rows, b0 + hf_lane());
+        total += s.tiles * kv_ranges(s, p.each);
+    }
+    p.total = hf_wave_sum_u32(total);
+    return p;
 }
-__device__ __forceinline__ uint32_t kv_ranges(const uint32_t steps, const uint32_t each) {
-    return max(1u, (steps + each - 1u) / each);
-}
-// The sequence that unit `unit` belongs to; false: there are fewer units.
-__device__ __forceinline__ bool kv_find(const hf_kv_attend_args& a, const uint32_t tile_rows,
-                                        const uint32_t unit, kv_cut& cut) {
-    cut.steps_each = kv_steps_each(a, tile_rows);
+// Walks the sequences 64 at a time; `pick` sees a lane's sequence, its shape and the units before it.
+template <typename F>
+__device__ __forceinline__ bool kv_walk(const hf_kv_attend_args& a, const uint32_t tile_rows, const kv_plan_dev& p,
+                                        F&& pick, kv_cut& cut) {
     uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < a.s.batch; b0 += 64) {
         const uint32_t b = b0 + hf_lane();
-        uint32_t tiles = 0, steps = 0;
-        if (b < a.s.batch) kv_shape(a, tile_rows, b, tiles, steps);
-        const uint32_t ranges = kv_ranges(steps, cut.steps_each), own = tiles * ranges;
-        uint32_t incl = own;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t up = __shfl_up(incl, o);
-            if (hf_lane() >= o) incl += up;
+        kv_shape s = p.first;
+        if (b0) {
+            s = kv_shape_of(a, tile_rows, b);
+            s.ranges = kv_ranges(s, p.each);
         }
-        const unsigned long long hit = __ballot(before + incl > unit);
+        const uint32_t own = s.tiles * s.ranges, incl = kv_wave_scan(own);
+        const unsigned long long hit = __ballot(pick(b, before + incl - own, own));
         if (hit) {
             const int l = __ffsll((unsigned long long)hit) - 1;
             cut.b = b0 + l;
             cut.n_before = before + __builtin_amdgcn_readlane(incl - own, l);
-            cut.tiles = __builtin_amdgcn_readlane(tiles, l);
-            cut.ranges = __builtin_amdgcn_readlane(ranges, l);
+            cut.tiles = __builtin_amdgcn_readlane(s.tiles, l);
+            cut.ranges = __builtin_amdgcn_readlane(s.ranges, l);
+            const uint32_t steps = __builtin_amdgcn_readlane(s.steps, l);
+            cut.steps_each = ((steps + cut.ranges - 1u) / cut.ranges + kWaves - 1u) / kWaves * kWaves;
             return true;
         }
         before += __builtin_amdgcn_readlane(incl, 63);
     }
     return false;
+}
+__device__ __forceinline__ bool kv_find(const hf_kv_attend_args& a, const uint32_t tile_rows, kv_cut& cut) {
+    const kv_plan_dev p = kv_plan_now(a, tile_rows);
+    const uint32_t eighth = (p.total + 7u) / 8u;
+    cut.unit = blockIdx.x % 8u * eighth + blockIdx.x / 8u;
+    if (blockIdx.x / 8u >= eighth) return false;
+    const uint32_t unit = cut.unit;
+    return kv_walk(a, tile_rows, p, [&](uint32_t, uint32_t first, uint32_t own) { return unit < first + own; }, cut);
 }
 
 // ---- one unit ------------------------------------------------------------------------------------
@@ -389,6 +433,55 @@ struct kv_unit {
             }
     }
 
+    // The values of VD elements from d of token `off` of a page (codes at p), as the products take them.
+    __device__ __forceinline__ void values(const hf_g8* p, const int32_t page, const uint32_t off, const int d,
+                                           float (&v)[VD]) const {
+        kv_raw<VB> r;
+        r.load(p);
+        float s = 0.0f;
+        if constexpr (bits != 16)
+            s = __uint_as_float((uint32_t)((const hf_g8*)a.c.v_scale)[(((int64_t)page * a.c.heads + head) * a.c.groups
+                                                                       << a.c.page_shift) + off +
+                                                                      ((int64_t)(d >> a.c.group_shift) << a.c.page_shift)]
+                                << 23);
+        uint32_t w[VD / 2];
+        if constexpr (bits == 16) {
+#pragma unroll
+            for (int i = 0; i < VD / 2; ++i) w[i] = r.w[i];
+        } else if constexpr (bits == 8) {
+#pragma unroll
+            for (int i = 0; i < VD / 4; ++i) {
+                w[2 * i] = kv_pair<QT, FMT, 0>(r.w[i], s);
+                w[2 * i + 1] = kv_pair<QT, FMT, 1>(r.w[i], s);
+            }
+        } else {
+            w[0] = kv_pair<QT, FMT, 0>(r.w[0], s);
+            w[1] = kv_pair<QT, FMT, 1>(r.w[0], s);
+            if constexpr (VD >= 8) {
+                w[2] = kv_pair<QT, FMT, 2>(r.w[0], s);
+                w[3] = kv_pair<QT, FMT, 3>(r.w[0], s);
+            }
+            if constexpr (VD >= 16) {
+                w[4] = kv_pair<QT, FMT, 0>(r.w[1], s);
+                w[5] = kv_pair<QT, FMT, 1>(r.w[1], s);
+                w[6] = kv_pair<QT, FMT, 2>(r.w[1], s);
+                w[7] = kv_pair<QT, FMT, 3>(r.w[1], s);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VD / 2; ++i) {
+            const uint32_t x = w[i];
+            if constexpr (QT == HF_DT_BF16) {
+                v[2 * i] = __uint_as_float(x << 16);
+                v[2 * i + 1] = __uint_as_float(x & 0xFFFF0000u);
+            } else {
+                const f16x2 h = __builtin_bit_cast(f16x2, x);
+                v[2 * i] = (float)h.x;
+                v[2 * i + 1] = (float)h.y;
+            }
+        }
+    }
+
     // A step: 32 tokens from t.  FULL: every row sees all of them.
     template <bool FULL>
     __device__ __forceinline__ void step(const uint32_t t, const tile& x, const int32_t row_lo,
@@ -575,10 +668,10 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
     constexpr uint32_t tile_rows = 16 * R;
     __shared__ kv_lds<DP, R> lds;
     kv_cut cut;
-    if (!kv_find(a, tile_rows, blockIdx.x, cut)) return;
+    if (!kv_find(a, tile_rows, cut)) return;
     U u(a);
     u.q = hf_kv_sequence(a.s, cut.b, a.c.page_shift);
-    const uint32_t in_seq = blockIdx.x - cut.n_before;
+    const uint32_t in_seq = cut.unit - cut.n_before;
     const uint32_t row_tiles = cut.tiles / a.c.heads;
     const uint32_t range = in_seq / cut.tiles, tile = in_seq % cut.tiles;
     u.head = tile / row_tiles;
@@ -596,6 +689,8 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
     end = min(end, t_lo + cut.steps_each * kStep);
 
     u.load_q(row_lo, rows);
+#pragma unroll
+    for (int r = 0; r < R; ++r) kv_arrived(u.qr[r]);
     uint32_t t = t_lo + kStep * (uint32_t)wave;
     if (t < end) {
         constexpr uint32_t stride = kStep * kWaves;
@@ -660,7 +755,7 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
         const int32_t i = row_lo + 16 * r + u.m;
         if (cut.ranges > 1) {  // to be joined with the other ranges
             if (i >= rows) continue;
-            const int64_t row = (int64_t)blockIdx.x * tile_rows + 16 * r + u.m;
+            const int64_t row = (int64_t)cut.unit * tile_rows + 16 * r + u.m;
             float* dst = a.part + row * DP;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -702,47 +797,21 @@ template <int QT, int DP>
 __global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a, const uint32_t tile_rows) {
     typedef kv_type<QT> T;
     constexpr uint32_t cols = DP / 4, deal = 64 / cols;
-    const uint32_t each = kv_steps_each(a, tile_rows);
     const uint32_t q_heads = a.c.heads * a.per;
     const uint32_t id = blockIdx.x * 4u + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int32_t row = (int32_t)(id / q_heads);
     const uint32_t out_head = id % q_heads;
     if ((uint32_t)row >= a.s.rows) return;
-    // the sequence of the row, and the units before it
-    uint32_t before = 0;
-    bool found = false;
-    hf_kv_seq q;
-    uint32_t tiles = 0, ranges = 0;
-    for (uint32_t b0 = 0; b0 < a.s.batch && !found; b0 += 64) {
-        const uint32_t b = b0 + hf_lane();
-        uint32_t nt = 0, steps = 0;
-        bool mine = false;
-        if (b < a.s.batch) {
-            const hf_kv_seq s = hf_kv_sequence(a.s, b, a.c.page_shift);
-            nt = s.n > 0 ? a.c.heads * (((uint32_t)s.n * a.per + tile_rows - 1u) / tile_rows) : 0u;
-            steps = ((uint32_t)s.len + kStep - 1u) / kStep;
-            mine = row >= s.row0 && row < s.row0 + s.n;
-        }
-        const uint32_t nr = kv_ranges(steps, each);
-        uint32_t units = nt * nr, incl = units;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t up = __shfl_up(incl, o);
-            if (hf_lane() >= o) incl += up;
-        }
-        const unsigned long long hit = __ballot(mine);
-        if (hit) {
-            const int l = __ffsll((unsigned long long)hit) - 1;
-            found = true;
-            q = hf_kv_sequence(a.s, b0 + l, a.c.page_shift);
-            before += __builtin_amdgcn_readlane(incl - units, l);
-            tiles = __builtin_amdgcn_readlane(nt, l);
-            ranges = __builtin_amdgcn_readlane(nr, l);
-        } else {
-            before += __builtin_amdgcn_readlane(incl, 63);
-        }
-    }
+    const kv_plan_dev p = kv_plan_now(a, tile_rows);
+    kv_cut cut;
+    const bool found = kv_walk(a, tile_rows, p, [&](uint32_t b, uint32_t, uint32_t) {
+        if (b >= a.s.batch) return false;
+        const hf_kv_seq s = hf_kv_sequence(a.s, b, a.c.page_shift);
+        return row >= s.row0 && row < s.row0 + s.n;
+    }, cut);
+    const uint32_t tiles = cut.tiles, ranges = cut.ranges, before = cut.n_before;
     if (!found || ranges < 2) return;
+    const hf_kv_seq q = hf_kv_sequence(a.s, cut.b, a.c.page_shift);
     const uint32_t i = (uint32_t)(row - q.row0) * a.per + out_head % a.per;
     const uint32_t tile = out_head / a.per * (tiles / a.c.heads) + i / tile_rows;
     // (offsets that cover a row twice, which the attending kernel reports, can count more units

@@ -10,7 +10,7 @@ void hf_launch_kv_attend_fp4_e2m1(const hf_kv_attend_args&, int, int, hipStream_
 int hf_kv_attend_tile_rows(uint32_t max_q, uint32_t per, uint32_t head_dim) {
     const uint64_t rows = (uint64_t)max_q * per;
     if (rows <= 16) return 16;
-    return rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 || head_dim > 128 ? 128 : 256;
 }
 
 void hf_launch_kv_attend(const hf_kv_attend_args& a, int dtype, int format, int tile_rows,

@@ -1,17 +1,23 @@
 // Attention of many rows (a drafted tree, a chunk of a prompt) over quantised pages: like
-// hf_k_kv_attend, but the WR wavefronts of a workgroup have 32 rows each and share what they read.
+// hf_k_kv_attend, but the wavefronts of a workgroup share what they read.
 //
-// The workgroup takes TT tokens at a time: its wavefronts load the codes, turn them into 16-bit
-// operands once (a conversion that applies the scale, and byte permutes for V) and put them into LDS,
-// K as [token][d], V transposed as [d][token]; then every wavefront multiplies its own rows with
-// them.  The codes of the next tokens are loaded into registers while the present ones are in use.
+// WR x WS wavefronts: WR groups of 32 rows, and for each WS wavefronts that take the tokens 32 at a
+// time in turn.  The workgroup takes TT tokens at a time: its wavefronts load the codes, turn them
+// into 16-bit operands once (a conversion that applies the scale, and byte permutes for V) and put
+// them into LDS, K as [token][d], V transposed as [d][token]; then every wavefront multiplies its own
+// rows with them.  The codes of the next tokens are loaded into registers while the present ones are
+// in use.
 //   S^T = K Q^T    32 tokens x 32 rows: a lane has, of row lane % 32, sixteen tokens
 //   O^T = V^T P^T  needs eight tokens of the lane's row as operand B, in registers, as it has them: K's
 //                  tokens are read in an order (bits 2 and 3 of a token's number swapped) that makes
 //                  them eight neighbours, sixteen bytes of a row of V^T
 // 16-byte pieces of a row are stored at their number XOR a number of the row, such that sixteen lanes
 // that read or write the same column of sixteen rows meet sixteen different places of the banks.
+// Everything is meant to stay in registers: a spilled address is reloaded behind the loads under way,
+// and its wait is theirs.
 #pragma once
+
+#include <type_traits>
 
 #include "hf_kv_attend.h"
 
@@ -30,37 +36,26 @@ __device__ __forceinline__ f32x16 kv_mma32(hf_u32x4 a, hf_u32x4 b, f32x16 c) {
 template <int QT>
 __device__ __forceinline__ float kv_add_pair(const uint32_t pair, const float a) {
     constexpr uint32_t two = kv_type<QT>::one | kv_type<QT>::one << 16;
-    if constexpr (QT == HF_DT_BF16) {
-        typedef short s16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (QT == HF_DT_BF16)
         return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, two), a, false);
-    } else {
+    else
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), __builtin_bit_cast(f16x2, two), a, false);
-    }
 }
 
 template <int DP, int TT>
 struct kv_share {
     hf_u32x4 k[TT][DP / 8];
     hf_u32x4 v[DP][TT / 8];
-    uint32_t odd[TT / 32];  // values that are not finite, per 32 tokens
+};
+// What WS - 1 wavefronts of a row group hand to the first.
+template <int DP, int WR, int WS>
+struct kv_hand {
+    float acc[WS > 1 ? WS - 1 : 1][WS > 1 ? WR : 1][WS > 1 ? DP / 2 : 1][64];
+    float st[WS > 1 ? WS - 1 : 1][WS > 1 ? WR : 1][3][64];
 };
 
-template <int QT, int FMT, int DP, int WR>
-struct kv_block {
-    typedef kv_type<QT> T;
-    typedef kv_unit<QT, FMT, DP, 1> U;
-    static constexpr int TT = WR == 1 ? 32 : 64;
-    static constexpr int bits = kv_bits<FMT>();
-    static constexpr int VD = DP / 16, KS = DP / 16, NB = DP / 32, NT = TT / 32;
-    static constexpr int CH = TT / 8;  // 16-byte pieces of a row of V^T
-    // a wavefront stages K or V of 32 tokens: parts of all of them, and of one
-    static constexpr int parts = 2 * NT, own = parts / WR;
-    static_assert(own >= 1 && own * WR == parts, "staging is dealt evenly");
-
-};
-
-// A part as loaded: K of 32 tokens (two tokens of the lane, KP pieces each) or V (eight tokens), and
-// their scale bytes, in the same registers.
+// A part of the staging, a wavefront's work: K of 32 tokens (two tokens of the lane, KP pieces of
+// each) or V of 32 tokens (eight tokens of the lane), with their scale bytes, as loaded.
 template <int QT, int FMT, int DP>
 struct kv_part {
     typedef kv_unit<QT, FMT, DP, 1> U;
@@ -70,117 +65,26 @@ struct kv_part {
     hf_u32x2 s[U::bits == 16 ? 1 : 2 * U::KP];
 };
 
-// Loads of a wavefront's K part: tokens t + 16 b + m of 32, d in pieces as in kv_unit.
-template <int QT, int FMT, int DP>
-__device__ __forceinline__ void kv_load_k(const kv_unit<QT, FMT, DP, 1>& u, const hf_kv_attend_args& a, const uint32_t t,
-                                          const int32_t (&pages)[2], kv_part<QT, FMT, DP>& x, uint32_t& bad) {
-    typedef kv_unit<QT, FMT, DP, 1> U;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        int32_t page = pages[b];
-        if ((uint32_t)page >= a.c.n_pages) { bad = 1; page = 0; }
-        const uint32_t off = u.group_at(t + 16u * b + 8u * (u.m >> 3)) & ((1u << a.c.page_shift) - 1u);
-        const hf_g8* p = (const hf_g8*)a.c.k + (int64_t)page * a.c.page_stride +
-                         (int64_t)(off + (u.m & 7)) * a.c.token_stride + (int64_t)u.head * a.c.head_stride;
-        const int64_t sc = (((int64_t)page * a.c.heads + u.head) * a.c.groups << a.c.page_shift) + off;
-#pragma unroll
-        for (int h = 0; h < U::KP; ++h) {
-            const int d = 4 * U::DPC * h + U::DPC * u.g;
-            kv_raw<U::KB> r;
-            if (d < (int)a.c.head_dim) r.load(p + d * U::bits / 8);
-            else r.clear();
-#pragma unroll
-            for (int i = 0; i < U::KB / 4; ++i) x.w[(b * U::KP + h) * (U::KB / 4) + i] = r.w[i];
-            if constexpr (U::bits != 16) {
-                x.s[2 * h + b] = hf_u32x2{0, 0};
-                if (d < (int)a.c.head_dim)
-                    x.s[2 * h + b] = *(const hf_gmem_u32x2*)((const hf_g8*)a.c.k_scale + sc +
-                                                        ((int64_t)(d >> a.c.group_shift) << a.c.page_shift));
-            }
-        }
-    }
-}
-template <int QT, int FMT, int DP>
-__device__ __forceinline__ void kv_load_v(const kv_unit<QT, FMT, DP, 1>& u, const hf_kv_attend_args& a, const uint32_t t,
-                                          int32_t page, kv_part<QT, FMT, DP>& x, uint32_t& bad) {
-    typedef kv_unit<QT, FMT, DP, 1> U;
-    if ((uint32_t)page >= a.c.n_pages) { bad = 1; page = 0; }
-    const uint32_t off = u.group_at(t + 8u * u.g) & ((1u << a.c.page_shift) - 1u);
-    const hf_g8* p = (const hf_g8*)a.c.v + (int64_t)page * a.c.page_stride + (int64_t)off * a.c.token_stride +
-                     (int64_t)u.head * a.c.head_stride + U::VB * u.m;
-    const bool on = U::VD * u.m < (int)a.c.head_dim;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        kv_raw<U::VB> r;
-        if (on) r.load(p);
-        else r.clear();
-#pragma unroll
-        for (int i = 0; i < kv_part<QT, FMT, DP>::vw; ++i) x.w[j * kv_part<QT, FMT, DP>::vw + i] = r.w[i];
-        p += a.c.token_stride;
-    }
-    if constexpr (U::bits != 16) {
-        x.s[0] = hf_u32x2{0, 0};
-        if (on)
-            x.s[0] = *(const hf_gmem_u32x2*)((const hf_g8*)a.c.v_scale +
-                                          (((int64_t)page * a.c.heads + u.head) * a.c.groups << a.c.page_shift) + off +
-                                          ((int64_t)((U::VD * u.m) >> a.c.group_shift) << a.c.page_shift));
-    }
-}
-
-// A K part into LDS: piece c of token row at c ^ (row % 16).
-template <int QT, int FMT, int DP, int TT>
-__device__ __forceinline__ void kv_store_k(const kv_unit<QT, FMT, DP, 1>& u, const int at,
-                                           const kv_part<QT, FMT, DP>& x, kv_share<DP, TT>& lds) {
-    typedef kv_unit<QT, FMT, DP, 1> U;
-    constexpr int per = U::DPC / 8;  // 16-byte pieces that a loaded piece becomes
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        const int row = at + 16 * b + u.m;
-#pragma unroll
-        for (int h = 0; h < U::KP; ++h) {
-            float f = 0.0f;
-            if constexpr (U::bits != 16) {
-                const uint32_t w = u.m & 4 ? x.s[2 * h + b].y : x.s[2 * h + b].x;
-                f = __uint_as_float(__builtin_amdgcn_ubfe(w, 8u * (u.m & 3), 8u) << 23);
-            }
-            const uint32_t* kw = x.w + (b * U::KP + h) * (U::KB / 4);
-#pragma unroll
-            for (int i = 0; i < per; ++i) {
-                hf_u32x4 o;
-                if constexpr (U::bits == 16) {
-                    o = hf_u32x4{kw[0], kw[1], kw[2], kw[3]};
-                } else if constexpr (U::bits == 8) {
-                    o[0] = kv_pair<QT, FMT, 0>(kw[2 * i], f);
-                    o[1] = kv_pair<QT, FMT, 1>(kw[2 * i], f);
-                    o[2] = kv_pair<QT, FMT, 0>(kw[2 * i + 1], f);
-                    o[3] = kv_pair<QT, FMT, 1>(kw[2 * i + 1], f);
-                } else {
-                    o[0] = kv_pair<QT, FMT, 0>(kw[i], f);
-                    o[1] = kv_pair<QT, FMT, 1>(kw[i], f);
-                    o[2] = kv_pair<QT, FMT, 2>(kw[i], f);
-                    o[3] = kv_pair<QT, FMT, 3>(kw[i], f);
-                }
-                const int c = (4 * U::DPC * h + U::DPC * u.g) / 8 + i;
-                lds.k[row][(c ^ (row & 15)) & (DP / 8 - 1)] = o;
-            }
-        }
-    }
-}
-
-template <int QT, int FMT, int DP, int WR>
-__global__ __launch_bounds__(64 * WR) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2)))
+template <int QT, int FMT, int DP, int WR, int WS, int TT, int NBUF>
+__global__ __launch_bounds__(64 * WR * WS) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2)))
 void hf_k_kv_attend_block(const hf_kv_attend_args a) {
-    typedef kv_block<QT, FMT, DP, WR> B;
     typedef kv_unit<QT, FMT, DP, 1> U;
+    typedef kv_part<QT, FMT, DP> P;
     typedef kv_type<QT> T;
-    constexpr int TT = B::TT, KS = B::KS, NB = B::NB, NT = B::NT, CH = B::CH;
+    constexpr int bits = U::bits, VD = DP / 16, KS = DP / 16, NB = DP / 32, NT = TT / 32, CH = TT / 8;
+    constexpr int waves = WR * WS, own = 2 * NT / waves;  // parts of a wavefront: all K or all V
+    static_assert(own >= 1 && own * waves == 2 * NT && NT % WS == 0, "staging and tokens are dealt evenly");
     constexpr uint32_t tile_rows = 32 * WR;
-    __shared__ kv_share<DP, TT> lds;
+    __shared__ union {
+        kv_share<DP, TT> x[NBUF];
+        kv_hand<DP, WR, WS> hand;
+    } lds;
+    __shared__ uint32_t any_odd;
     kv_cut cut;
-    if (!kv_find(a, tile_rows, blockIdx.x, cut)) return;
+    if (!kv_find(a, tile_rows, cut)) return;
     U u(a);
     u.q = hf_kv_sequence(a.s, cut.b, a.c.page_shift);
-    const uint32_t in_seq = blockIdx.x - cut.n_before;
+    const uint32_t in_seq = cut.unit - cut.n_before;
     const uint32_t row_tiles = cut.tiles / a.c.heads;
     const uint32_t range = in_seq / cut.tiles, tile = in_seq % cut.tiles;
     u.head = tile / row_tiles;
@@ -188,22 +92,24 @@ void hf_k_kv_attend_block(const hf_kv_attend_args a) {
     const int32_t row_lo = (int32_t)(tile % row_tiles * tile_rows);
     u.table = (const hf_gi32*)(a.s.table + (int64_t)cut.b * a.s.table_stride);
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wr = wave % WR, ws = wave / WR;
     const int n = u.lane & 31, kg = u.lane >> 5;
 
     // the wavefront's row of this lane, and how far the wavefront's rows see everything, or anything
-    const int32_t w_lo = row_lo + 32 * wave, i_row = w_lo + n;
+    const int32_t w_lo = row_lo + 32 * wr, i_row = w_lo + n;
     const bool on = i_row < rows;
-    const int32_t tok = (on ? i_row : 0) / (int32_t)a.per, hq = (on ? i_row : 0) % (int32_t)a.per;
+    const int32_t tok = (on ? i_row : 0) / (int32_t)a.per;
     const int32_t last = (min(w_lo + 32, rows) - 1) / (int32_t)a.per;
-    const uint32_t len = (uint32_t)u.q.len;
-    const uint32_t whole = (uint32_t)(a.mask ? u.q.past : u.q.past + w_lo / (int32_t)a.per + 1);
-    const uint32_t some = w_lo >= rows ? 0u : a.mask ? len : (uint32_t)(u.q.past + last + 1);
+    const uint32_t len = (uint32_t)u.q.len, past = (uint32_t)u.q.past;
+    const uint32_t whole = a.mask ? past : past + (uint32_t)(w_lo / (int32_t)a.per) + 1u;
+    const uint32_t some = w_lo >= rows ? 0u : a.mask ? len : past + (uint32_t)last + 1u;
     const int32_t tile_last = (min(row_lo + (int32_t)tile_rows, rows) - 1) / (int32_t)a.per;
     const uint32_t t_lo = range * cut.steps_each * kStep;
-    const uint32_t end = min(t_lo + cut.steps_each * kStep, a.mask ? len : (uint32_t)(u.q.past + tile_last + 1));
+    const uint32_t end = min(t_lo + cut.steps_each * kStep, a.mask ? len : past + (uint32_t)tile_last + 1u);
 
     hf_u32x4 qr[KS];
     {
+        const int32_t hq = (on ? i_row : 0) % (int32_t)a.per;
         const hf_g8* p = (const hf_g8*)a.q.p + ((int64_t)(u.q.row0 + tok) * a.q.row_stride +
                                                 (int64_t)(u.head * a.per + hq) * a.q.head_stride) * 2;
 #pragma unroll
@@ -220,95 +126,178 @@ void hf_k_kv_attend_block(const hf_kv_attend_args a) {
         for (int i = 0; i < 16; ++i) acc[q][i] = 0.0f;
     float nm = 3.402823466e38f, sum = 0.0f, div = 0.0f;  // p = exp2(scale_log2 s + nm)
     uint32_t bad = 0;
+    bool huge = false;  // |nm| where fused exponents would not do
 
-    // the wavefront's parts of the staging: K halves first, then V halves
-    constexpr int own = B::own;
-    kv_part<QT, FMT, DP> part[own];
-    const bool does_k = own > 1 || wave < WR / 2;  // one part each: half of the wavefronts K, half V
-    const bool does_v = own > 1 || !does_k;
-    auto part_at = [&](const int i) { return own > 1 ? wave * (own / 2) + i : wave % NT; };
-    int32_t kpage[own > 1 ? own / 2 : 1][2], vpage[own > 1 ? own / 2 : 1];
+    // The staging of a wavefront: K parts for the first half of the wavefronts, V for the others.  A
+    // part's place is the lane's own (fixed) plus its page and its first token's place in the page.
+    // Where head_dim ends inside the padded one, the lanes behind it load other d of their token: of
+    // K the values are cleared, of V they make outputs that nobody takes.
+    const bool is_k = wave < waves / 2;
+    const int part0 = 32 * own * (is_k ? wave : wave - waves / 2);  // its first token in the tile
+    const uint32_t in_page = (1u << a.c.page_shift) - 1u;
+    const uint32_t page_scales = a.c.heads * a.c.groups << a.c.page_shift;
+    const int my_d = is_k ? U::DPC * u.g : VD * u.m;
+    const int my_off = is_k ? u.m & 7 : 0;  // token in a group of eight
+    const int my_grp = 8 * (is_k ? u.m >> 3 : u.g);
+    const bool cuts = a.c.head_dim < (uint32_t)DP;
+    const hf_g8* const base = (const hf_g8*)(is_k ? a.c.k : a.c.v) + (int64_t)my_off * a.c.token_stride +
+                              (int64_t)u.head * a.c.head_stride + (my_d < (int)a.c.head_dim ? my_d * bits / 8 : 0);
+    const hf_g8* const sbase = (const hf_g8*)(is_k ? a.c.k_scale : a.c.v_scale) +
+                               ((int64_t)u.head * a.c.groups << a.c.page_shift) +
+                               ((int64_t)((my_d < (int)a.c.head_dim ? my_d : 0) >> a.c.group_shift) << a.c.page_shift);
+    P part[own];
+    int32_t page[own][2];
     auto find_pages = [&](const uint32_t t) {
 #pragma unroll
-        for (int i = 0; i < (own > 1 ? own / 2 : 1); ++i) {
-            const uint32_t at = t + 32u * part_at(i);
-            if (does_k) {
-                kpage[i][0] = u.page_at(at + 8u * (u.m >> 3));
-                kpage[i][1] = u.page_at(at + 16u + 8u * (u.m >> 3));
-            }
-            if (does_v) vpage[i] = u.page_at(at + 8u * u.g);
+        for (int i = 0; i < own; ++i) {
+            page[i][0] = u.page_at(t + part0 + 32 * i + my_grp);
+            if (is_k) page[i][1] = u.page_at(t + part0 + 32 * i + 16 + my_grp);
         }
+    };
+    // row of codes and of scale bytes of the lane's token(s) from `at` on
+    auto place = [&](const uint32_t at, const int32_t page_id, const hf_g8*& p, const hf_g8*& sp) {
+        uint32_t pg = (uint32_t)page_id;
+        if (pg >= a.c.n_pages) {
+            bad = 1;
+            pg = 0;
+        }
+        const uint32_t off = u.group_at(at) & in_page;
+        p = base + (uint64_t)pg * (uint32_t)a.c.page_stride + (uint64_t)off * (uint32_t)a.c.token_stride;
+        sp = sbase + (uint64_t)pg * page_scales + off;
     };
     auto load = [&](const uint32_t t) {
 #pragma unroll
-        for (int i = 0; i < (own > 1 ? own / 2 : 1); ++i) {
-            const uint32_t at = t + 32u * part_at(i);
-            if (does_k) kv_load_k<QT, FMT, DP>(u, a, at, kpage[i], part[i], bad);
-            if (does_v) kv_load_v<QT, FMT, DP>(u, a, at, vpage[i], part[own - 1 - i], bad);
+        for (int i = 0; i < own; ++i) {
+            const uint32_t at = t + part0 + 32 * i + my_grp;
+            const hf_g8 *p, *sp;
+            if (is_k) {
+                const int d0 = my_d < (int)a.c.head_dim ? my_d : 0;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    place(at + 16 * b, page[i][b], p, sp);
+#pragma unroll
+                    for (int h = 0; h < U::KP; ++h) {
+                        // (uniform where nothing is cut: then a constant offset)
+                        const int d = cuts && my_d + 4 * U::DPC * h >= (int)a.c.head_dim ? 0 : 4 * U::DPC * h;
+                        kv_raw<U::KB> r;
+                        r.load(p + d * bits / 8);
+#pragma unroll
+                        for (int e = 0; e < P::kw; ++e) part[i].w[(b * U::KP + h) * P::kw + e] = r.w[e];
+                        if constexpr (bits != 16)
+                            part[i].s[2 * h + b] = *(const hf_gmem_u32x2*)(
+                                sp + ((((d0 + d) >> a.c.group_shift) - (d0 >> a.c.group_shift)) << a.c.page_shift));
+                    }
+                }
+            } else {
+                place(at, page[i][0], p, sp);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    kv_raw<U::VB> r;
+                    r.load(p);
+#pragma unroll
+                    for (int e = 0; e < P::vw; ++e) part[i].w[j * P::vw + e] = r.w[e];
+                    p += a.c.token_stride;
+                }
+                if constexpr (bits != 16) part[i].s[0] = *(const hf_gmem_u32x2*)sp;
+            }
         }
     };
-    const int swz = n & ~12, krow = swz | (n & 4) << 1 | (n & 8) >> 1;  // bits 2 and 3 swapped
-    const int vf = (n / (16 / CH)) % CH;
-
-    if (t_lo < end) {
-        find_pages(t_lo);
-        load(t_lo);
-        find_pages(t_lo + TT);
-    }
-    for (uint32_t t = t_lo; t < end; t += TT) {
-        __syncthreads();
+    // Operands of the parts into LDS.  EDGE: some of the tokens may be behind the last one, where
+    // nothing is known of what a page holds, or not seen by every row: what is not finite is left out
+    // here, so that it does not reach other rows as 0 x infinity, and added at the end.
+    auto stage = [&](const uint32_t t, kv_share<DP, TT>& to, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
 #pragma unroll
-        for (int i = 0; i < (own > 1 ? own / 2 : 1); ++i) {
-            const int at = 32 * part_at(i);
-            if (does_k) kv_store_k<QT, FMT, DP, TT>(u, at, part[i], lds);
-            if (does_v) {
-                hf_u32x4 av[B::VD];
-                const int32_t left = min(max(u.q.len - (int32_t)(t + at + 8u * u.g), 0), 8);
-                typename U::tile x;
+        for (int i = 0; i < own; ++i) {
+            const int at = part0 + 32 * i;
+            if (is_k) {
+                constexpr int per = U::DPC / 8;  // 16-byte pieces that a loaded piece becomes
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int row = at + 16 * b + u.m;
+#pragma unroll
+                    for (int h = 0; h < U::KP; ++h) {
+                        float f = 0.0f;
+                        if constexpr (bits != 16) {
+                            const uint32_t w = u.m & 4 ? part[i].s[2 * h + b].y : part[i].s[2 * h + b].x;
+                            f = __uint_as_float(__builtin_amdgcn_ubfe(w, 8u * (u.m & 3), 8u) << 23);
+                        }
+                        uint32_t kw[P::kw];
+#pragma unroll
+                        for (int e = 0; e < P::kw; ++e) kw[e] = part[i].w[(b * U::KP + h) * P::kw + e];
+#pragma unroll
+                        for (int c = 0; c < per; ++c) {
+                            hf_u32x4 o;
+                            if constexpr (bits == 16) {
+                                o = hf_u32x4{kw[0], kw[1], kw[2], kw[3]};
+                            } else if constexpr (bits == 8) {
+                                o[0] = kv_pair<QT, FMT, 0>(kw[2 * c], f);
+                                o[1] = kv_pair<QT, FMT, 1>(kw[2 * c], f);
+                                o[2] = kv_pair<QT, FMT, 0>(kw[2 * c + 1], f);
+                                o[3] = kv_pair<QT, FMT, 1>(kw[2 * c + 1], f);
+                            } else {
+                                o[0] = kv_pair<QT, FMT, 0>(kw[c], f);
+                                o[1] = kv_pair<QT, FMT, 1>(kw[c], f);
+                                o[2] = kv_pair<QT, FMT, 2>(kw[c], f);
+                                o[3] = kv_pair<QT, FMT, 3>(kw[c], f);
+                            }
+                            const int d = 4 * U::DPC * h + U::DPC * u.g;
+                            if (cuts && d >= (int)a.c.head_dim) o = hf_u32x4{0, 0, 0, 0};
+                            to.k[row][((d / 8 + c) ^ (row & 15)) & (DP / 8 - 1)] = o;
+                        }
+                    }
+                }
+            } else {
+                hf_u32x4 av[VD];
+                typename U::tile v;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int e = 0; e < kv_part<QT, FMT, DP>::vw; ++e)
-                        x.v[j].w[e] = part[own - 1 - i].w[j * kv_part<QT, FMT, DP>::vw + e];
-                x.vs = part[own - 1 - i].s[0];
-                u.columns(x, (1u << left) - 1u, av);
-                uint32_t odd = 0;
+                    for (int e = 0; e < P::vw; ++e) v.v[j].w[e] = part[i].w[j * P::vw + e];
+                v.vs = part[i].s[0];
+                uint32_t there = 0xFFu;
+                if constexpr (EDGE) there = (1u << min(max(u.q.len - (int32_t)(t + at + 8u * u.g), 0), 8)) - 1u;
+                u.columns(v, there, av);
+                if constexpr (EDGE) {
+                    bool odd = false;
 #pragma unroll
-                for (int c = 0; c < B::VD; ++c) {
+                    for (int c = 0; c < VD; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t hit = ((av[c][e] & T::expo) + T::unit) & 0x80008000u;
+                            odd = odd || hit;
+                            av[c][e] &= ~((hit >> 15) * 0xFFFFu);
+                        }
+                    if (__ballot(odd) && u.lane == 0) any_odd = 1;
+                }
+#pragma unroll
+                for (int c = 0; c < VD; ++c) {
                     const int row = 16 * c + u.m;
-                    lds.v[row][(at / 8 + u.g) ^ ((row / (16 / CH)) % CH)] = av[c];
+                    to.v[row][(at / 8 + u.g) ^ ((row / (16 / CH)) % CH)] = av[c];
                 }
-                if (t + TT > (uint32_t)u.q.past) {  // (only where rows see different tokens)
-#pragma unroll
-                    for (int c = 0; c < B::VD; ++c)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) odd |= ((av[c][e] & T::expo) + T::unit) & 0x80008000u;
-                }
-                const bool any = __ballot(odd != 0) != 0;
-                if (u.lane == 0) lds.odd[at / 32] = any;
             }
         }
-        if (t + TT < end) {
-            load(t + TT);
-            find_pages(t + 2 * TT);
-        }
-        __syncthreads();
-        if (t >= some) continue;
-        // 32 tokens after the other: half the scores and weights in registers at a time
-#pragma unroll
-        for (int b = 0; b < NT; ++b) {
-            const uint32_t tb = t + 32 * b;
-            const bool full = tb + 32 <= whole && tb + 32 <= end;
+    };
+    const int krow = (n & ~12) | (n & 4) << 1 | (n & 8) >> 1;  // bits 2 and 3 swapped
+    const int vf = (n / (16 / CH)) % CH;
+
+    // The wavefront's tokens of a tile against its rows, 32 after the other (so that half of the scores
+    // and weights are in registers at a time).  FULL: every row sees all of them.
+    auto multiply = [&](const uint32_t t, const kv_share<DP, TT>& x, auto is_full) {
+        constexpr bool FULL = decltype(is_full)::value;
+#pragma unroll 1
+        for (int bi = 0; bi < NT / WS; ++bi) {
+            const int b = bi * WS + ws;
             f32x16 s;
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
-                s = kv_mma32<QT>(lds.k[32 * b + krow][((2 * ks + kg) ^ (krow & 15)) & (DP / 8 - 1)], qr[ks], s);
-            if (!full) {
+                s = kv_mma32<QT>(x.k[32 * b + krow][((2 * ks + kg) ^ (krow & 15)) & (DP / 8 - 1)], qr[ks], s);
+            if constexpr (!FULL) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t see = u.seen_at(tok, tb + 16 * h + 8 * kg, on);
+                    const uint32_t see = u.seen_at(tok, t + 32 * b + 16 * h + 8 * kg, on);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) s[8 * h + j] = see >> j & 1u ? s[8 * h + j] : -__builtin_inff();
                 }
@@ -325,106 +314,144 @@ void hf_k_kv_attend_block(const hf_kv_attend_args a) {
                 div *= f;
 #pragma unroll
                 for (int q = 0; q < NB; ++q) acc[q] *= f;
+                huge = __ballot(fabsf(nm) > 65536.0f && nm != 3.402823466e38f) != 0;
             }
             // (fused: the error of scale x maximum is the same factor for the whole row; where it
             // could pass 1 / 256 of a power of two, the products are rounded first, as the maximum's was)
-            if (__ballot(fabsf(nm) > 65536.0f && nm != 3.402823466e38f)) {
+            if (huge) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = s[i] * a.scale_log2 + nm;
             } else {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], a.scale_log2, nm);
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]);
-            if (a.lse) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sum += s[i];
-            }
             hf_u32x4 p[2];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[i] = __builtin_amdgcn_exp2f(s[i]);
+                sum += s[i];
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 p[i / 4][i % 4] = T::pack(s[2 * i], s[2 * i + 1]);
                 div = kv_add_pair<QT>(p[i / 4][i % 4], div);
             }
-            if (full || lds.odd[b] == 0) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int q = 0; q < NB; ++q)
-                        acc[q] = kv_mma32<QT>(lds.v[32 * q + n][(4 * b + 2 * h + kg) ^ vf], p[h], acc[q]);
-            } else {
-                // infinities and NaN of tokens that some rows may not see (kv_unit::not_finite)
+                for (int q = 0; q < NB; ++q)
+                    acc[q] = kv_mma32<QT>(x.v[32 * q + n][(4 * b + 2 * h + kg) ^ vf], p[h], acc[q]);
+        }
+    };
+
+    if (threadIdx.x == 0) any_odd = 0;
+    __syncthreads();
+    kv_arrived(qr);
+    auto stage_at = [&](const uint32_t t, kv_share<DP, TT>& to) {
+        if (t + TT > past) stage(t, to, std::true_type{});
+        else stage(t, to, std::false_type{});
+        if (t + TT < end) {
+            load(t + TT);
+            find_pages(t + 2 * TT);
+        }
+    };
+    if (t_lo < end) {
+        find_pages(t_lo);
+        load(t_lo);
+        find_pages(t_lo + TT);
+        if constexpr (NBUF == 2) stage_at(t_lo, lds.x[0]);
+    }
+    int buf = 0;
+    for (uint32_t t = t_lo; t < end; t += TT) {
+        __syncthreads();  // tile t is in its half, and nobody reads the other any more
+        if constexpr (NBUF == 2) {
+            if (t + TT < end) stage_at(t + TT, lds.x[buf ^ 1]);
+        } else {
+            stage_at(t, lds.x[0]);
+            __syncthreads();
+        }
+        if (t + TT <= whole) multiply(t, lds.x[buf], std::true_type{});
+        else if (t < some) multiply(t, lds.x[buf], std::false_type{});
+        buf ^= NBUF - 1;
+    }
+    __syncthreads();
+    if (bad) atomicOr(a.err, HF_KERR_CORRUPT);
+    if (any_odd) {
+        // What was left out: of the tokens staged as EDGE, the values that are not finite.
 #pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
-                    const hf_u32x4 ph = h ? p[1] : p[0];
-                    const uint32_t see = u.seen_at(tok, tb + 16 * h + 8 * kg, on);
-                    hf_u32x4 ones;
+        for (uint32_t t = max(t_lo, past / TT * TT); t < min(end, some); ++t) {
+            if (ws != (int)(t / 32 % WS)) continue;
+            const int32_t pg = u.page_at(t);
+            const bool sees = on && (t < past || (u.seen_at(tok, t, on) & 1u));
+            if ((uint32_t)pg >= a.c.n_pages || !sees) continue;
+            const uint32_t off = t & in_page;
+            const hf_g8* p = (const hf_g8*)a.c.v + (int64_t)pg * a.c.page_stride + (int64_t)off * a.c.token_stride +
+                             (int64_t)u.head * a.c.head_stride;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        ones[i] = (see >> (2 * i) & 1u ? T::one : 0u) | (see >> (2 * i + 1) & 1u ? T::one << 16 : 0u);
+            for (int e = 0; e < 8; ++e) {
+                const int m = 8 * (e >> 2) + 4 * kg + (e & 3), d = VD * m;
+                if (d < (int)a.c.head_dim) {
+                    float v[VD];
+                    u.values(p + d * bits / 8, pg, off, d, v);
 #pragma unroll
-                    for (int q = 0; q < NB; ++q) {
-                        hf_u32x4 av = lds.v[32 * q + n][(4 * b + 2 * h + kg) ^ vf];
-#pragma unroll 1
-                        for (int kind = 0; kind < 3; ++kind) {
-                            const uint32_t want = kind == 1 ? T::inf : T::inf | 0x8000u;
-                            hf_u32x4 is;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t lo = av[i] & 0xFFFFu, hi = av[i] >> 16;
-                                const bool l = kind == 0 ? (lo & 0x7FFFu) > T::inf : lo == want;
-                                const bool r = kind == 0 ? (hi & 0x7FFFu) > T::inf : hi == want;
-                                is[i] = (l ? T::one : 0u) | (r ? T::one << 16 : 0u);
-                            }
-                            f32x16 count;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) count[i] = 0.0f;
-                            count = kv_mma32<QT>(is, ones, count);
-                            const float add = kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (count[i] > 0.0f) acc[q][i] += add;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if ((av[i] & 0x7FFFu) >= T::inf) av[i] &= 0xFFFF0000u;
-                            if ((av[i] >> 16 & 0x7FFFu) >= T::inf) av[i] &= 0xFFFFu;
-                        }
-                        acc[q] = kv_mma32<QT>(av, ph, acc[q]);
-                    }
+                    for (int c = 0; c < VD; ++c)
+                        if (!(fabsf(v[c]) <= 3.402823466e38f)) acc[c / 2][8 * (c & 1) + e] += v[c];
                 }
             }
         }
     }
-    if (bad) atomicOr(a.err, HF_KERR_CORRUPT);
     sum += __shfl_xor(sum, 32);
     div += __shfl_xor(div, 32);
+    if constexpr (WS > 1) {  // the wavefronts of a row group, in order
+        if (ws > 0) {
+            lds.hand.st[ws - 1][wr][0][u.lane] = nm;
+            lds.hand.st[ws - 1][wr][1][u.lane] = sum;
+            lds.hand.st[ws - 1][wr][2][u.lane] = div;
+#pragma unroll
+            for (int q = 0; q < NB; ++q)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) lds.hand.acc[ws - 1][wr][16 * q + i][u.lane] = acc[q][i];
+        }
+        __syncthreads();
+        if (ws > 0) return;
+#pragma unroll 1
+        for (int w = 0; w < WS - 1; ++w) {
+            const float other = lds.hand.st[w][wr][0][u.lane], least = fminf(nm, other);
+            const float f = __builtin_amdgcn_exp2f(least - nm), h = __builtin_amdgcn_exp2f(least - other);
+            nm = least;
+            sum = sum * f + lds.hand.st[w][wr][1][u.lane] * h;
+            div = div * f + lds.hand.st[w][wr][2][u.lane] * h;
+#pragma unroll
+            for (int q = 0; q < NB; ++q)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[q][i] = acc[q][i] * f + lds.hand.acc[w][wr][16 * q + i][u.lane] * h;
+        }
+    }
     if (!on) return;
     // the lane's outputs: for each of eight m, VD neighbouring d: VD m + 2 q + i / 8
     if (cut.ranges > 1) {
-        const int64_t row = (int64_t)blockIdx.x * tile_rows + 32 * wave + n;
+        const int64_t row = (int64_t)cut.unit * tile_rows + 32 * wr + n;
         float* dst = a.part + row * DP;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int m = 8 * (e >> 2) + 4 * kg + (e & 3);
 #pragma unroll
             for (int q = 0; q < NB; q += 2)
-                *(f32x4*)(dst + B::VD * m + 2 * q) = f32x4{acc[q][e], acc[q][8 + e], acc[q + 1][e], acc[q + 1][8 + e]};
+                *(f32x4*)(dst + VD * m + 2 * q) = f32x4{acc[q][e], acc[q][8 + e], acc[q + 1][e], acc[q + 1][8 + e]};
         }
         if (kg == 0) *(f32x4*)(a.part_ml + 4 * row) = f32x4{nm, sum, div, 0.0f};
     } else {
-        const uint32_t out_head = u.head * a.per + hq;
+        const uint32_t out_head = u.head * a.per + (uint32_t)(i_row % (int32_t)a.per);
         const float f = div == 0.0f ? 0.0f : 1.0f / div;
         hf_g8* dst = (hf_g8*)a.out.p + ((int64_t)(u.q.row0 + tok) * a.out.row_stride +
                                         (int64_t)out_head * a.out.head_stride) * 2;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int m = 8 * (e >> 2) + 4 * kg + (e & 3);
-            if (B::VD * m < (int)a.c.head_dim) {
+            if (VD * m < (int)a.c.head_dim) {
 #pragma unroll
                 for (int q = 0; q < NB; q += 2)
-                    *(hf_gmem_u32x2*)(dst + 2 * (B::VD * m + 2 * q)) =
+                    *(hf_gmem_u32x2*)(dst + 2 * (VD * m + 2 * q)) =
                         hf_u32x2{T::pack(acc[q][e] * f, acc[q][8 + e] * f), T::pack(acc[q + 1][e] * f, acc[q + 1][8 + e] * f)};
             }
         }
@@ -444,11 +471,13 @@ void kv_launch_rows(const hf_kv_attend_args& a, const int tile_rows, hipStream_t
     if (tile_rows == 16)
         hipLaunchKernelGGL((hf_k_kv_attend<QT, FMT, DP, 1>), dim3(a.units), dim3(64 * kWaves), 0, st, a);
     else if (tile_rows == 32)
-        hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 1>), dim3(a.units), dim3(64), 0, st, a);
+        hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 1, 2, 64, DP == 256 ? 1 : 2>), dim3(a.units), dim3(128), 0, st, a);
     else if (tile_rows == 64)
-        hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 2>), dim3(a.units), dim3(128), 0, st, a);
-    else
-        hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 4>), dim3(a.units), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 2, 2, 64, DP == 256 ? 1 : 2>), dim3(a.units), dim3(256), 0, st, a);
+    else if (tile_rows == 128)
+        hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 4, 1, 64, 2>), dim3(a.units), dim3(256), 0, st, a);
+    else if constexpr (DP <= 128)
+        hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 8, 1, 128, 2>), dim3(a.units), dim3(512), 0, st, a);
     kv_join<QT, DP>(a, (uint32_t)tile_rows, st);
 }
 template <int QT, int FMT>
