@@ -1629,13 +1629,14 @@ struct kv_plan {
     int tile_rows;
     uint32_t target, min_steps, units;
     bool join;
-    uint64_t part_floats, bytes;
+    uint64_t part_floats, ml_floats, bytes;
 };
 int kv_plan_of(const hf_ctx* ctx, const hf_kv_pools& p, const hf_kv_seqs& s, uint32_t per, kv_plan* o) {
     o->tile_rows = hf_kv_attend_tile_rows(s.most, per, p.head_dim);
-    // (units per compute unit: short ones even out a ragged batch of single tokens, 198 -> 163 us from
-    // 2 to 6 for 64 sequences of up to 8000; larger tiles pay more for each unit they are cut into)
-    o->target = (uint32_t)ctx->num_cu * (o->tile_rows == 16 ? 6u : o->tile_rows == 32 ? 4u : 2u);
+    // units aimed at: of small tiles six per compute unit, which evens out a ragged batch of single
+    // tokens (64 sequences of up to 8000: 198 us with two, 163 with six); of larger ones what runs at
+    // once, two workgroups of 32 .. 128 rows to a compute unit or one of 256
+    o->target = (uint32_t)ctx->num_cu * (o->tile_rows == 16 ? 6u : o->tile_rows == 256 || p.head_dim > 128 ? 1u : 2u);
     o->min_steps = 4;
     const uint64_t rows = (uint64_t)s.rows * per;
     const uint64_t by_rows = rows / o->tile_rows + s.batch;
@@ -1652,7 +1653,8 @@ int kv_plan_of(const hf_ctx* ctx, const hf_kv_pools& p, const hf_kv_seqs& s, uin
     o->units = (uint32_t)units;
     const uint64_t pad = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
     o->part_floats = o->join ? units * (uint64_t)o->tile_rows * pad : 0;
-    o->bytes = o->join ? 4 * o->part_floats + 16 * units * (uint64_t)o->tile_rows : 0;
+    o->ml_floats = o->join ? 4 * units * (uint64_t)o->tile_rows : 0;
+    o->bytes = o->join ? 4 * (o->part_floats + o->ml_floats) + 16 * ((uint64_t)s.batch + 1) : 0;
     return HF_OK;
 }
 
@@ -1724,7 +1726,8 @@ int hf_kv_attend(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch
     a.mask_words = query->mask_words;
     a.scale_log2 = query->scale * 1.4426950408889634f;
     a.part = (float*)d_work;
-    a.part_ml = (float*)d_work + plan.part_floats;
+    a.part_ml = a.part + plan.part_floats;
+    a.plan = (uint32_t*)(a.part_ml + plan.ml_floats);
     a.target = plan.target;
     a.min_steps = plan.min_steps;
     a.units = plan.units;

@@ -52,6 +52,7 @@ struct hf_kv_attend_args {
     float scale_log2;      // softmax scale x log2(e)
     float* part;           // partial outputs of the units, [units][rows of a tile][padded head_dim]
     float* part_ml;        // their maxima and two sums, [units][rows of a tile][4]
+    uint32_t* plan;        // [batch + 1][4]: the cut, for joining
     uint32_t target;       // units the call is cut into, about
     uint32_t min_steps;    // tokens / 32 a unit has at least
     uint32_t units;        // workgroups of the call, and room of the partial buffers

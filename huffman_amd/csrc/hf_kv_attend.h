@@ -137,22 +137,26 @@ __device__ __forceinline__ void kv_arrived(hf_u32x4 (&x)[N]) {
 
 // ---- the cut of a call into units ---------------------------------------------------------------
 // Every wavefront finds its unit from the device's own lengths, so a captured call follows lengths
-// that change between replays and a ragged batch is cut evenly: all sequences' steps (32 tokens)
-// times their row tiles are summed and divided by the units aimed at, and a sequence has as many
-// equal ranges as it needs for about that many steps (a quarter more is let pass: a range costs its
-// partial outputs).  Units of a sequence are numbered range by range, in it by cache head, in it by
-// row tile, so that the tiles that read the same tokens are neighbours; and since consecutive
-// workgroups go to the eight XCDs in turn, each with an L2 of its own, XCD x takes the x-th eighth of
-// the units.
+// that change between replays and a ragged batch is cut evenly.  All sequences' steps (32 tokens)
+// times their row tiles are summed and divided by the units aimed at; a sequence has as many equal
+// ranges as it needs for about that many steps.  Tiles of 16 rows leave little behind per unit (a
+// range's partial outputs), so their units are many and small.  Larger tiles leave as much as they
+// read, so there are as many units as run at once: where the tiles alone are fewer than half of
+// that, the steps of a range are raised until the units do not start a second round; where they are
+// not, a range may be a quarter longer before it is cut.
+// Units of a sequence are numbered range by range, in it by cache head, in it by row tile, so that
+// the tiles that read the same tokens are neighbours; and since consecutive workgroups go to the
+// eight XCDs in turn, each with an L2 of its own, XCD x takes the x-th eighth of the units.
+// Workgroup 0 leaves the cut in memory for the kernel that joins the ranges.
 struct kv_cut {
     uint32_t unit, b, n_before;  // unit; its sequence; units of the sequences before that
     uint32_t tiles, ranges, steps_each;
 };
 struct kv_shape {
-    uint32_t tiles, steps, ranges;
+    uint32_t tiles, steps;
 };
 __device__ __forceinline__ kv_shape kv_shape_of(const hf_kv_attend_args& a, const uint32_t tile_rows, const uint32_t b) {
-    kv_shape s = {0, 0, 1};
+    kv_shape s = {0, 0};
     if (b < a.s.batch) {
         const hf_kv_seq q = hf_kv_sequence(a.s, b, a.c.page_shift);
         if (q.bad) atomicOr(a.err, HF_KERR_CORRUPT);
@@ -161,8 +165,16 @@ __device__ __forceinline__ kv_shape kv_shape_of(const hf_kv_attend_args& a, cons
     }
     return s;
 }
-__device__ __forceinline__ uint32_t kv_ranges(const kv_shape& s, const uint32_t each) {
-    return max(1u, (s.steps + each - 1u - each / 4u) / each);
+// x / y rounded up for x + y below 2^31; the float quotient is off by at most one
+__device__ __forceinline__ uint32_t kv_div_up(const uint32_t x, const uint32_t y) {
+    const uint32_t z = x + y - 1u;
+    uint32_t q = (uint32_t)((float)z * __builtin_amdgcn_rcpf((float)y));
+    if ((unsigned long long)q * y > z) --q;
+    if ((unsigned long long)(q + 1u) * y <= z) ++q;
+    return q;
+}
+__device__ __forceinline__ uint32_t kv_ranges(const kv_shape& s, const uint32_t each, const uint32_t slack) {
+    return s.steps <= each + slack ? 1u : kv_div_up(s.steps - slack, each);
 }
 __device__ __forceinline__ uint32_t kv_wave_scan(const uint32_t v) {  // inclusive
     uint32_t incl = v;
@@ -173,32 +185,47 @@ __device__ __forceinline__ uint32_t kv_wave_scan(const uint32_t v) {  // inclusi
     }
     return incl;
 }
-// What the whole call comes to: steps of a range, units.
+__device__ __forceinline__ float kv_wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
 struct kv_plan_dev {
-    uint32_t each, total;
+    uint32_t each, slack, total;  // steps of a range, those let pass, units
     kv_shape first;  // of the lane's sequence among the first 64: most calls have no more
 };
 __device__ __forceinline__ kv_plan_dev kv_plan_now(const hf_kv_attend_args& a, const uint32_t tile_rows) {
     kv_plan_dev p;
     p.first = kv_shape_of(a, tile_rows, hf_lane());
-    unsigned long long sum = (unsigned long long)p.first.tiles * p.first.steps;
+    // (the sums decide nothing but the cut, and every wavefront takes the same ones: floats do)
+    float work = (float)p.first.tiles * (float)p.first.steps, tiles = (float)p.first.tiles;
     for (uint32_t b0 = 64; b0 < a.s.batch; b0 += 64) {
         const kv_shape s = kv_shape_of(a, tile_rows, b0 + hf_lane());
-        sum += (unsigned long long)s.tiles * s.steps;
+        work += (float)s.tiles * (float)s.steps;
+        tiles += (float)s.tiles;
     }
-    sum = hf_wave_sum_u64(sum);
-    const unsigned long long each = (sum + a.target - 1u) / a.target;
-    p.each = (uint32_t)max(each, (unsigned long long)a.min_steps);
-    p.first.ranges = kv_ranges(p.first, p.each);
-    uint32_t total = p.first.tiles * p.first.ranges;
-    for (uint32_t b0 = 64; b0 < a.s.batch; b0 += 64) {
-        const kv_shape s = kv_shape_of(a, tile_rows, b0 + hf_lane());
-        total += s.tiles * kv_ranges(s, p.each);
+    work = kv_wave_sum(work);
+    p.each = max((uint32_t)(work / (float)a.target * 1.0001f) + 1u, a.min_steps);
+    p.slack = 0;
+    bool fit = false;
+    if (tile_rows > 16) {
+        fit = 2.0f * kv_wave_sum(tiles) <= (float)a.target;
+        if (!fit) p.slack = p.each / 4u;
     }
-    p.total = hf_wave_sum_u32(total);
+    for (int turn = 0;; ++turn) {
+        uint32_t total = p.first.tiles * kv_ranges(p.first, p.each, p.slack);
+        for (uint32_t b0 = 64; b0 < a.s.batch; b0 += 64) {
+            const kv_shape s = kv_shape_of(a, tile_rows, b0 + hf_lane());
+            total += s.tiles * kv_ranges(s, p.each, p.slack);
+        }
+        p.total = hf_wave_sum_u32(total);
+        if (!fit || turn == 8 || p.total <= a.target) break;
+        p.each += max(1u, p.each / 16u);
+    }
     return p;
 }
-// Walks the sequences 64 at a time; `pick` sees a lane's sequence, its shape and the units before it.
+// Walks the sequences 64 at a time; `pick` sees a lane's sequence, its shape and ranges and the units
+// before it, and says whether it is the one.
 template <typename F>
 __device__ __forceinline__ bool kv_walk(const hf_kv_attend_args& a, const uint32_t tile_rows, const kv_plan_dev& p,
                                         F&& pick, kv_cut& cut) {
@@ -206,33 +233,45 @@ __device__ __forceinline__ bool kv_walk(const hf_kv_attend_args& a, const uint32
     for (uint32_t b0 = 0; b0 < a.s.batch; b0 += 64) {
         const uint32_t b = b0 + hf_lane();
         kv_shape s = p.first;
-        if (b0) {
-            s = kv_shape_of(a, tile_rows, b);
-            s.ranges = kv_ranges(s, p.each);
-        }
-        const uint32_t own = s.tiles * s.ranges, incl = kv_wave_scan(own);
-        const unsigned long long hit = __ballot(pick(b, before + incl - own, own));
+        if (b0) s = kv_shape_of(a, tile_rows, b);
+        const uint32_t ranges = kv_ranges(s, p.each, p.slack);
+        const uint32_t own = s.tiles * ranges, incl = kv_wave_scan(own);
+        const unsigned long long hit = __ballot(pick(b, s, ranges, before + incl - own));
         if (hit) {
             const int l = __ffsll((unsigned long long)hit) - 1;
             cut.b = b0 + l;
             cut.n_before = before + __builtin_amdgcn_readlane(incl - own, l);
             cut.tiles = __builtin_amdgcn_readlane(s.tiles, l);
-            cut.ranges = __builtin_amdgcn_readlane(s.ranges, l);
+            cut.ranges = __builtin_amdgcn_readlane(ranges, l);
             const uint32_t steps = __builtin_amdgcn_readlane(s.steps, l);
-            cut.steps_each = ((steps + cut.ranges - 1u) / cut.ranges + kWaves - 1u) / kWaves * kWaves;
+            cut.steps_each = (kv_div_up(steps, cut.ranges) + kWaves - 1u) / kWaves * kWaves;
             return true;
         }
         before += __builtin_amdgcn_readlane(incl, 63);
     }
     return false;
 }
+// What the joining kernel reads of a sequence: units before it, tiles, ranges; behind the last
+// sequence: whether any has more than one range.
 __device__ __forceinline__ bool kv_find(const hf_kv_attend_args& a, const uint32_t tile_rows, kv_cut& cut) {
     const kv_plan_dev p = kv_plan_now(a, tile_rows);
+    if (blockIdx.x == 0 && threadIdx.x < 64 && a.join) {
+        bool split = false;
+        kv_walk(a, tile_rows, p, [&](const uint32_t b, const kv_shape& s, const uint32_t ranges, const uint32_t first) {
+            if (b < a.s.batch) *(hf_u32x4*)(a.plan + 4 * (int64_t)b) = hf_u32x4{first, s.tiles, ranges, 0};
+            split = split || (s.tiles && ranges > 1);
+            return false;
+        }, cut);
+        split = __ballot(split) != 0;
+        if (threadIdx.x == 0) a.plan[4 * (int64_t)a.s.batch] = split;
+    }
     const uint32_t eighth = (p.total + 7u) / 8u;
     cut.unit = blockIdx.x % 8u * eighth + blockIdx.x / 8u;
     if (blockIdx.x / 8u >= eighth) return false;
     const uint32_t unit = cut.unit;
-    return kv_walk(a, tile_rows, p, [&](uint32_t, uint32_t first, uint32_t own) { return unit < first + own; }, cut);
+    return kv_walk(a, tile_rows, p, [&](uint32_t, const kv_shape& s, const uint32_t ranges, const uint32_t first) {
+        return unit < first + s.tiles * ranges;
+    }, cut);
 }
 
 // ---- one unit ------------------------------------------------------------------------------------
@@ -791,65 +830,72 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
     }
 }
 
-// Joins the ranges of a row: a wavefront per row, DP / 4 lanes along the row and the ranges dealt to
-// the groups of lanes that are left.
+// Joins the ranges of rows that have several: a wavefront takes a row of a head at a time, DP / 4
+// lanes along it and the ranges dealt to the groups of lanes that are left.
 template <int QT, int DP>
 __global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a, const uint32_t tile_rows) {
     typedef kv_type<QT> T;
     constexpr uint32_t cols = DP / 4, deal = 64 / cols;
-    const uint32_t q_heads = a.c.heads * a.per;
-    const uint32_t id = blockIdx.x * 4u + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int32_t row = (int32_t)(id / q_heads);
-    const uint32_t out_head = id % q_heads;
-    if ((uint32_t)row >= a.s.rows) return;
-    const kv_plan_dev p = kv_plan_now(a, tile_rows);
-    kv_cut cut;
-    const bool found = kv_walk(a, tile_rows, p, [&](uint32_t b, uint32_t, uint32_t) {
-        if (b >= a.s.batch) return false;
-        const hf_kv_seq s = hf_kv_sequence(a.s, b, a.c.page_shift);
-        return row >= s.row0 && row < s.row0 + s.n;
-    }, cut);
-    const uint32_t tiles = cut.tiles, ranges = cut.ranges, before = cut.n_before;
-    if (!found || ranges < 2) return;
-    const hf_kv_seq q = hf_kv_sequence(a.s, cut.b, a.c.page_shift);
-    const uint32_t i = (uint32_t)(row - q.row0) * a.per + out_head % a.per;
-    const uint32_t tile = out_head / a.per * (tiles / a.c.heads) + i / tile_rows;
-    // (offsets that cover a row twice, which the attending kernel reports, can count more units
-    // than there are)
-    if ((uint64_t)before + (uint64_t)tiles * ranges > a.units) return;
-    const int64_t first = (int64_t)(before + tile) * tile_rows + i % tile_rows;
-    const int64_t jump = (int64_t)tiles * tile_rows;
-    const uint32_t col = (uint32_t)hf_lane() % cols, part = (uint32_t)hf_lane() / cols;
-    float least = 3.402823466e38f;
-    for (uint32_t s = hf_lane(); s < ranges; s += 64) least = fminf(least, a.part_ml[4 * (first + s * jump)]);
+    if (a.plan[4 * (int64_t)a.s.batch] == 0) return;
+    const uint32_t q_heads = a.c.heads * a.per, all = a.s.rows * q_heads;
+    const uint32_t first_id = blockIdx.x * 4u + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    for (uint32_t id = first_id; id < all; id += gridDim.x * 4u) {
+        const int32_t row = (int32_t)(id / q_heads);
+        const uint32_t out_head = id % q_heads;
+        uint32_t b = a.s.cu ? a.s.batch : (uint32_t)row;
+        if (a.s.cu) {
+            for (uint32_t b0 = 0; b0 < a.s.batch && b == a.s.batch; b0 += 64) {
+                const uint32_t mine = b0 + hf_lane();
+                bool hit = false;
+                if (mine < a.s.batch) hit = row >= a.s.cu[mine] && row < a.s.cu[mine + 1];
+                const unsigned long long hits = __ballot(hit);
+                if (hits) b = b0 + __ffsll(hits) - 1;
+            }
+            if (b == a.s.batch) continue;
+        }
+        const hf_u32x4 plan = *(const hf_u32x4*)(a.plan + 4 * (int64_t)b);
+        const uint32_t before = plan[0], tiles = plan[1], ranges = plan[2];
+        if (tiles == 0 || ranges < 2) continue;
+        const hf_kv_seq q = hf_kv_sequence(a.s, b, a.c.page_shift);
+        const uint32_t i = (uint32_t)(row - q.row0) * a.per + out_head % a.per;
+        const uint32_t tile = out_head / a.per * (tiles / a.c.heads) + i / tile_rows;
+        // (offsets that cover a row twice, which the attending kernel reports, can count more units
+        // than there are)
+        if ((uint64_t)before + (uint64_t)tiles * ranges > a.units) continue;
+        const int64_t first = (int64_t)(before + tile) * tile_rows + i % tile_rows;
+        const int64_t jump = (int64_t)tiles * tile_rows;
+        const uint32_t col = (uint32_t)hf_lane() % cols, part = (uint32_t)hf_lane() / cols;
+        float least = 3.402823466e38f;
+        for (uint32_t s = hf_lane(); s < ranges; s += 64) least = fminf(least, a.part_ml[4 * (first + s * jump)]);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) least = fminf(least, __shfl_xor(least, o));
-    f32x4 acc = {0, 0, 0, 0};
-    float sum = 0.0f, div = 0.0f;
+        for (int o = 32; o > 0; o >>= 1) least = fminf(least, __shfl_xor(least, o));
+        f32x4 acc = {0, 0, 0, 0};
+        float sum = 0.0f, div = 0.0f;
 #pragma unroll 4
-    for (uint32_t s = part; s < ranges; s += deal) {
-        const int64_t at = first + s * jump;
-        const f32x4 ml = *(const f32x4*)(a.part_ml + 4 * at);
-        const float w = __builtin_amdgcn_exp2f(least - ml[0]);
-        sum += w * ml[1];
-        div += w * ml[2];
-        acc += w * *(const f32x4*)(a.part + at * DP + 4 * col);
-    }
+        for (uint32_t s = part; s < ranges; s += deal) {
+            const int64_t at = first + s * jump;
+            const f32x4 ml = *(const f32x4*)(a.part_ml + 4 * at);
+            const float w = __builtin_amdgcn_exp2f(least - ml[0]);
+            sum += w * ml[1];
+            div += w * ml[2];
+            acc += w * *(const f32x4*)(a.part + at * DP + 4 * col);
+        }
 #pragma unroll
-    for (int o = cols; o < 64; o <<= 1) {
-        sum += __shfl_xor(sum, o);
-        div += __shfl_xor(div, o);
+        for (int o = cols; o < 64; o <<= 1) {
+            sum += __shfl_xor(sum, o);
+            div += __shfl_xor(div, o);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
+            for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
+        }
+        const float f = div == 0.0f ? 0.0f : 1.0f / div;
+        if (part == 0 && 4 * col < a.c.head_dim) {
+            hf_g8* dst = (hf_g8*)a.out.p + ((int64_t)row * a.out.row_stride + (int64_t)out_head * a.out.head_stride) * 2;
+            *(hf_gmem_u32x2*)(dst + 8 * col) =
+                hf_u32x2{T::pack(acc[0] * f, acc[1] * f), T::pack(acc[2] * f, acc[3] * f)};
+        }
+        if (a.lse && hf_lane() == 0)
+            a.lse[(int64_t)row * q_heads + out_head] = kv_lse(least, sum);
     }
-    const float f = div == 0.0f ? 0.0f : 1.0f / div;
-    if (part == 0 && 4 * col < a.c.head_dim) {
-        hf_g8* dst = (hf_g8*)a.out.p + ((int64_t)row * a.out.row_stride + (int64_t)out_head * a.out.head_stride) * 2;
-        *(hf_gmem_u32x2*)(dst + 8 * col) =
-            hf_u32x2{T::pack(acc[0] * f, acc[1] * f), T::pack(acc[2] * f, acc[3] * f)};
-    }
-    if (a.lse && hf_lane() == 0)
-        a.lse[(int64_t)row * q_heads + out_head] = kv_lse(least, sum);
 }
 
 }  // namespace

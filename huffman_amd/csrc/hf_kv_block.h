@@ -463,8 +463,8 @@ void hf_k_kv_attend_block(const hf_kv_attend_args a) {
 template <int QT, int DP>
 void kv_join(const hf_kv_attend_args& a, const uint32_t tile_rows, hipStream_t st) {
     if (!a.join) return;
-    const uint64_t rows = (uint64_t)a.s.rows * a.c.heads * a.per;
-    hipLaunchKernelGGL((hf_k_kv_join<QT, DP>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, st, a, tile_rows);
+    const uint64_t blocks = ((uint64_t)a.s.rows * a.c.heads * a.per + 3) / 4;
+    hipLaunchKernelGGL((hf_k_kv_join<QT, DP>), dim3((uint32_t)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, a, tile_rows);
 }
 template <int QT, int FMT, int DP>
 void kv_launch_rows(const hf_kv_attend_args& a, const int tile_rows, hipStream_t st) {
