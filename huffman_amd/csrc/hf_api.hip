@@ -1542,16 +1542,16 @@ int kv_check_cache(const hf_kv_cache* c, hf_kv_pools* p) {
     }
     if (!aligned16(c->d_k) || !aligned16(c->d_v)) return HF_ERR_ALIGN;
     if ((c->page_stride | c->token_stride | c->head_stride) & 15) return HF_ERR_ALIGN;
-    // (an offset inside a pool is computed in 63 bits)
+    // (the kernels hold strides in 32 bits and compute places in 64)
     if (c->page_stride > (1ll << 31) || c->token_stride > (1ll << 31) || c->head_stride > (1ll << 31))
         return HF_ERR_RANGE;
     p->k = (uint8_t*)c->d_k;
     p->v = (uint8_t*)c->d_v;
     p->k_scale = bits < 16 ? c->d_k_scale : nullptr;
     p->v_scale = bits < 16 ? c->d_v_scale : nullptr;
-    p->page_stride = c->page_stride;
-    p->token_stride = c->token_stride;
-    p->head_stride = c->head_stride;
+    p->page_stride = (uint32_t)c->page_stride;
+    p->token_stride = (uint32_t)c->token_stride;
+    p->head_stride = (uint32_t)c->head_stride;
     p->n_pages = (uint32_t)c->n_pages;
     p->page_shift = (uint32_t)log2ceil_i((int)c->page_size);
     p->heads = c->heads;
@@ -1567,10 +1567,11 @@ int kv_check_batch(const hf_kv_batch* b, hf_kv_seqs* s) {
     if (b->batch && (!b->d_kv_len || !b->d_table || b->table_width < 1 || b->table_stride < b->table_width))
         return HF_ERR_ARG;
     if (!b->d_cu_rows && b->rows != b->batch) return HF_ERR_ARG;
+    if (b->table_stride > (1ll << 31)) return HF_ERR_RANGE;
     s->cu = b->d_cu_rows;
     s->kv_len = b->d_kv_len;
     s->table = b->d_table;
-    s->table_stride = b->table_stride;
+    s->table_stride = (uint32_t)b->table_stride;
     s->width = b->table_width;
     s->batch = b->batch;
     s->rows = b->rows;
@@ -1585,8 +1586,8 @@ int kv_check_rows(const void* p, int64_t row_stride, int64_t head_stride, int el
     if (row_stride < 0 || head_stride < 0) return HF_ERR_ARG;
     if (row_stride > (1ll << 31) || head_stride > (1ll << 31)) return HF_ERR_RANGE;
     r->p = const_cast<void*>(p);
-    r->row_stride = row_stride;
-    r->head_stride = head_stride;
+    r->row_stride = (uint32_t)row_stride;
+    r->head_stride = (uint32_t)head_stride;
     return HF_OK;
 }
 
@@ -1634,8 +1635,8 @@ struct kv_plan {
 int kv_plan_of(const hf_ctx* ctx, const hf_kv_pools& p, const hf_kv_seqs& s, uint32_t per, kv_plan* o) {
     o->tile_rows = hf_kv_attend_tile_rows(s.most, per, p.head_dim);
     // units aimed at: of small tiles six per compute unit, which evens out a ragged batch of single
-    // tokens (64 sequences of up to 8000: 198 us with two, 163 with six); of larger ones what runs at
-    // once, two workgroups of 32 .. 128 rows to a compute unit or one of 256
+    // tokens (64 sequences of up to 8000: 169 us with two, 155 with six, 165 with twelve); of larger ones
+    // what runs at once, two workgroups of 64 or 128 rows to a compute unit or one of 256
     o->target = (uint32_t)ctx->num_cu * (o->tile_rows == 16 ? 6u : o->tile_rows == 256 || p.head_dim > 128 ? 1u : 2u);
     o->min_steps = 4;
     const uint64_t rows = (uint64_t)s.rows * per;

@@ -9,9 +9,9 @@ struct hf_kv_pools {
     uint8_t* v;
     uint8_t* k_scale;  // [n_pages][heads][groups][page_size], NULL for the 16-bit formats
     uint8_t* v_scale;
-    int64_t page_stride;
-    int64_t token_stride;
-    int64_t head_stride;
+    uint32_t page_stride;  // (strides stay below 2^32 and in 32 bits: scalar registers are short)
+    uint32_t token_stride;
+    uint32_t head_stride;
     uint32_t n_pages;
     uint32_t page_shift;  // page_size = 1 << page_shift, at least 8 tokens
     uint32_t heads;
@@ -26,7 +26,7 @@ struct hf_kv_seqs {
     const int32_t* cu;
     const int32_t* kv_len;
     const int32_t* table;
-    int64_t table_stride;
+    uint32_t table_stride;
     uint32_t width;  // pages in a row of the table
     uint32_t batch;
     uint32_t rows;   // rows of the row tensors
@@ -36,8 +36,8 @@ struct hf_kv_seqs {
 // Row tensors [rows][heads][head_dim], strides in elements, head_dim contiguous.
 struct hf_kv_rows {
     void* p;
-    int64_t row_stride;
-    int64_t head_stride;
+    uint32_t row_stride;
+    uint32_t head_stride;
 };
 
 struct hf_kv_attend_args {

@@ -35,6 +35,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+typedef __attribute__((address_space(4))) int32_t kv_const_i32;
 constexpr int kWaves = 4;
 constexpr int kStep = 32;  // tokens a wavefront takes at a time
 
@@ -295,8 +296,8 @@ struct kv_unit {
         hf_u32x2 ks[bits == 16 ? 1 : KP];  // scale bytes of the lane's eight tokens, by piece
         hf_u32x2 vs;
     };
-    struct pages {  // pages of the lane's tokens as a row of K and as eight columns of V
-        int32_t k, v;
+    struct pages {  // of four groups of eight tokens
+        int32_t id[4];
     };
 
     const hf_kv_attend_args& a;
@@ -309,10 +310,36 @@ struct kv_unit {
     f32x4 div[R];         // sums of the rounded p (all four alike)
     float nm[R], sum[R];  // p = exp2(scale_log2 s + nm); the lane's share of the sum of p
     hf_u32x4 qr[R][KS];
-    uint32_t bad;
+    uint32_t bad, odd;  // a page out of range; values that were left out
+    // the lane's own part of its places in the pools and in the scales
+    const hf_g8 *kbase, *vbase, *ksbase, *vsbase;
+    bool cuts;  // head_dim ends inside the padded one
 
     __device__ __forceinline__ kv_unit(const hf_kv_attend_args& args)
-        : a(args), lane(hf_lane()), m(lane & 15), g(lane >> 4), bad(0) {}
+        : a(args), lane(hf_lane()), m(lane & 15), g(lane >> 4), bad(0), odd(0) {}
+
+    // Lanes whose d are behind head_dim load the row's first ones instead: of K the values are
+    // cleared, of V they make outputs that nobody takes.
+    __device__ __forceinline__ void bases() {
+        cuts = a.c.head_dim < (uint32_t)DP;
+        const int dk = DPC * g < (int)a.c.head_dim ? DPC * g : 0, dv = VD * m < (int)a.c.head_dim ? VD * m : 0;
+        const int64_t h = (int64_t)head * a.c.head_stride;
+        kbase = (const hf_g8*)a.c.k + h + (int64_t)(m & 3) * a.c.token_stride + dk * bits / 8;
+        vbase = (const hf_g8*)a.c.v + h + dv * bits / 8;
+        const int64_t hs = (int64_t)head * a.c.groups << a.c.page_shift;
+        ksbase = (const hf_g8*)a.c.k_scale + hs + ((int64_t)(dk >> a.c.group_shift) << a.c.page_shift);
+        vsbase = (const hf_g8*)a.c.v_scale + hs + ((int64_t)(dv >> a.c.group_shift) << a.c.page_shift);
+    }
+    __device__ __forceinline__ int64_t place(const uint32_t at, int32_t page_id, int64_t& scale) {
+        uint32_t pg = (uint32_t)page_id;
+        if (pg >= a.c.n_pages) {
+            bad = 1;
+            pg = 0;
+        }
+        const uint32_t off = group_at(at) & ((1u << a.c.page_shift) - 1u);
+        scale = (int64_t)((uint64_t)pg * (a.c.heads * a.c.groups << a.c.page_shift) + off);
+        return (int64_t)((uint64_t)pg * (uint32_t)a.c.page_stride + (uint64_t)off * (uint32_t)a.c.token_stride);
+    }
 
     // d of the lane's elements of product ks: first of eight
     __device__ __forceinline__ int d_of(const int ks) const {
@@ -353,56 +380,49 @@ struct kv_unit {
         int32_t p = table[group_at(t) >> a.c.page_shift];
         return p;
     }
-    __device__ __forceinline__ pages find(const uint32_t t) {
-        pages p;
-        p.k = page_at(t + 8u * (m >> 2));
-        p.v = page_at(t + 8u * g);
-        return p;
+    // The pages of 32 tokens, four groups of eight: through the scalar cache, so that the wait for
+    // them is not one for the vector loads in front of them.
+    __device__ __forceinline__ void find(const uint32_t t, pages& p) const {
+        const kv_const_i32* tab = (const kv_const_i32*)(const int32_t*)table;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p.id[i] = tab[__builtin_amdgcn_readfirstlane(group_at(t + 8u * i) >> a.c.page_shift)];
     }
-    __device__ __forceinline__ void load(const uint32_t t, pages p, tile& x) {
-        if ((uint32_t)p.k >= a.c.n_pages) { bad = 1; p.k = 0; }
-        if ((uint32_t)p.v >= a.c.n_pages) { bad = 1; p.v = 0; }
-        const uint32_t in_page = (1u << a.c.page_shift) - 1u;
-        const uint32_t ok = group_at(t + 8u * (m >> 2)) & in_page;
-        const uint32_t ov = group_at(t + 8u * g) & in_page;
-        const int64_t hk = (int64_t)head * a.c.head_stride;
-        const hf_g8* pk = (const hf_g8*)a.c.k + (int64_t)p.k * a.c.page_stride +
-                          (int64_t)(ok + (m & 3)) * a.c.token_stride + hk;
-        const hf_g8* pv = (const hf_g8*)a.c.v + (int64_t)p.v * a.c.page_stride +
-                          (int64_t)ov * a.c.token_stride + hk;
+    static __device__ __forceinline__ int32_t of_group(const pages& p, const int i) {
+        const int32_t lo = i & 1 ? p.id[1] : p.id[0], hi = i & 1 ? p.id[3] : p.id[2];
+        return i & 2 ? hi : lo;
+    }
+    __device__ __forceinline__ void load_k(const uint32_t t, const pages p, tile& x) {
+        int64_t sc;
+        const hf_g8* pk = kbase + place(t + 8u * (m >> 2), of_group(p, m >> 2), sc);
+        const int dk = DPC * g < (int)a.c.head_dim ? DPC * g : 0;
+        // (where nothing is cut, a constant offset)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
 #pragma unroll
             for (int h = 0; h < KP; ++h) {
-                const int d = 4 * DPC * h + DPC * g;
-                if (d < (int)a.c.head_dim) x.k[b][h].load(pk + d * bits / 8);
-                else x.k[b][h].clear();
+                const int d = cuts && 4 * DPC * h + DPC * g >= (int)a.c.head_dim ? 0 : 4 * DPC * h;
+                x.k[b][h].load(pk + d * bits / 8);
             }
             pk += 4 * a.c.token_stride;
         }
-        const bool on = VD * m < (int)a.c.head_dim;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (on) x.v[j].load(pv + VB * m);
-            else x.v[j].clear();
-            pv += a.c.token_stride;
-        }
         if constexpr (bits != 16) {
-            const int64_t sk = (((int64_t)p.k * a.c.heads + head) * a.c.groups << a.c.page_shift) + ok;
-            const int64_t sv = (((int64_t)p.v * a.c.heads + head) * a.c.groups << a.c.page_shift) + ov;
 #pragma unroll
             for (int h = 0; h < KP; ++h) {
-                const int d = 4 * DPC * h + DPC * g;
-                x.ks[h] = hf_u32x2{0, 0};
-                if (d < (int)a.c.head_dim)
-                    x.ks[h] = *(const hf_gmem_u32x2*)((const hf_g8*)a.c.k_scale + sk +
-                                                      ((int64_t)(d >> a.c.group_shift) << a.c.page_shift));
+                const int d = cuts && 4 * DPC * h + DPC * g >= (int)a.c.head_dim ? 0 : 4 * DPC * h;
+                x.ks[h] = *(const hf_gmem_u32x2*)(
+                    ksbase + sc + ((((dk + d) >> a.c.group_shift) - (dk >> a.c.group_shift)) << a.c.page_shift));
             }
-            x.vs = hf_u32x2{0, 0};
-            if (on)
-                x.vs = *(const hf_gmem_u32x2*)((const hf_g8*)a.c.v_scale + sv +
-                                               ((int64_t)((VD * m) >> a.c.group_shift) << a.c.page_shift));
         }
+    }
+    __device__ __forceinline__ void load_v(const uint32_t t, const pages p, tile& x) {
+        int64_t sc;
+        const hf_g8* pv = vbase + place(t + 8u * g, of_group(p, g), sc);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x.v[j].load(pv);
+            pv += a.c.token_stride;
+        }
+        if constexpr (bits != 16) x.vs = *(const hf_gmem_u32x2*)(vsbase + sc);
     }
 
     // Which of the lane's eight tokens t + 8 g + 0..7 row i (of the sequence's n rows) may see.
@@ -522,49 +542,58 @@ struct kv_unit {
     }
 
     // A step: 32 tokens from t.  FULL: every row sees all of them.
-    template <bool FULL>
+    // next_k, next_v: called where the tile's K and V are in use no more, to load the next ones there.
+    template <bool FULL, typename NK, typename NV>
     __device__ __forceinline__ void step(const uint32_t t, const tile& x, const int32_t row_lo,
-                                         const int32_t rows) {
-        f32x4 s[R][2];
-        {
+                                         const int32_t rows, NK&& next_k, NV&& next_v) {
+        hf_u32x4 ka[2][KS];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                hf_u32x4 ka[KS];
+        for (int b = 0; b < 2; ++b) {
 #pragma unroll
-                for (int h = 0; h < KP; ++h) {
-                    float f = 0.0f;
-                    if constexpr (bits != 16) {
-                        const uint32_t w = b ? x.ks[h].y : x.ks[h].x;
-                        f = __uint_as_float(__builtin_amdgcn_ubfe(w, 8u * (m & 3), 8u) << 23);
-                    }
-                    if constexpr (bits == 16) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) ka[h][i] = x.k[b][h].w[i];
-                    } else if constexpr (bits == 8) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            ka[2 * h + i / 2][2 * (i % 2)] = kv_pair<QT, FMT, 0>(x.k[b][h].w[i], f);
-                            ka[2 * h + i / 2][2 * (i % 2) + 1] = kv_pair<QT, FMT, 1>(x.k[b][h].w[i], f);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < KB / 4; ++i) {
-                            constexpr int per = DPC / 8;
-                            ka[per * h + i][0] = kv_pair<QT, FMT, 0>(x.k[b][h].w[i], f);
-                            ka[per * h + i][1] = kv_pair<QT, FMT, 1>(x.k[b][h].w[i], f);
-                            ka[per * h + i][2] = kv_pair<QT, FMT, 2>(x.k[b][h].w[i], f);
-                            ka[per * h + i][3] = kv_pair<QT, FMT, 3>(x.k[b][h].w[i], f);
-                        }
-                    }
+            for (int h = 0; h < KP; ++h) {
+                float f = 0.0f;
+                if constexpr (bits != 16) {
+                    const uint32_t w = b ? x.ks[h].y : x.ks[h].x;
+                    f = __uint_as_float(__builtin_amdgcn_ubfe(w, 8u * (m & 3), 8u) << 23);
                 }
+                if constexpr (bits == 16) {
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    s[r][b] = f32x4{0, 0, 0, 0};
+                    for (int i = 0; i < 4; ++i) ka[b][h][i] = x.k[b][h].w[i];
+                } else if constexpr (bits == 8) {
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) s[r][b] = T::mma(ka[ks], qr[r][ks], s[r][b]);
+                    for (int i = 0; i < 4; ++i) {
+                        ka[b][2 * h + i / 2][2 * (i % 2)] = kv_pair<QT, FMT, 0>(x.k[b][h].w[i], f);
+                        ka[b][2 * h + i / 2][2 * (i % 2) + 1] = kv_pair<QT, FMT, 1>(x.k[b][h].w[i], f);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < KB / 4; ++i) {
+                        constexpr int per = DPC / 8;
+                        ka[b][per * h + i][0] = kv_pair<QT, FMT, 0>(x.k[b][h].w[i], f);
+                        ka[b][per * h + i][1] = kv_pair<QT, FMT, 1>(x.k[b][h].w[i], f);
+                        ka[b][per * h + i][2] = kv_pair<QT, FMT, 2>(x.k[b][h].w[i], f);
+                        ka[b][per * h + i][3] = kv_pair<QT, FMT, 3>(x.k[b][h].w[i], f);
+                    }
                 }
             }
         }
+        if (cuts) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+                    if (d_of(ks) >= (int)a.c.head_dim) ka[b][ks] = hf_u32x4{0, 0, 0, 0};
+        }
+        next_k();
+        f32x4 s[R][2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                s[r][b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) s[r][b] = T::mma(ka[b][ks], qr[r][ks], s[r][b]);
+            }
         uint32_t see[R];
         float top[R];
         bool up = false;
@@ -631,14 +660,18 @@ struct kv_unit {
             there = (1u << left) - 1u;
         }
         columns(x, there, av);
+        next_v();
         if constexpr (!FULL) {
-            // A token that some rows may not see must not reach them as 0 x infinity or NaN.
-            uint32_t odd = 0;
+            // A token that some rows may not see must not reach them as 0 x infinity or NaN: what is
+            // not finite is left out here and added at the end (left_out).
 #pragma unroll
             for (int c = 0; c < VD; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) odd |= ((av[c][i] & T::expo) + T::unit) & 0x80008000u;
-            if (__ballot(odd != 0)) not_finite(av, see);
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t hit = ((av[c][i] & T::expo) + T::unit) & 0x80008000u;
+                    odd |= hit;
+                    av[c][i] &= ~((hit >> 15) * 0xFFFFu);
+                }
         }
 #pragma unroll
         for (int c = 0; c < VD; ++c)
@@ -646,45 +679,33 @@ struct kv_unit {
             for (int r = 0; r < R; ++r) acc[r][c] = T::mma(av[c], p[r], acc[r][c]);
     }
 
-    // Takes infinities and NaN out of the tokens' values and adds them to the outputs of the rows
-    // that see their token: how many a row sees of each kind is a product of ones.
-    __device__ __forceinline__ void not_finite(hf_u32x4 (&av)[VD], const uint32_t (&see)[R]) {
+    // The values of tokens t .. t + 31 that are not finite, to the rows that see them.
+    __device__ __forceinline__ void left_out(const uint32_t t, const int32_t row_lo, const int32_t rows) {
 #pragma unroll 1
-        for (int kind = 0; kind < 3; ++kind) {
-            const float add = kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
+        for (uint32_t at = t; at < t + kStep && at < (uint32_t)q.len; ++at) {
+            const int32_t pg = page_at(at);
+            if ((uint32_t)pg >= a.c.n_pages) continue;
+            const uint32_t off = at & ((1u << a.c.page_shift) - 1u);
+            const hf_g8* p = (const hf_g8*)a.c.v + (int64_t)pg * a.c.page_stride + (int64_t)off * a.c.token_stride +
+                             (int64_t)head * a.c.head_stride;
 #pragma unroll
-            for (int c = 0; c < VD; ++c) {
-                hf_u32x4 is;
+            for (int r = 0; r < R; ++r) {
+                const int32_t i = row_lo + 16 * r + m;
+                const bool on = i < rows;
+                const bool sees = on && (at < (uint32_t)q.past || (seen_at((on ? i : 0) / (int32_t)a.per, at, on) & 1u));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    is[i] = 0;
+                for (int e = 0; e < 4; ++e) {
+                    const int d = VD * (4 * g + e);
+                    if (sees && d < (int)a.c.head_dim) {
+                        float v[VD];
+                        values(p + d * bits / 8, pg, off, d, v);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t x = av[c][i] >> (16 * h) & 0xFFFFu, mag = x & 0x7FFFu;
-                        const bool hit = kind == 0 ? mag > T::inf : x == (kind == 1 ? T::inf : T::inf | 0x8000u);
-                        if (hit) is[i] |= T::one << (16 * h);
+                        for (int c = 0; c < VD; ++c)
+                            if (!(fabsf(v[c]) <= 3.402823466e38f)) acc[r][c][e] += v[c];
                     }
-                }
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    hf_u32x4 ones;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        ones[i] = (see[r] >> (2 * i) & 1u ? T::one : 0u) | (see[r] >> (2 * i + 1) & 1u ? T::one << 16 : 0u);
-                    const f32x4 count = T::mma(is, ones, f32x4{0, 0, 0, 0});
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (count[i] > 0.0f) acc[r][c][i] += add;
                 }
             }
         }
-#pragma unroll
-        for (int c = 0; c < VD; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if ((av[c][i] & 0x7FFFu) >= T::inf) av[c][i] &= 0xFFFF0000u;
-                if ((av[c][i] >> 16 & 0x7FFFu) >= T::inf) av[c][i] &= 0xFFFFu;
-            }
     }
 };
 
@@ -728,31 +749,37 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
     end = min(end, t_lo + cut.steps_each * kStep);
 
     u.load_q(row_lo, rows);
-#pragma unroll
-    for (int r = 0; r < R; ++r) kv_arrived(u.qr[r]);
+    u.bases();
     uint32_t t = t_lo + kStep * (uint32_t)wave;
     if (t < end) {
         constexpr uint32_t stride = kStep * kWaves;
-        typename U::tile x0, x1;
-        typename U::pages p = u.find(t);
-        u.load(t, p, x0);
-        p = u.find(t + stride);
-        auto one = [&](typename U::tile& now, typename U::tile& next) {
-            // the next tokens' bytes and the pages of those after them are under way meanwhile
-            if (t + stride < end) {
-                u.load(t + stride, p, next);
-                p = u.find(t + 2 * stride);
-            }
-            if (t + kStep <= whole && t + kStep <= end) u.template step<true>(t, now, row_lo, rows);
-            else u.template step<false>(t, now, row_lo, rows);
-            t += stride;
+        typename U::tile x;
+        typename U::pages p;
+        u.find(t, p);
+        u.load_k(t, p, x);
+        u.load_v(t, p, x);
+        u.find(t + stride, p);
+#pragma unroll
+        for (int r = 0; r < R; ++r) kv_arrived(u.qr[r]);
+        auto one = [&](auto&& next_k, auto&& next_v) {
+            if (t + kStep <= whole && t + kStep <= end) u.template step<true>(t, x, row_lo, rows, next_k, next_v);
+            else u.template step<false>(t, x, row_lo, rows, next_k, next_v);
         };
-        while (true) {
-            one(x0, x1);
-            if (t >= end) break;
-            one(x1, x0);
-            if (t >= end) break;
-        }
+        // The next tokens' bytes, and the pages of those behind them, are under way as soon as the
+        // registers of the present ones are free.  (The last turn stands apart: loads under a
+        // condition would make every wait one for all of them.)
+#pragma unroll 1
+        for (; t + stride < end; t += stride)
+            one([&]() { u.load_k(t + stride, p, x); },
+                [&]() {
+                    u.load_v(t + stride, p, x);
+                    u.find(t + 2 * stride, p);
+                });
+        one([]() {}, []() {});
+    }
+    if (__ballot(u.odd != 0)) {
+        for (t = t_lo + kStep * (uint32_t)wave; t < end; t += kStep * kWaves)
+            if (t + kStep > whole || t + kStep > end) u.left_out(t, row_lo, rows);
     }
     if (u.bad) atomicOr(a.err, HF_KERR_CORRUPT);
 

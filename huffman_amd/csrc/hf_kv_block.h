@@ -468,16 +468,16 @@ void kv_join(const hf_kv_attend_args& a, const uint32_t tile_rows, hipStream_t s
 }
 template <int QT, int FMT, int DP>
 void kv_launch_rows(const hf_kv_attend_args& a, const int tile_rows, hipStream_t st) {
-    if (tile_rows == 16)
-        hipLaunchKernelGGL((hf_k_kv_attend<QT, FMT, DP, 1>), dim3(a.units), dim3(64 * kWaves), 0, st, a);
-    else if (tile_rows == 32)
-        hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 1, 2, 64, DP == 256 ? 1 : 2>), dim3(a.units), dim3(128), 0, st, a);
-    else if (tile_rows == 64)
-        hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 2, 2, 64, DP == 256 ? 1 : 2>), dim3(a.units), dim3(256), 0, st, a);
-    else if (tile_rows == 128)
+    if constexpr (DP <= 128) {
+        if (tile_rows == 16)
+            hipLaunchKernelGGL((hf_k_kv_attend<QT, FMT, DP, 1>), dim3(a.units), dim3(64 * kWaves), 0, st, a);
+        else if (tile_rows == 64)
+            hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 2, 2, 64, 2>), dim3(a.units), dim3(256), 0, st, a);
+        else if (tile_rows == 256)
+            hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 8, 1, 128, 2>), dim3(a.units), dim3(512), 0, st, a);
+    }
+    if (tile_rows == 128)
         hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 4, 1, 64, 2>), dim3(a.units), dim3(256), 0, st, a);
-    else if constexpr (DP <= 128)
-        hipLaunchKernelGGL((hf_k_kv_attend_block<QT, FMT, DP, 8, 1, 128, 2>), dim3(a.units), dim3(512), 0, st, a);
     kv_join<QT, DP>(a, (uint32_t)tile_rows, st);
 }
 template <int QT, int FMT>

@@ -294,9 +294,9 @@ __global__ __launch_bounds__(kThreads) void hf_k_kv_write(const hf_kv_pools c, c
         const int64_t at = place.code[tok];
         const uint32_t head = (piece * d.inv) >> 21, col = (piece - head * d.per_head) * 8u;
         const int64_t row = t0 + tok;
-        const hf_g8* pk = (const hf_g8*)k.p + (row * k.row_stride + head * k.head_stride + col) * es;
-        const hf_g8* pv = (const hf_g8*)v.p + (row * v.row_stride + head * v.head_stride + col) * es;
-        const int64_t code = at + head * c.head_stride + (int64_t)(col * kv_fmt<FMT>::bits / 8);
+        const hf_g8* pk = (const hf_g8*)k.p + (row * k.row_stride + (int64_t)head * k.head_stride + col) * es;
+        const hf_g8* pv = (const hf_g8*)v.p + (row * v.row_stride + (int64_t)head * v.head_stride + col) * es;
+        const int64_t code = at + (int64_t)head * c.head_stride + (int64_t)(col * kv_fmt<FMT>::bits / 8);
         if constexpr (kv_fmt<FMT>::bits == 16) {
             if (at >= 0) {
                 if constexpr (DT == HF_DT_FP32) {
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(kThreads) void hf_k_kv_read(const hf_kv_pools c, co
         const uint32_t head = (piece * d.inv) >> 21, col = (piece - head * d.per_head) * 8u;
         if (at >= 0) {
             const int64_t row = t0 + tok;
-            const int64_t code = at + head * c.head_stride + (int64_t)(col * kv_fmt<FMT>::bits / 8);
+            const int64_t code = at + (int64_t)head * c.head_stride + (int64_t)(col * kv_fmt<FMT>::bits / 8);
             uint32_t sk = 0, sv = 0;
             if constexpr (kv_fmt<FMT>::bits != 16) {
                 const uint32_t g = col >> c.group_shift;
@@ -360,8 +360,8 @@ __global__ __launch_bounds__(kThreads) void hf_k_kv_read(const hf_kv_pools c, co
             float x[8], y[8];
             dequantise8<FMT>((const hf_g8*)c.k + code, sk, x);
             dequantise8<FMT>((const hf_g8*)c.v + code, sv, y);
-            store8<DT>((hf_g8*)k.p + (row * k.row_stride + head * k.head_stride + col) * es, x);
-            store8<DT>((hf_g8*)v.p + (row * v.row_stride + head * v.head_stride + col) * es, y);
+            store8<DT>((hf_g8*)k.p + (row * k.row_stride + (int64_t)head * k.head_stride + col) * es, x);
+            store8<DT>((hf_g8*)v.p + (row * v.row_stride + (int64_t)head * v.head_stride + col) * es, y);
         }
         tok += dtok;
         piece += dpiece;

@@ -9,6 +9,7 @@ decodes stored pages straight into a pool.  The reference names the operand form
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -18,6 +19,10 @@ from ._lib import check
 from .api import Context, _Module, default_context
 
 _DTYPES = {torch.bfloat16: L.HF_DT_BF16, torch.float16: L.HF_DT_FP16, torch.float32: L.HF_DT_FP32}
+# hf_kv_batch and hf_kv_query as bytes: a ctypes structure takes longer to fill than a small call runs
+_BATCH = struct.Struct("=QQQqIIII")
+_QUERY = struct.Struct("=QQQQqqqqIIIf")
+assert _BATCH.size == C.sizeof(L.hf_kv_batch) and _QUERY.size == C.sizeof(L.hf_kv_query)
 _POOL_DTYPES = {
     L.HF_KV_BF16: (torch.bfloat16,), L.HF_KV_FP16: (torch.float16,),
     L.HF_KV_FP8_E4M3: (torch.uint8, torch.float8_e4m3fn),
@@ -68,6 +73,8 @@ class KvCache(_Module):
             group = dim // k_scale.shape[2]
         self.k, self.v, self.k_scale, self.v_scale, self.fmt = k, v, k_scale, v_scale, fmt
         self.heads, self.head_dim, self.group, self.page_size = heads, dim, group, page_size
+        self._device, self._index = k.device, k.device.index
+        self._need = {}  # scratch of hf_kv_attend by the sizes it depends on
         size = k.element_size()
         self._c = L.hf_kv_cache(
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if group else 0,
@@ -100,39 +107,57 @@ class KvCache(_Module):
         return KvCache(*pools, *scales, fmt=fmt, ctx=ctx)
 
     # -- arguments -------------------------------------------------------------------------------
-    def _ints(self, name: str, t: torch.Tensor, dim: int) -> torch.Tensor:
-        if t.dtype != torch.int32 or t.dim() != dim or t.device != self.k.device or \
+    def _handle(self):
+        ctx = self.ctx
+        if ctx.device != self._index:
+            raise ValueError(f"the pools are on {self._device}, the context on cuda:{ctx.device}")
+        return ctx.handle
+
+    def _empty(self, *tensors):
+        """Tensors (shape, dtype) that belong to the context's stream, where the kernels use them."""
+        ctx = self.ctx
+        if torch.cuda.current_stream(self._index) == ctx.stream:
+            return [torch.empty(shape, dtype=dtype, device=self._device) for shape, dtype in tensors]
+        with torch.cuda.stream(ctx.stream):
+            return [torch.empty(shape, dtype=dtype, device=self._device) for shape, dtype in tensors]
+
+    def _ints(self, name: str, t: torch.Tensor, dim: int) -> torch.Size:
+        if t.dtype != torch.int32 or t.dim() != dim or t.get_device() != self._index or \
                 (t.numel() and t.stride(-1) != 1):
             raise ValueError(f"{name}: int32, {dim} dimension(s), contiguous rows, on the pools' device")
-        return t
+        return t.shape
 
-    def _batch(self, table, kv_len, cu, rows: int, max_rows: int) -> L.hf_kv_batch:
-        if self.k.device.index != self.ctx.device:
-            raise ValueError(f"the pools are on {self.k.device}, the context on cuda:{self.ctx.device}")
-        self._ints("table", table, 2)
-        self._ints("kv_len", kv_len, 1)
-        batch = table.shape[0]
-        if kv_len.shape[0] != batch:
+    def _batch(self, table, kv_len, cu, rows: int, max_rows: int) -> bytes:
+        batch, width = self._ints("table", table, 2)
+        if self._ints("kv_len", kv_len, 1)[0] != batch:
             raise ValueError("kv_len: one length for every row of the table")
+        offsets = 0
         if cu is None:
             if rows != batch:
                 raise ValueError("without cu there is one row for each sequence")
-        elif self._ints("cu", cu, 1).shape[0] != batch + 1:
-            raise ValueError("cu: batch + 1 row offsets")
-        return L.hf_kv_batch(cu.data_ptr() if cu is not None else 0, kv_len.data_ptr(), table.data_ptr(),
-                             table.stride(0) if batch > 1 else table.shape[1], table.shape[1], batch,
-                             rows, max_rows)
+        else:
+            if self._ints("cu", cu, 1)[0] != batch + 1:
+                raise ValueError("cu: batch + 1 row offsets")
+            offsets = cu.data_ptr()
+        if not 0 <= max_rows < 1 << 32:
+            raise ValueError("a sequence's largest number of rows is a 32-bit number")
+        return _BATCH.pack(offsets, kv_len.data_ptr(), table.data_ptr(), table.stride(0) if batch > 1 else width,
+                           width, batch, rows, max_rows)
 
     def _rows(self, name: str, t: torch.Tensor, heads: int) -> Tuple[int, int, int]:
         """Pointer and strides of a row tensor."""
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim or t.device != self.k.device \
-                or (t.numel() and t.stride(2) != 1):
-            raise ValueError(f"{name}: [rows, {heads}, {self.head_dim}] on the pools' device, last dimension contiguous")
+        shape = t.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or t.get_device() != self._index:
+            raise ValueError(f"{name}: [rows, {heads}, {self.head_dim}] on the pools' device")
         if t.dtype not in _DTYPES:
             raise TypeError(f"{name}: bf16, fp16 or fp32, not {t.dtype}")
+        row, head, one = t.stride()
+        if one != 1 and t.numel():
+            raise ValueError(f"{name}: the last dimension is contiguous")
         # (a stride of a dimension of one says nothing)
-        head = t.stride(1) if heads > 1 else self.head_dim
-        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else heads * head, head
+        if heads == 1:
+            head = self.head_dim
+        return t.data_ptr(), row if shape[0] > 1 else heads * head, head
 
     # -- calls -----------------------------------------------------------------------------------
     def write(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor,
@@ -144,7 +169,7 @@ class KvCache(_Module):
         pk, kr, kh = self._rows("k", k, self.heads)
         pv, vr, vh = self._rows("v", v, self.heads)
         b = self._batch(table, kv_len, cu, k.shape[0], 0)
-        check(L.lib().hf_kv_write(self.ctx.handle, C.byref(self._c), C.byref(b), pk, pv, kr, kh, vr, vh,
+        check(L.lib().hf_kv_write(self._handle(), C.addressof(self._c), b, pk, pv, kr, kh, vr, vh,
                                   _DTYPES[k.dtype]), "hf_kv_write")
 
     def read(self, table: torch.Tensor, kv_len: torch.Tensor, cu: Optional[torch.Tensor] = None,
@@ -157,16 +182,16 @@ class KvCache(_Module):
             n = table.shape[0] if cu is None and rows is None else rows
             if n is None:
                 raise ValueError("rows: how many the offsets of cu cover")
-            with torch.cuda.stream(self.ctx.stream):
-                out = tuple(torch.empty(n, self.heads, self.head_dim, dtype=dtype, device=self.k.device)
-                            for _ in range(2))
+            if dtype not in _DTYPES:
+                raise TypeError(f"bf16, fp16 or fp32, not {dtype}")
+            out = self._empty(((n, self.heads, self.head_dim), dtype), ((n, self.heads, self.head_dim), dtype))
         k, v = out
         if k.shape[0] != v.shape[0] or k.dtype != v.dtype:
             raise ValueError("out: as many rows of the same type")
         pk, kr, kh = self._rows("out[0]", k, self.heads)
         pv, vr, vh = self._rows("out[1]", v, self.heads)
         b = self._batch(table, kv_len, cu, k.shape[0], 0)
-        check(L.lib().hf_kv_read(self.ctx.handle, C.byref(self._c), C.byref(b), pk, pv, kr, kh, vr, vh,
+        check(L.lib().hf_kv_read(self._handle(), C.addressof(self._c), b, pk, pv, kr, kh, vr, vh,
                                  _DTYPES[k.dtype]), "hf_kv_read")
         return k, v
 
@@ -183,30 +208,42 @@ class KvCache(_Module):
             raise ValueError(f"q: [rows, a multiple of {self.heads}, {self.head_dim}], bf16 or fp16")
         rows, heads = q.shape[0], q.shape[1]
         pq, qr, qh = self._rows("q", q, heads)
-        b = self._batch(table, kv_len, cu, rows, max_q if cu is not None else 1)
-        ctx, words = self.ctx, 0
+        if cu is None:
+            max_q = 1
+        b = self._batch(table, kv_len, cu, rows, max_q)
+        handle, cache, words, bits = self._handle(), C.addressof(self._c), 0, 0
         if mask is not None:
-            if self._ints("mask", mask, 2).shape[0] != rows or not mask.is_contiguous():
+            shape = self._ints("mask", mask, 2)
+            words = shape[1]
+            if shape[0] != rows or not mask.is_contiguous():
                 raise ValueError("mask: contiguous int32 [rows, words]")
-            words = mask.shape[1]
-            if 32 * words < min(b.max_rows, rows):
+            if 32 * words < min(max_q, rows):
                 raise ValueError("mask: a bit for each of the max_q rows of a sequence")
-        with torch.cuda.stream(ctx.stream):
-            if out is None:
-                out = torch.empty(rows, heads, self.head_dim, dtype=q.dtype, device=q.device)
-            elif out.shape != q.shape or out.dtype != q.dtype:
-                raise ValueError("out: the shape and type of q")
-            sums = torch.empty(rows, heads, dtype=torch.float32, device=q.device) if lse else None
-            need = L.lib().hf_kv_attend_work_bytes(ctx.handle, C.byref(self._c), C.byref(b), heads)
-            # taken from torch's allocator for this call: another stream's call, or a captured
-            # graph, has its own
-            work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+            bits = mask.data_ptr()
+        # The scratch is taken from torch's allocator for this call: another stream's call, or a
+        # captured graph, has its own.
+        sizes = (table.shape, rows, max_q, cu is None, heads, self.ctx.device)
+        need = self._need.get(sizes)
+        if need is None:
+            need = self._need[sizes] = L.lib().hf_kv_attend_work_bytes(handle, cache, b, heads)
+            if len(self._need) > 1000:
+                self._need = {sizes: need}
+        wanted = [((need,), torch.uint8)]
+        if lse:
+            wanted.append(((rows, heads), torch.float32))
+        if out is None:
+            wanted.append((q.shape, q.dtype))
+        elif out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out: the shape and type of q")
+        got = self._empty(*wanted)
+        work, sums = got[0], got[1] if lse else None
+        if out is None:
+            out = got[-1]
         po, orow, oh = self._rows("out", out, heads)
-        query = L.hf_kv_query(pq, po, sums.data_ptr() if lse else 0, mask.data_ptr() if mask is not None else 0,
-                              qr, qh, orow, oh, heads, words, _DTYPES[q.dtype],
-                              self.head_dim ** -0.5 if scale is None else scale)
-        check(L.lib().hf_kv_attend(ctx.handle, C.byref(self._c), C.byref(b), C.byref(query),
-                                   work.data_ptr() if need else None, need), "hf_kv_attend")
+        query = _QUERY.pack(pq, po, sums.data_ptr() if lse else 0, bits, qr, qh, orow, oh, heads, words,
+                            _DTYPES[q.dtype], self.head_dim ** -0.5 if scale is None else scale)
+        check(L.lib().hf_kv_attend(handle, cache, b, query, work.data_ptr() if need else None, need),
+              "hf_kv_attend")
         return (out, sums) if lse else out
 
     def keep(self, table: torch.Tensor, kv_len: torch.Tensor, cu: Optional[torch.Tensor],
@@ -215,18 +252,15 @@ class KvCache(_Module):
         """``hf_kv_keep``: of the sequences' last rows (drafts), keep those that ``path`` int32
         [batch, width] names in ascending order, ``path_len`` int32 [batch] of them; returns the
         sequences' new lengths.  ``rows``: rows that ``cu`` covers (default: any number)."""
-        self._ints("path", path, 2)
-        self._ints("path_len", path_len, 1)
         batch = table.shape[0]
-        if path.shape[0] != batch or path_len.shape[0] != batch:
+        if self._ints("path", path, 2)[0] != batch or self._ints("path_len", path_len, 1)[0] != batch:
             raise ValueError("path and path_len: one row for each sequence")
         b = self._batch(table, kv_len, cu, batch if cu is None else 0x7FFFFFFF if rows is None else rows, 0)
         if new_len is None:
-            with torch.cuda.stream(self.ctx.stream):
-                new_len = torch.empty(batch, dtype=torch.int32, device=self.k.device)
-        elif self._ints("new_len", new_len, 1).shape[0] != batch:
+            new_len, = self._empty(((batch,), torch.int32))
+        elif self._ints("new_len", new_len, 1)[0] != batch:
             raise ValueError("new_len: one length for each sequence")
-        check(L.lib().hf_kv_keep(self.ctx.handle, C.byref(self._c), C.byref(b), path.data_ptr(),
+        check(L.lib().hf_kv_keep(self._handle(), C.addressof(self._c), b, path.data_ptr(),
                                  path.stride(0) if batch > 1 else path.shape[1], path.shape[1],
                                  path_len.data_ptr(), new_len.data_ptr()), "hf_kv_keep")
         return new_len
