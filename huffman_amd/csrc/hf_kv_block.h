@@ -364,15 +364,16 @@ void hf_k_kv_attend_block(const hf_kv_attend_args a) {
     int buf = 0;
     for (uint32_t t = t_lo; t < end; t += TT) {
         __syncthreads();  // tile t is in its half, and nobody reads the other any more
-        if constexpr (NBUF == 2) {
-            if (t + TT < end) stage_at(t + TT, lds.x[buf ^ 1]);
-        } else {
+        if constexpr (NBUF == 1) {
             stage_at(t, lds.x[0]);
             __syncthreads();
         }
         if (t + TT <= whole) multiply(t, lds.x[buf], std::true_type{});
         else if (t < some) multiply(t, lds.x[buf], std::false_type{});
-        buf ^= NBUF - 1;
+        if constexpr (NBUF == 2) {  // (behind the products: 2 % faster than in front of them)
+            if (t + TT < end) stage_at(t + TT, lds.x[buf ^ 1]);
+            buf ^= 1;
+        }
     }
     __syncthreads();
     if (bad) atomicOr(a.err, HF_KERR_CORRUPT);
