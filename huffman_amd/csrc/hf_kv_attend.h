@@ -166,14 +166,7 @@ __device__ __forceinline__ kv_shape kv_shape_of(const hf_kv_attend_args& a, cons
     }
     return s;
 }
-// x / y rounded up for x + y below 2^31; the float quotient is off by at most one
-__device__ __forceinline__ uint32_t kv_div_up(const uint32_t x, const uint32_t y) {
-    const uint32_t z = x + y - 1u;
-    uint32_t q = (uint32_t)((float)z * __builtin_amdgcn_rcpf((float)y));
-    if ((unsigned long long)q * y > z) --q;
-    if ((unsigned long long)(q + 1u) * y <= z) ++q;
-    return q;
-}
+__device__ __forceinline__ uint32_t kv_div_up(const uint32_t x, const uint32_t y) { return (x + y - 1u) / y; }
 __device__ __forceinline__ uint32_t kv_ranges(const kv_shape& s, const uint32_t each, const uint32_t slack) {
     return s.steps <= each + slack ? 1u : kv_div_up(s.steps - slack, each);
 }
@@ -266,7 +259,12 @@ __device__ __forceinline__ bool kv_find(const hf_kv_attend_args& a, const uint32
         split = __ballot(split) != 0;
         if (threadIdx.x == 0) a.plan[4 * (int64_t)a.s.batch] = split;
     }
-    const uint32_t eighth = (p.total + 7u) / 8u;
+    // (offsets that cover a row twice, which is reported, can count more units than the call has)
+    const uint32_t eighth = p.total <= a.units ? (p.total + 7u) / 8u : a.units;
+    if (8u * (uint64_t)eighth > a.units) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err, HF_KERR_CORRUPT);
+        return false;
+    }
     cut.unit = blockIdx.x % 8u * eighth + blockIdx.x / 8u;
     if (blockIdx.x / 8u >= eighth) return false;
     const uint32_t unit = cut.unit;

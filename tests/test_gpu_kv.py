@@ -482,6 +482,29 @@ def test_bad_lists_are_reported_and_stay_inside(kv, hf):
         assert torch.equal(c.k, kv_before) and torch.equal(c.k_scale, scale_before)
 
 
+def test_offsets_that_cover_rows_twice(kv, hf):
+    """Offsets that fall let two sequences have the same rows, more than the call is cut for: reported,
+    and nothing outside the outputs and the scratch is written."""
+    from huffman_amd import HuffhipError
+    ctx = hf.Context()
+    batch, n = 40, 64
+    c = make(kv, "e4m3", 64, 16, 8, 64, 32, ctx=ctx)
+    c.k.fill_(0)
+    c.v.fill_(0)
+    table = np.tile(np.arange(64, dtype=np.int32), (batch, 1))
+    cu = np.array([0, n] * (batch // 2) + [0], np.int32)  # every second sequence has all the rows
+    q = torch.zeros(n, 32, 64, device="cuda", dtype=torch.bfloat16)
+    guard = torch.full((2, n, 32, 64), 5.0, device="cuda", dtype=torch.bfloat16)
+    c.attend(q, dev(table), dev(np.full(batch, 1000, np.int32)), dev(cu), max_q=n, out=guard[0])
+    with pytest.raises(HuffhipError):
+        ctx.sync()
+    assert (guard[1] == 5.0).all()
+    # the context goes on as before
+    good = c.attend(q, dev(table[:1]), dev(np.full(1, 1000, np.int32)), dev(cu[:2]), max_q=n)
+    ctx.sync()
+    assert (good == 0).all()
+
+
 def test_refusals(kv, hf):
     c = make(kv, "e4m3", 4, 16, 2, 64, 32)
     t, l = dev(np.zeros((1, 1), np.int32)), dev(np.ones(1, np.int32))
