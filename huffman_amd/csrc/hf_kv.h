@@ -79,7 +79,8 @@ typedef __attribute__((address_space(1))) const int32_t hf_gi32;
 
 // Sequence b of a call, from the device's own lists.  Lists that do not describe rows of the call
 // (offsets that fall or leave the row tensors, more rows than tokens, more tokens than the table
-// holds) give n = 0 and bad = true: nothing of such a sequence is read or written.
+// holds or than 2^31 - 65536, so that the numbers of tokens a little behind the last stay positive)
+// give n = 0 and bad = true: nothing of such a sequence is read or written.
 struct hf_kv_seq {
     int32_t row0, n, past, len;
     bool bad;
@@ -97,7 +98,7 @@ __host__ __device__ __forceinline__ hf_kv_seq hf_kv_sequence(const hf_kv_seqs& s
     q.n = (int32_t)((uint32_t)hi - (uint32_t)lo);  // (may wrap: such lists are bad)
     q.past = (int32_t)((uint32_t)q.len - (uint32_t)q.n);
     q.bad = lo < 0 || hi < lo || (uint32_t)hi > s.rows || (uint32_t)q.n > s.most || q.len < q.n ||
-            (uint64_t)(uint32_t)q.len > ((uint64_t)s.width << page_shift);
+            q.len > 0x7FFF0000 || (uint64_t)(uint32_t)q.len > ((uint64_t)s.width << page_shift);
     if (q.bad) {
         q.row0 = 0;
         q.n = 0;

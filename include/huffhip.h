@@ -584,9 +584,10 @@ int hf_container_codebook(hf_ctx* ctx, const void* d_blob, const hf_container_in
  * behind the last are left as they are.  These lists stay on the device, so a captured call
  * follows their contents; lists that do not fit the call (offsets that fall or leave the row
  * tensors, a sequence of more rows than tokens, or than max_rows in hf_kv_attend, more tokens than
- * the table's row holds, a page number >= n_pages where a page is needed) are reported as
- * HF_ERR_CORRUPT by the next call that synchronises (hf_sync); memory outside the buffers is
- * neither read nor written, and what such a sequence's rows hold afterwards is not defined (offsets that fall: what any row of the call holds).
+ * the table's row holds or than 2^31 - 65536, a page number >= n_pages where a page is needed) are
+ * reported as HF_ERR_CORRUPT by the next call that synchronises (hf_sync); memory outside the
+ * buffers is neither read nor written, and what such a sequence's rows hold afterwards is not
+ * defined (offsets that fall: what any row of the call holds).
  * A page may belong to several sequences (a shared prefix) as long as no call writes it for two.
  *
  * All calls only enqueue work, allocate nothing and can be captured.  Row tensors are 16-byte

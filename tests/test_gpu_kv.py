@@ -505,6 +505,30 @@ def test_offsets_that_cover_rows_twice(kv, hf):
     assert (good == 0).all()
 
 
+def test_the_longest_sequence(kv, hf):
+    """2^31 - 65536 tokens, all in one page of zeros and ones: the outputs are ones and the sum of the
+    weights is the number of tokens; one token more is refused."""
+    from huffman_amd import HuffhipError
+    ctx = hf.Context()
+    pages, size, longest = 32768, 65536, 2**31 - 65536
+    c = make(kv, "e2m1", 1, size, 1, 32, 32, ctx=ctx)
+    c.k.fill_(0)
+    c.v.fill_(0x22)  # 1.0 twice
+    c.k_scale.fill_(127)
+    c.v_scale.fill_(127)
+    table = dev(np.zeros((1, pages), np.int32))
+    q = torch.ones(1, 1, 32, device="cuda", dtype=torch.bfloat16)
+    out, lse = c.attend(q, table, dev(np.array([longest], np.int32)), lse=True)
+    ctx.sync()
+    assert (out == 1).all()
+    # (counts up to 2^24 are exact in fp32: the ranges' are, and fewer than 2^12 of them are added, each
+    # sum off by 2^-24 of itself at most: 2^-12 of the sum, and that much of its logarithm)
+    assert abs(lse.item() - np.log(float(longest))) < 2.0**-12 + 22 * 2.0**-22
+    c.attend(q, table, dev(np.array([longest + 1], np.int32)))
+    with pytest.raises(HuffhipError):
+        ctx.sync()
+
+
 def test_refusals(kv, hf):
     c = make(kv, "e4m3", 4, 16, 2, 64, 32)
     t, l = dev(np.zeros((1, 1), np.int32)), dev(np.ones(1, np.int32))
