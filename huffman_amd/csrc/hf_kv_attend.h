@@ -401,7 +401,7 @@ struct kv_unit {
                 const int d = cuts && 4 * DPC * h + DPC * g >= (int)a.c.head_dim ? 0 : 4 * DPC * h;
                 x.k[b][h].load(pk + d * bits / 8);
             }
-            pk += 4 * a.c.token_stride;
+            pk += 4 * (int64_t)a.c.token_stride;
         }
         if constexpr (bits != 16) {
 #pragma unroll

@@ -529,6 +529,34 @@ def test_the_longest_sequence(kv, hf):
         ctx.sync()
 
 
+@pytest.mark.parametrize("n", [1, 64])
+def test_tokens_a_gibibyte_apart(kv, hf, n):
+    """A pool whose tokens lie 2^30 bytes apart (four of them pass 32 bits) gives, bit for bit, what the
+    same codes next to one another give."""
+    ctx = hf.Context()
+    g = torch.Generator(device="cuda").manual_seed(31)
+    dense = make(kv, "e4m3", 24, 8, 1, 64, 64, ctx=ctx)
+    dense.k.copy_(torch.randint(0, 0x70, dense.k.shape, generator=g, device="cuda", dtype=torch.uint8))
+    dense.v.copy_(torch.randint(0, 0x70, dense.v.shape, generator=g, device="cuda", dtype=torch.uint8))
+    dense.k_scale.fill_(122)
+    dense.v_scale.fill_(125)
+    far = torch.empty(7 * 2**30 + 2 * 24 * 64, dtype=torch.uint8, device="cuda")
+    k = far.as_strided(dense.k.shape, (64, 2**30, 64, 1))
+    v = far.as_strided(dense.k.shape, (64, 2**30, 64, 1), 24 * 64)
+    k.copy_(dense.k)
+    v.copy_(dense.v)
+    wide = kv.KvCache(k, v, dense.k_scale, dense.v_scale, fmt=dense.fmt, ctx=ctx)
+    table = dev(np.random.default_rng(3).permutation(24).astype(np.int32)[None])
+    length, cu = dev(np.array([24 * 8 - 3], np.int32)), dev(np.array([0, n], np.int32))
+    q = torch.randn(n, 4, 64, generator=g, device="cuda").bfloat16()
+    got = [c.attend(q, table, length, cu, max_q=n) for c in (dense, wide)]
+    ctx.sync()
+    assert torch.isfinite(got[0]).all() and torch.equal(*got)
+    read = [c.read(table, length, cu, rows=n) for c in (dense, wide)]
+    ctx.sync()
+    assert torch.equal(read[0][0], read[1][0]) and torch.equal(read[0][1], read[1][1])
+
+
 def test_refusals(kv, hf):
     c = make(kv, "e4m3", 4, 16, 2, 64, 32)
     t, l = dev(np.zeros((1, 1), np.int32)), dev(np.ones(1, np.int32))
