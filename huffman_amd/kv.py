@@ -16,6 +16,7 @@ import torch
 
 from . import _lib as L
 from ._lib import check
+from . import api
 from .api import Context, _Module, default_context
 
 _DTYPES = {torch.bfloat16: L.HF_DT_BF16, torch.float16: L.HF_DT_FP16, torch.float32: L.HF_DT_FP32}
@@ -38,6 +39,9 @@ class KvCache(_Module):
     contiguous last dimension, the same for both.  ``k_scale``, ``v_scale``: uint8 [pages, heads,
     head_dim / group, page_size], contiguous; None for a 16-bit cache.  The pools stay the
     caller's: the cache keeps them alive and never allocates, copies or clears them.
+
+    Without ``ctx`` every call runs on torch's current stream of the pools' device (its default
+    context, made at the first call there, which therefore cannot be a captured one).
 
     In every call ``table`` is int32 [batch, pages of a sequence], ``kv_len`` int32 [batch] (tokens
     of a sequence, the call's rows included) and ``cu`` int32 [batch + 1], the first row of each
@@ -74,6 +78,8 @@ class KvCache(_Module):
         self.k, self.v, self.k_scale, self.v_scale, self.fmt = k, v, k_scale, v_scale, fmt
         self.heads, self.head_dim, self.group, self.page_size = heads, dim, group, page_size
         self._device, self._index = k.device, k.device.index
+        if ctx is not None and ctx.device != self._index:
+            raise ValueError(f"the pools are on {k.device}, the context on cuda:{ctx.device}")
         self._need = {}  # scratch of hf_kv_attend by the sizes it depends on
         size = k.element_size()
         self._c = L.hf_kv_cache(
@@ -92,7 +98,7 @@ class KvCache(_Module):
               group: Optional[int] = None, ctx: Optional[Context] = None) -> "KvCache":
         """A cache with dense pools of its own, cleared.  ``group``: elements of a row that share a
         scale (default: the largest power of two that divides head_dim)."""
-        ctx = ctx if ctx is not None else default_context()
+        own, ctx = ctx, ctx if ctx is not None else default_context()
         dev = f"cuda:{ctx.device}"
         wide = fmt in (L.HF_KV_BF16, L.HF_KV_FP16)
         dtype = {L.HF_KV_BF16: torch.bfloat16, L.HF_KV_FP16: torch.float16}.get(fmt, torch.uint8)
@@ -104,21 +110,31 @@ class KvCache(_Module):
             scales = [None, None] if wide else [
                 torch.full((pages, heads, head_dim // group, page_size), 127, dtype=torch.uint8, device=dev)
                 for _ in range(2)]
-        return KvCache(*pools, *scales, fmt=fmt, ctx=ctx)
+        return KvCache(*pools, *scales, fmt=fmt, ctx=own)
 
     # -- arguments -------------------------------------------------------------------------------
+    @property
+    def ctx(self) -> Context:
+        if self._ctx is not None:
+            return self._ctx
+        stream = torch.cuda.current_stream(self._index)
+        key = (self._index, stream.cuda_stream)
+        ctx = api._default_ctx.get(key)
+        if ctx is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the captured stream has no context yet: make one before the capture "
+                                   "(Context(stream=...)) or call once on that stream")
+            ctx = api._default_ctx[key] = Context(self._index, stream)
+        return ctx
+
     def _handle(self):
-        ctx = self.ctx
-        if ctx.device != self._index:
-            raise ValueError(f"the pools are on {self._device}, the context on cuda:{ctx.device}")
-        return ctx.handle
+        return self.ctx.handle
 
     def _empty(self, *tensors):
         """Tensors (shape, dtype) that belong to the context's stream, where the kernels use them."""
-        ctx = self.ctx
-        if torch.cuda.current_stream(self._index) == ctx.stream:
+        if self._ctx is None or torch.cuda.current_stream(self._index) == self._ctx.stream:
             return [torch.empty(shape, dtype=dtype, device=self._device) for shape, dtype in tensors]
-        with torch.cuda.stream(ctx.stream):
+        with torch.cuda.stream(self._ctx.stream):
             return [torch.empty(shape, dtype=dtype, device=self._device) for shape, dtype in tensors]
 
     def _ints(self, name: str, t: torch.Tensor, dim: int) -> torch.Size:
@@ -222,7 +238,7 @@ class KvCache(_Module):
             bits = mask.data_ptr()
         # The scratch is taken from torch's allocator for this call: another stream's call, or a
         # captured graph, has its own.
-        sizes = (table.shape, rows, max_q, cu is None, heads, self.ctx.device)
+        sizes = (table.shape, rows, max_q, cu is None, heads)
         need = self._need.get(sizes)
         if need is None:
             need = self._need[sizes] = L.lib().hf_kv_attend_work_bytes(handle, cache, b, heads)

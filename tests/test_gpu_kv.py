@@ -557,6 +557,32 @@ def test_tokens_a_gibibyte_apart(kv, hf, n):
     assert torch.equal(read[0][0], read[1][0]) and torch.equal(read[0][1], read[1][1])
 
 
+def test_without_a_context_the_current_stream_is_the_calls(kv, hf):
+    """Calls on a side stream run there, in order with the side stream's own work; a capture on a
+    stream that has no context is refused before anything is captured."""
+    c = make(kv, "e4m3", 4, 16, 2, 64, 32)
+    t, l = dev(np.array([[2]], np.int32)), dev(np.array([1], np.int32))
+    side = torch.cuda.Stream()
+    x = torch.zeros(1, 2, 64, device="cuda", dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        assert c.ctx.stream == side
+        for i in range(1, 30):
+            x.fill_(float(i % 8))
+            c.write(x, x, t, l)
+            k, v = c.read(t, l)
+            assert k.float().max().item() == i % 8 and v.float().min().item() == i % 8
+    assert c.ctx.stream == torch.cuda.current_stream()
+    g = torch.cuda.CUDAGraph()
+    fresh = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="capture"):
+        with torch.cuda.graph(g, stream=fresh):
+            y = x + 1
+            c.write(y, y, t, l)
+    torch.cuda.synchronize()
+
+
 def test_refusals(kv, hf):
     c = make(kv, "e4m3", 4, 16, 2, 64, 32)
     t, l = dev(np.zeros((1, 1), np.int32)), dev(np.ones(1, np.int32))
