@@ -1,9 +1,9 @@
 // Attention of a sequence's last rows over its quantised pages: the kernel, as a template over the
-// type of the queries, the format of the cache, the padded head dimension DP and the row blocks R.
+// type of the queries, the format of the cache and the padded head dimension DP.
 //
 //   o_i = sum_t p_it v_t / sum_t p_it,   p_it = exp(scale q_i . k_t - m_i),   t over what i may see
 //
-// One unit = 16 R rows (tokens x query heads of one cache head of one sequence) against one range
+// One unit = 16 rows (tokens x query heads of one cache head of one sequence) against one range
 // of the sequence's tokens; a workgroup of four wavefronts takes a unit, its wavefronts taking the
 // unit's tokens 32 at a time in turn, each with its own running maximum and sum, and joins them
 // through LDS at the end.  There is no LDS and no barrier in the loop: the products are arranged so
@@ -274,7 +274,7 @@ __device__ __forceinline__ bool kv_find(const hf_kv_attend_args& a, const uint32
 }
 
 // ---- one unit ------------------------------------------------------------------------------------
-template <int QT, int FMT, int DP, int R>
+template <int QT, int FMT, int DP>
 struct kv_unit {
     typedef kv_type<QT> T;
     static constexpr int bits = kv_bits<FMT>();
@@ -304,10 +304,10 @@ struct kv_unit {
     hf_kv_seq q;
     const hf_gi32* table;
     uint32_t groups_of_page;  // groups of eight tokens the table has pages for
-    f32x4 acc[R][VD];
-    f32x4 div[R];         // sums of the rounded p (all four alike)
-    float nm[R], sum[R];  // p = exp2(scale_log2 s + nm); the lane's share of the sum of p
-    hf_u32x4 qr[R][KS];
+    f32x4 acc[VD];
+    f32x4 div;      // sums of the rounded p (all four alike)
+    float nm, sum;  // p = exp2(scale_log2 s + nm); the lane's share of the sum of p
+    hf_u32x4 qr[KS];
     uint32_t bad, odd;  // a page out of range; values that were left out
     // the lane's own part of its places in the pools and in the scales
     const hf_g8 *kbase, *vbase, *ksbase, *vsbase;
@@ -346,26 +346,23 @@ struct kv_unit {
     }
 
     __device__ __forceinline__ void load_q(const int32_t row_lo, const int32_t rows) {
+        const int32_t i = row_lo + m;
+        const bool on = i < rows;
+        const int32_t tok = (on ? i : 0) / (int32_t)a.per, hq = (on ? i : 0) % (int32_t)a.per;
+        const hf_g8* p = (const hf_g8*)a.q.p + ((int64_t)(q.row0 + tok) * a.q.row_stride +
+                                                (int64_t)(head * a.per + hq) * a.q.head_stride) * 2;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int32_t i = row_lo + 16 * r + m;
-            const bool on = i < rows;
-            const int32_t tok = (on ? i : 0) / (int32_t)a.per, hq = (on ? i : 0) % (int32_t)a.per;
-            const hf_g8* p = (const hf_g8*)a.q.p + ((int64_t)(q.row0 + tok) * a.q.row_stride +
-                                                    (int64_t)(head * a.per + hq) * a.q.head_stride) * 2;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const int d = d_of(ks);
-                hf_u32x4 x = {0, 0, 0, 0};
-                if (on && d < (int)a.c.head_dim) x = *(const hf_gmem_u32x4*)(p + 2 * d);
-                qr[r][ks] = x;
-            }
-            nm[r] = 3.402823466e38f;
-            sum[r] = 0.0f;
-            div[r] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int c = 0; c < VD; ++c) acc[r][c] = f32x4{0, 0, 0, 0};
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d = d_of(ks);
+            hf_u32x4 x = {0, 0, 0, 0};
+            if (on && d < (int)a.c.head_dim) x = *(const hf_gmem_u32x4*)(p + 2 * d);
+            qr[ks] = x;
         }
+        nm = 3.402823466e38f;
+        sum = 0.0f;
+        div = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < VD; ++c) acc[c] = f32x4{0, 0, 0, 0};
     }
 
     // Tokens past the end of the sequence are taken from its last group of eight (a page holds
@@ -583,74 +580,54 @@ struct kv_unit {
                     if (d_of(ks) >= (int)a.c.head_dim) ka[b][ks] = hf_u32x4{0, 0, 0, 0};
         }
         next_k();
-        f32x4 s[R][2];
+        f32x4 s[2];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < 2; ++b) {
+            s[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                s[r][b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) s[r][b] = T::mma(ka[b][ks], qr[r][ks], s[r][b]);
-            }
-        uint32_t see[R];
-        float top[R];
-        bool up = false;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if constexpr (!FULL) {
-                const int32_t i = row_lo + 16 * r + m;
-                see[r] = seen((i < rows ? i : 0) / (int32_t)a.per, t, i < rows);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    s[r][e / 4][e % 4] = see[r] >> e & 1u ? s[r][e / 4][e % 4] : -__builtin_inff();
-            }
-            top[r] = s[r][0][0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) top[r] = fmaxf(top[r], s[r][e / 4][e % 4]);
-            up = up || __builtin_fmaf(top[r], a.scale_log2, nm[r]) > T::off + T::rise;
+            for (int ks = 0; ks < KS; ++ks) s[b] = T::mma(ka[b][ks], qr[ks], s[b]);
         }
-        if (__ballot(up)) {  // seldom after the first step: sums and outputs to a new maximum
+        if constexpr (!FULL) {
+            const int32_t i = row_lo + m;
+            const uint32_t see = seen((i < rows ? i : 0) / (int32_t)a.per, t, i < rows);
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const float was = nm[r];
-                nm[r] = fminf(was, T::off - kv_row_max(top[r]) * a.scale_log2);
-                const float f = __builtin_amdgcn_exp2f(nm[r] - was);
-                sum[r] *= f;
-                div[r] *= f;
-#pragma unroll
-                for (int c = 0; c < VD; ++c) acc[r][c] *= f;
-            }
+            for (int e = 0; e < 8; ++e)
+                s[e / 4][e % 4] = see >> e & 1u ? s[e / 4][e % 4] : -__builtin_inff();
         }
-        hf_u32x4 p[R];
+        float top = s[0][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e / 4][e % 4]);
+        // seldom after the first step: sums and outputs to a new maximum
+        if (__ballot(__builtin_fmaf(top, a.scale_log2, nm) > T::off + T::rise)) {
+            const float was = nm;
+            nm = fminf(was, T::off - kv_row_max(top) * a.scale_log2);
+            const float f = __builtin_amdgcn_exp2f(nm - was);
+            sum *= f;
+            div *= f;
+#pragma unroll
+            for (int c = 0; c < VD; ++c) acc[c] *= f;
+        }
+        hf_u32x4 p;
         // (fused: the error of scale x maximum is the same factor for the whole row; where it could
         // pass 1 / 256 of a power of two, the products are rounded first, as the maximum's was)
-        bool far = false;
+        const bool huge = __ballot(fabsf(nm) > 65536.0f && nm != 3.402823466e38f) != 0;
+        float e[8];
+        if (huge) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) far = far || (fabsf(nm[r]) > 65536.0f && nm[r] != 3.402823466e38f);
-        const bool huge = __ballot(far) != 0;
+            for (int i = 0; i < 8; ++i) e[i] = s[i / 4][i % 4] * a.scale_log2 + nm;
+        } else {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float e[8];
-            if (huge) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = s[r][i / 4][i % 4] * a.scale_log2 + nm[r];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = __builtin_fmaf(s[r][i / 4][i % 4], a.scale_log2, nm[r]);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                e[i] = __builtin_amdgcn_exp2f(e[i]);
-                sum[r] += e[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[r][i] = T::pack(e[2 * i], e[2 * i + 1]);
+            for (int i = 0; i < 8; ++i) e[i] = __builtin_fmaf(s[i / 4][i % 4], a.scale_log2, nm);
         }
-        {
-            constexpr uint32_t two = T::one | T::one << 16;
 #pragma unroll
-            for (int r = 0; r < R; ++r) div[r] = T::mma(hf_u32x4{two, two, two, two}, p[r], div[r]);
+        for (int i = 0; i < 8; ++i) {
+            e[i] = __builtin_amdgcn_exp2f(e[i]);
+            sum += e[i];
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = T::pack(e[2 * i], e[2 * i + 1]);
+        constexpr uint32_t two = T::one | T::one << 16;
+        div = T::mma(hf_u32x4{two, two, two, two}, p, div);
         hf_u32x4 av[VD];
         uint32_t there = 0xFFu;
         if constexpr (!FULL) {
@@ -673,8 +650,7 @@ struct kv_unit {
         }
 #pragma unroll
         for (int c = 0; c < VD; ++c)
-#pragma unroll
-            for (int r = 0; r < R; ++r) acc[r][c] = T::mma(av[c], p[r], acc[r][c]);
+            acc[c] = T::mma(av[c], p, acc[c]);
     }
 
     // The values of tokens t .. t + 31 that are not finite, to the rows that see them.
@@ -686,21 +662,18 @@ struct kv_unit {
             const uint32_t off = at & ((1u << a.c.page_shift) - 1u);
             const hf_g8* p = (const hf_g8*)a.c.v + (int64_t)pg * a.c.page_stride + (int64_t)off * a.c.token_stride +
                              (int64_t)head * a.c.head_stride;
+            const int32_t i = row_lo + m;
+            const bool on = i < rows;
+            const bool sees = on && (at < (uint32_t)q.past || (seen_at((on ? i : 0) / (int32_t)a.per, at, on) & 1u));
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int32_t i = row_lo + 16 * r + m;
-                const bool on = i < rows;
-                const bool sees = on && (at < (uint32_t)q.past || (seen_at((on ? i : 0) / (int32_t)a.per, at, on) & 1u));
+            for (int e = 0; e < 4; ++e) {
+                const int d = VD * (4 * g + e);
+                if (sees && d < (int)a.c.head_dim) {
+                    float v[VD];
+                    values(p + d * bits / 8, pg, off, d, v);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int d = VD * (4 * g + e);
-                    if (sees && d < (int)a.c.head_dim) {
-                        float v[VD];
-                        values(p + d * bits / 8, pg, off, d, v);
-#pragma unroll
-                        for (int c = 0; c < VD; ++c)
-                            if (!(fabsf(v[c]) <= 3.402823466e38f)) acc[r][c][e] += v[c];
-                    }
+                    for (int c = 0; c < VD; ++c)
+                        if (!(fabsf(v[c]) <= 3.402823466e38f)) acc[c][e] += v[c];
                 }
             }
         }
@@ -713,18 +686,22 @@ __device__ __forceinline__ float kv_lse(const float nm, const float sum) {
 }
 
 // Scratch of a workgroup: what two wavefronts hand to the other two.
-template <int DP, int R>
+template <int DP>
 struct kv_lds {
-    f32x4 acc[2][R][DP / 16][64];
-    float nm[2][R][64], sum[2][R][64], div[2][R][64];
+    f32x4 acc[2][DP / 16][64];
+    float nm[2][64], sum[2][64], div[2][64];
 };
 
-template <int QT, int FMT, int DP, int R>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(R == 4 || DP * R > 256 ? 1 : 2)))
+// Bound by memory and the latency of its loads: 64 sequences of up to 8001 tokens, 8 heads of 128 in
+// e4m3 (675 MB), in 145 us, 4.6 TB/s; 64 of 32 k at 5.1 TB/s, where a large read reaches 6.1.  The
+// registers of a tile are loaded again as soon as they have been turned into operands (a second tile
+// in flight costs a wavefront of two and was slower, 187 us).
+template <int QT, int FMT, int DP>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
 void hf_k_kv_attend(const hf_kv_attend_args a) {
-    typedef kv_unit<QT, FMT, DP, R> U;
-    constexpr uint32_t tile_rows = 16 * R;
-    __shared__ kv_lds<DP, R> lds;
+    typedef kv_unit<QT, FMT, DP> U;
+    constexpr uint32_t tile_rows = 16;
+    __shared__ kv_lds<DP> lds;
     kv_cut cut;
     if (!kv_find(a, tile_rows, cut)) return;
     U u(a);
@@ -757,8 +734,7 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
         u.load_k(t, p, x);
         u.load_v(t, p, x);
         u.find(t + stride, p);
-#pragma unroll
-        for (int r = 0; r < R; ++r) kv_arrived(u.qr[r]);
+        kv_arrived(u.qr);
         auto one = [&](auto&& next_k, auto&& next_v) {
             if (t + kStep <= whole && t + kStep <= end) u.template step<true>(t, x, row_lo, rows, next_k, next_v);
             else u.template step<false>(t, x, row_lo, rows, next_k, next_v);
@@ -782,81 +758,68 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
     if (u.bad) atomicOr(a.err, HF_KERR_CORRUPT);
 
     // join the wavefronts: 2 and 3 hand to 0 and 1, then 1 to 0
-#pragma unroll
-    for (int r = 0; r < R; ++r) u.sum[r] = kv_row_sum(u.sum[r]);
+    u.sum = kv_row_sum(u.sum);
 #pragma unroll 1
     for (int half = 2; half >= 1; half >>= 1) {
         if (wave >= half && wave < 2 * half) {
+            lds.nm[wave - half][u.lane] = u.nm;
+            lds.sum[wave - half][u.lane] = u.sum;
+            lds.div[wave - half][u.lane] = u.div[0];
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                lds.nm[wave - half][r][u.lane] = u.nm[r];
-                lds.sum[wave - half][r][u.lane] = u.sum[r];
-                lds.div[wave - half][r][u.lane] = u.div[r][0];
-#pragma unroll
-                for (int c = 0; c < U::VD; ++c) lds.acc[wave - half][r][c][u.lane] = u.acc[r][c];
-            }
+            for (int c = 0; c < U::VD; ++c) lds.acc[wave - half][c][u.lane] = u.acc[c];
         }
         __syncthreads();
         if (wave < half) {
+            const float other = lds.nm[wave][u.lane];
+            const float least = fminf(u.nm, other);
+            const float f = __builtin_amdgcn_exp2f(least - u.nm);
+            const float h = __builtin_amdgcn_exp2f(least - other);
+            u.nm = least;
+            u.sum = u.sum * f + lds.sum[wave][u.lane] * h;
+            u.div[0] = u.div[0] * f + lds.div[wave][u.lane] * h;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const float other = lds.nm[wave][r][u.lane];
-                const float least = fminf(u.nm[r], other);
-                const float f = __builtin_amdgcn_exp2f(least - u.nm[r]);
-                const float h = __builtin_amdgcn_exp2f(least - other);
-                u.nm[r] = least;
-                u.sum[r] = u.sum[r] * f + lds.sum[wave][r][u.lane] * h;
-                u.div[r][0] = u.div[r][0] * f + lds.div[wave][r][u.lane] * h;
-#pragma unroll
-                for (int c = 0; c < U::VD; ++c) u.acc[r][c] = u.acc[r][c] * f + lds.acc[wave][r][c][u.lane] * h;
-            }
+            for (int c = 0; c < U::VD; ++c) u.acc[c] = u.acc[c] * f + lds.acc[wave][c][u.lane] * h;
         }
         __syncthreads();
     }
     if (wave != 0) return;
+    const int32_t i = row_lo + u.m;
+    if (i >= rows) return;
+    if (cut.ranges > 1) {  // to be joined with the other ranges
+        const int64_t row = (int64_t)cut.unit * tile_rows + u.m;
+        float* dst = a.part + row * DP;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int32_t i = row_lo + 16 * r + u.m;
-        if (cut.ranges > 1) {  // to be joined with the other ranges
-            if (i >= rows) continue;
-            const int64_t row = (int64_t)cut.unit * tile_rows + 16 * r + u.m;
-            float* dst = a.part + row * DP;
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int c = 0; c < U::VD; c += 4)
+                *(f32x4*)(dst + U::VD * (4 * u.g + e) + c) =
+                    f32x4{u.acc[c][e], u.acc[c + 1][e], u.acc[c + 2][e], u.acc[c + 3][e]};
+        if (u.g == 0) *(f32x4*)(a.part_ml + 4 * row) = f32x4{u.nm, u.sum, u.div[0], 0.0f};
+    } else {
+        const int32_t tok = i / (int32_t)a.per, hq = i % (int32_t)a.per;
+        const uint32_t out_head = u.head * a.per + hq;
+        const float f = u.div[0] == 0.0f ? 0.0f : 1.0f / u.div[0];  // no token seen: zeros
+        hf_g8* dst = (hf_g8*)a.out.p + ((int64_t)(u.q.row0 + tok) * a.out.row_stride +
+                                        (int64_t)out_head * a.out.head_stride) * 2;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int d = U::VD * (4 * u.g + e);
+            if (d < (int)a.c.head_dim) {
 #pragma unroll
                 for (int c = 0; c < U::VD; c += 4)
-                    *(f32x4*)(dst + U::VD * (4 * u.g + e) + c) =
-                        f32x4{u.acc[r][c][e], u.acc[r][c + 1][e], u.acc[r][c + 2][e], u.acc[r][c + 3][e]};
-            if (u.g == 0) {
-                *(f32x4*)(a.part_ml + 4 * row) = f32x4{u.nm[r], u.sum[r], u.div[r][0], 0.0f};
+                    *(hf_gmem_u32x2*)(dst + 2 * (d + c)) =
+                        hf_u32x2{U::T::pack(u.acc[c][e] * f, u.acc[c + 1][e] * f),
+                                 U::T::pack(u.acc[c + 2][e] * f, u.acc[c + 3][e] * f)};
             }
-        } else if (i < rows) {
-            const int32_t tok = i / (int32_t)a.per, hq = i % (int32_t)a.per;
-            const uint32_t out_head = u.head * a.per + hq;
-            const float l = u.sum[r], w = u.div[r][0];
-            const float f = w == 0.0f ? 0.0f : 1.0f / w;  // no token seen: zeros
-            hf_g8* dst = (hf_g8*)a.out.p + ((int64_t)(u.q.row0 + tok) * a.out.row_stride +
-                                            (int64_t)out_head * a.out.head_stride) * 2;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int d = U::VD * (4 * u.g + e);
-                if (d < (int)a.c.head_dim) {
-#pragma unroll
-                    for (int c = 0; c < U::VD; c += 4)
-                        *(hf_gmem_u32x2*)(dst + 2 * (d + c)) =
-                            hf_u32x2{U::T::pack(u.acc[r][c][e] * f, u.acc[r][c + 1][e] * f),
-                                     U::T::pack(u.acc[r][c + 2][e] * f, u.acc[r][c + 3][e] * f)};
-                }
-            }
-            if (a.lse && u.g == 0)
-                a.lse[(int64_t)(u.q.row0 + tok) * a.c.heads * a.per + out_head] =
-                    kv_lse(u.nm[r], l);
         }
+        if (a.lse && u.g == 0)
+            a.lse[(int64_t)(u.q.row0 + tok) * a.c.heads * a.per + out_head] = kv_lse(u.nm, u.sum);
     }
 }
 
 // Joins the ranges of rows that have several: a wavefront takes a row of a head at a time, DP / 4
-// lanes along it and the ranges dealt to the groups of lanes that are left.
+// lanes along it and the ranges dealt to the groups of lanes that are left.  4 us for one
+// token, 10 for eight trees of up to 63 tokens x 32 heads in four ranges.
 template <int QT, int DP>
 __global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a, const uint32_t tile_rows) {
     typedef kv_type<QT> T;
