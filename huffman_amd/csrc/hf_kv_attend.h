@@ -693,7 +693,7 @@ struct kv_lds {
 };
 
 // Bound by memory and the latency of its loads: 64 sequences of up to 8001 tokens, 8 heads of 128 in
-// e4m3 (675 MB), in 145 us, 4.6 TB/s; 64 of 32 k at 5.1 TB/s, where a large read reaches 6.1.  The
+// e4m3 (675 MB), in 151 us, 4.5 TB/s; 64 of 32 k at 5.1 TB/s, where a large read reaches 6.1.  The
 // registers of a tile are loaded again as soon as they have been turned into operands (a second tile
 // in flight costs a wavefront of two and was slower, 187 us).
 template <int QT, int FMT, int DP>

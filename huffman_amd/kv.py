@@ -31,6 +31,12 @@ _POOL_DTYPES = {
 }
 
 
+def _raw_stream(index: int) -> int:
+    """hipStream_t of torch's current stream; building the Stream object takes as long as a third of a
+    write call's launch (1.2 us)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 class KvCache(_Module):
     """Two page pools and their scales (include/huffhip.h has the layout and the arithmetic).
 
@@ -117,10 +123,10 @@ class KvCache(_Module):
     def ctx(self) -> Context:
         if self._ctx is not None:
             return self._ctx
-        stream = torch.cuda.current_stream(self._index)
-        key = (self._index, stream.cuda_stream)
+        key = (self._index, _raw_stream(self._index))
         ctx = api._default_ctx.get(key)
         if ctx is None:
+            stream = torch.cuda.current_stream(self._index)
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the captured stream has no context yet: make one before the capture "
                                    "(Context(stream=...)) or call once on that stream")
@@ -132,7 +138,7 @@ class KvCache(_Module):
 
     def _empty(self, *tensors):
         """Tensors (shape, dtype) that belong to the context's stream, where the kernels use them."""
-        if self._ctx is None or torch.cuda.current_stream(self._index) == self._ctx.stream:
+        if self._ctx is None or _raw_stream(self._index) == self._ctx.stream.cuda_stream:
             return [torch.empty(shape, dtype=dtype, device=self._device) for shape, dtype in tensors]
         with torch.cuda.stream(self._ctx.stream):
             return [torch.empty(shape, dtype=dtype, device=self._device) for shape, dtype in tensors]
