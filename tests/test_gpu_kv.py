@@ -273,7 +273,7 @@ def test_attend_scales_and_strides(kv, fmt, dtype, scale):
     wide = torch.full((n + 3, 2, 6, 128), 3.0, dtype=DT[dtype], device="cuda")
     wide[:n, 0] = q.cuda()
     out = wide[:, 1]
-    tall = torch.cat([mask, np.zeros((3, mask.shape[1]), np.uint32)]) if False else np.pad(mask, ((0, 3), (0, 0)))
+    tall = np.pad(mask, ((0, 3), (0, 0)))
     got, lse = c.attend(wide[:, 0], dev(table), dev(kv_len), dev(cu), max_q=20, mask=dev(tall.view(np.int32)),
                         scale=scale, lse=True, out=out)
     c.ctx.sync()
