@@ -1655,7 +1655,9 @@ int kv_plan_of(const hf_ctx* ctx, const hf_kv_pools& p, const hf_kv_seqs& s, uin
     const uint64_t pad = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
     o->part_floats = o->join ? units * (uint64_t)o->tile_rows * pad : 0;
     o->ml_floats = o->join ? 4 * units * (uint64_t)o->tile_rows : 0;
-    o->bytes = o->join ? 4 * (o->part_floats + o->ml_floats) + 16 * ((uint64_t)s.batch + 1) : 0;
+    // (the cut is in memory for the join, and for calls that make it in a launch of its own)
+    const bool cut = o->join || s.batch > HF_KV_OWN_CUT;
+    o->bytes = 4 * (o->part_floats + o->ml_floats) + (cut ? 16 * ((uint64_t)s.batch + 1) : 0);
     return HF_OK;
 }
 

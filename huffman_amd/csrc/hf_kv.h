@@ -52,13 +52,16 @@ struct hf_kv_attend_args {
     float scale_log2;      // softmax scale x log2(e)
     float* part;           // partial outputs of the units, [units][rows of a tile][padded head_dim]
     float* part_ml;        // their maxima and two sums, [units][rows of a tile][4]
-    uint32_t* plan;        // [batch + 1][4]: the cut, for joining
+    uint32_t* plan;        // [batch + 1][4]: the cut (of few sequences: for joining only)
     uint32_t target;       // units the call is cut into, about
     uint32_t min_steps;    // tokens / 32 a unit has at least
     uint32_t units;        // workgroups of the call, and room of the partial buffers
     uint32_t join;         // units may have to be joined (the partial buffers exist)
     uint32_t* err;
 };
+
+// up to this many sequences, attention finds its units without a launch in front
+constexpr uint32_t HF_KV_OWN_CUT = 128;
 
 int hf_kv_attend_tile_rows(uint32_t max_q, uint32_t per, uint32_t head_dim);
 void hf_launch_kv_write(const hf_kv_pools& c, const hf_kv_seqs& s, const hf_kv_rows& k,

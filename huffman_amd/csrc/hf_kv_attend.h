@@ -137,8 +137,8 @@ __device__ __forceinline__ void kv_arrived(hf_u32x4 (&x)[N]) {
 }
 
 // ---- the cut of a call into units ---------------------------------------------------------------
-// Every wavefront finds its unit from the device's own lengths, so a captured call follows lengths
-// that change between replays and a ragged batch is cut evenly.  All sequences' steps (32 tokens)
+// The cut is made on the device from the call's own lengths, so a captured call follows lengths that
+// change between replays and a ragged batch is cut evenly.  All sequences' steps (32 tokens)
 // times their row tiles are summed and divided by the units aimed at; a sequence has as many equal
 // ranges as it needs for about that many steps.  Tiles of 16 rows leave little behind per unit (a
 // range's partial outputs), so their units are many and small.  Larger tiles leave as much as they
@@ -148,7 +148,9 @@ __device__ __forceinline__ void kv_arrived(hf_u32x4 (&x)[N]) {
 // Units of a sequence are numbered range by range, in it by cache head, in it by row tile, so that
 // the tiles that read the same tokens are neighbours; and since consecutive workgroups go to the
 // eight XCDs in turn, each with an L2 of its own, XCD x takes the x-th eighth of the units.
-// Workgroup 0 leaves the cut in memory for the kernel that joins the ranges.
+// Up to HF_KV_OWN_CUT sequences every wavefront makes the whole cut by itself, a sequence to a lane, and
+// workgroup 0 leaves it in memory for the kernel that joins the ranges.  More sequences are cut by
+// one workgroup in a launch in front (hf_k_kv_plan), and a unit is searched in what it left.
 struct kv_cut {
     uint32_t unit, b, n_before;  // unit; its sequence; units of the sequences before that
     uint32_t tiles, ranges, steps_each;
@@ -167,9 +169,6 @@ __device__ __forceinline__ kv_shape kv_shape_of(const hf_kv_attend_args& a, cons
     return s;
 }
 __device__ __forceinline__ uint32_t kv_div_up(const uint32_t x, const uint32_t y) { return (x + y - 1u) / y; }
-__device__ __forceinline__ uint32_t kv_ranges(const kv_shape& s, const uint32_t each, const uint32_t slack) {
-    return s.steps <= each + slack ? 1u : kv_div_up(s.steps - slack, each);
-}
 __device__ __forceinline__ uint32_t kv_wave_scan(const uint32_t v) {  // inclusive
     uint32_t incl = v;
 #pragma unroll
@@ -184,38 +183,50 @@ __device__ __forceinline__ float kv_wave_sum(float v) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
+struct kv_steps {
+    uint32_t each, slack;  // steps of a range, those let pass
+    bool fit;              // the units are to be no more than aimed at
+    // (the sums of tiles x steps and of tiles decide nothing but the cut, and all who make it have the
+    // same ones: floats do)
+    __device__ __forceinline__ kv_steps(const hf_kv_attend_args& a, const uint32_t tile_rows, const float work,
+                                        const float tiles) {
+        each = max((uint32_t)(work / (float)a.target * 1.0001f) + 1u, a.min_steps);
+        fit = tile_rows > 16 && 2.0f * tiles <= (float)a.target;
+        slack = tile_rows > 16 && !fit ? each / 4u : 0u;
+    }
+    __device__ __forceinline__ uint32_t ranges(const kv_shape& s) const {
+        return s.steps <= each + slack ? 1u : kv_div_up(s.steps - slack, each);
+    }
+    // whether units were too many and are to be counted again
+    __device__ __forceinline__ bool raise(const hf_kv_attend_args& a, const uint32_t units, const int turn) {
+        if (!fit || turn == 8 || units <= a.target) return false;
+        each += max(1u, each / 16u);
+        return true;
+    }
+};
 struct kv_plan_dev {
-    uint32_t each, slack, total;  // steps of a range, those let pass, units
+    kv_steps steps;
+    uint32_t total;  // units
     kv_shape first;  // of the lane's sequence among the first 64: most calls have no more
 };
 __device__ __forceinline__ kv_plan_dev kv_plan_now(const hf_kv_attend_args& a, const uint32_t tile_rows) {
-    kv_plan_dev p;
-    p.first = kv_shape_of(a, tile_rows, hf_lane());
-    // (the sums decide nothing but the cut, and every wavefront takes the same ones: floats do)
-    float work = (float)p.first.tiles * (float)p.first.steps, tiles = (float)p.first.tiles;
+    const kv_shape lane = kv_shape_of(a, tile_rows, hf_lane());
+    float work = (float)lane.tiles * (float)lane.steps, tiles = (float)lane.tiles;
     for (uint32_t b0 = 64; b0 < a.s.batch; b0 += 64) {
         const kv_shape s = kv_shape_of(a, tile_rows, b0 + hf_lane());
         work += (float)s.tiles * (float)s.steps;
         tiles += (float)s.tiles;
     }
-    work = kv_wave_sum(work);
-    p.each = max((uint32_t)(work / (float)a.target * 1.0001f) + 1u, a.min_steps);
-    p.slack = 0;
-    bool fit = false;
-    if (tile_rows > 16) {
-        fit = 2.0f * kv_wave_sum(tiles) <= (float)a.target;
-        if (!fit) p.slack = p.each / 4u;
-    }
-    for (int turn = 0;; ++turn) {
-        uint32_t total = p.first.tiles * kv_ranges(p.first, p.each, p.slack);
+    kv_plan_dev p = {kv_steps(a, tile_rows, kv_wave_sum(work), kv_wave_sum(tiles)), 0u, lane};
+    int turn = 0;
+    do {
+        uint32_t total = p.first.tiles * p.steps.ranges(p.first);
         for (uint32_t b0 = 64; b0 < a.s.batch; b0 += 64) {
             const kv_shape s = kv_shape_of(a, tile_rows, b0 + hf_lane());
-            total += s.tiles * kv_ranges(s, p.each, p.slack);
+            total += s.tiles * p.steps.ranges(s);
         }
         p.total = hf_wave_sum_u32(total);
-        if (!fit || turn == 8 || p.total <= a.target) break;
-        p.each += max(1u, p.each / 16u);
-    }
+    } while (p.steps.raise(a, p.total, turn++));
     return p;
 }
 // Walks the sequences 64 at a time; `pick` sees a lane's sequence, its shape and ranges and the units
@@ -228,7 +239,7 @@ __device__ __forceinline__ bool kv_walk(const hf_kv_attend_args& a, const uint32
         const uint32_t b = b0 + hf_lane();
         kv_shape s = p.first;
         if (b0) s = kv_shape_of(a, tile_rows, b);
-        const uint32_t ranges = kv_ranges(s, p.each, p.slack);
+        const uint32_t ranges = p.steps.ranges(s);
         const uint32_t own = s.tiles * ranges, incl = kv_wave_scan(own);
         const unsigned long long hit = __ballot(pick(b, s, ranges, before + incl - own));
         if (hit) {
@@ -245,28 +256,55 @@ __device__ __forceinline__ bool kv_walk(const hf_kv_attend_args& a, const uint32
     }
     return false;
 }
-// What the joining kernel reads of a sequence: units before it, tiles, ranges; behind the last
-// sequence: whether any has more than one range.
+// The unit of this workgroup among `total`; false: none.
+__device__ __forceinline__ bool kv_unit_of(const hf_kv_attend_args& a, const uint32_t total, uint32_t& unit) {
+    // (offsets that cover a row twice, which is reported, can count more units than the call has)
+    const uint32_t eighth = total <= a.units ? (total + 7u) / 8u : a.units;
+    if (8u * (uint64_t)eighth > a.units) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err, HF_KERR_CORRUPT);
+        return false;
+    }
+    unit = blockIdx.x % 8u * eighth + blockIdx.x / 8u;
+    return blockIdx.x / 8u < eighth && unit < total;
+}
+// The unit's sequence in the cut that hf_k_kv_plan left: the last one with no more units before it
+// than the unit's number, 64 looked at at a time.
+__device__ __forceinline__ bool kv_search(const hf_kv_attend_args& a, kv_cut& cut) {
+    const uint32_t total = __builtin_amdgcn_readfirstlane(a.plan[4 * (int64_t)a.s.batch + 1]);
+    if (!kv_unit_of(a, total, cut.unit)) return false;
+    uint32_t b = 0, among = a.s.batch;
+    while (among > 1) {
+        const uint32_t apart = (among + 63u) / 64u, at = apart * hf_lane();
+        bool before = false;
+        if (at < among) before = a.plan[4 * (int64_t)(b + at)] <= cut.unit;
+        const uint32_t k = max((int)__popcll(__ballot(before)), 1) - 1;
+        b += k * apart;
+        among = min(apart, among - k * apart);
+    }
+    const hf_u32x4 p = *(const hf_u32x4*)(a.plan + 4 * (int64_t)b);
+    cut.b = b;
+    cut.n_before = __builtin_amdgcn_readfirstlane(p[0]);
+    cut.tiles = __builtin_amdgcn_readfirstlane(p[1]);
+    cut.ranges = __builtin_amdgcn_readfirstlane(p[2]);
+    cut.steps_each = (kv_div_up(__builtin_amdgcn_readfirstlane(p[3]), cut.ranges) + kWaves - 1u) / kWaves * kWaves;
+    return __builtin_amdgcn_readfirstlane(cut.unit) - cut.n_before < cut.tiles * cut.ranges;
+}
+// The cut in memory: of each sequence the units before it, tiles, ranges and steps; behind the last
+// sequence whether any has more than one range, and all units.
 __device__ __forceinline__ bool kv_find(const hf_kv_attend_args& a, const uint32_t tile_rows, kv_cut& cut) {
+    if (a.s.batch > HF_KV_OWN_CUT) return kv_search(a, cut);
     const kv_plan_dev p = kv_plan_now(a, tile_rows);
     if (blockIdx.x == 0 && threadIdx.x < 64 && a.join) {
         bool split = false;
         kv_walk(a, tile_rows, p, [&](const uint32_t b, const kv_shape& s, const uint32_t ranges, const uint32_t first) {
-            if (b < a.s.batch) *(hf_u32x4*)(a.plan + 4 * (int64_t)b) = hf_u32x4{first, s.tiles, ranges, 0};
+            if (b < a.s.batch) *(hf_u32x4*)(a.plan + 4 * (int64_t)b) = hf_u32x4{first, s.tiles, ranges, s.steps};
             split = split || (s.tiles && ranges > 1);
             return false;
         }, cut);
         split = __ballot(split) != 0;
         if (threadIdx.x == 0) a.plan[4 * (int64_t)a.s.batch] = split;
     }
-    // (offsets that cover a row twice, which is reported, can count more units than the call has)
-    const uint32_t eighth = p.total <= a.units ? (p.total + 7u) / 8u : a.units;
-    if (8u * (uint64_t)eighth > a.units) {
-        if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err, HF_KERR_CORRUPT);
-        return false;
-    }
-    cut.unit = blockIdx.x % 8u * eighth + blockIdx.x / 8u;
-    if (blockIdx.x / 8u >= eighth) return false;
+    if (!kv_unit_of(a, p.total, cut.unit)) return false;
     const uint32_t unit = cut.unit;
     return kv_walk(a, tile_rows, p, [&](uint32_t, const kv_shape& s, const uint32_t ranges, const uint32_t first) {
         return unit < first + s.tiles * ranges;

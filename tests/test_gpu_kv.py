@@ -342,6 +342,58 @@ def test_attend_rows_that_see_nothing(kv, fmt):
         verify(c, f, q, table, kv_len, cu, mask, got, lse, 0.5, "bf16")
 
 
+@pytest.mark.parametrize("batch", [127, 128, 129, 1025, 4100])
+@pytest.mark.parametrize("most,page", [(1, 64), (3, 8), (40, 16)])
+def test_attend_many_sequences(kv, hf, batch, most, page):
+    """Ragged batches around the number of sequences from which the call is cut in a launch of its own,
+    some without rows; captured once and replayed for other lengths; one sequence that does not fit."""
+    from huffman_amd import HuffhipError
+    if batch * most > 20000:
+        pytest.skip("the reference takes long")
+    rng = np.random.default_rng(batch + most)
+    new = [1] * batch if most == 1 else [int(n) for n in rng.integers(0, most + 1, batch)]
+    past = [int(n) for n in rng.integers(0, 40, batch)]
+    past[batch // 2], new[batch - 1] = 4000, most  # one long one, cut into ranges
+    stream = torch.cuda.Stream()
+    ctx = hf.Context(stream=stream)
+    c, f, q, table, kv_len, cu, _ = attend_case(kv, "e4m3", "bf16", new, past, page, 1, 2, 64, 64, "thd", None, 1, ctx)
+    qd, t, l, o = q.cuda(), dev(table), dev(kv_len), dev(cu)
+    out = torch.full_like(qd, 7.0)
+    torch.cuda.synchronize()
+    call = dict(cu=None if most == 1 else o, max_q=most, lse=True, out=out)
+    got, lse = c.attend(qd, t, l, **call)
+    ctx.sync()
+    verify(c, f, q, table, kv_len, cu, None, got, lse, 64 ** -0.5, "bf16")
+    first = got.clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        _, lse = c.attend(qd, t, l, **call)
+    shorter = np.minimum(kv_len, np.maximum(np.array(new), kv_len // 2)).astype(np.int32)
+    for lengths in (kv_len, shorter, kv_len):
+        l.copy_(dev(lengths))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            g.replay()
+        ctx.sync()
+        verify(c, f, q, table, lengths, cu, None, out, lse, 64 ** -0.5, "bf16")
+    assert torch.equal(out.view(torch.int16), first.view(torch.int16))
+    bad = kv_len.copy()
+    bad[3] = -1
+    l.copy_(dev(bad))
+    torch.cuda.synchronize()
+    _, lse2 = c.attend(qd, t, l, **call)
+    with pytest.raises(HuffhipError):
+        ctx.sync()
+    if new[3]:  # (the call may be cut otherwise without it: the others by the definition again)
+        keep = np.arange(batch) != 3
+        rest = np.r_[0:cu[3], cu[4]:cu[-1]]
+        verify(c, f, q[torch.from_numpy(rest)], table[keep], kv_len[keep],
+               np.concatenate([[0], np.cumsum(np.array(new)[keep])]).astype(np.int32), None, out[dev(rest)], lse2[dev(rest)],
+               64 ** -0.5, "bf16")
+
+
 def test_attend_long_and_past_four_gigabytes(kv):
     """A pool of more than 2^32 bytes, its last pages in use; a context cut into many ranges."""
     pages, page, dim = 35000, 64, 128  # 35000 x 64 x 16 x 128 = 4.6 GB a pool
@@ -482,12 +534,13 @@ def test_bad_lists_are_reported_and_stay_inside(kv, hf):
         assert torch.equal(c.k, kv_before) and torch.equal(c.k_scale, scale_before)
 
 
-def test_offsets_that_cover_rows_twice(kv, hf):
+@pytest.mark.parametrize("batch", [40, 200])
+def test_offsets_that_cover_rows_twice(kv, hf, batch):
     """Offsets that fall let two sequences have the same rows, more than the call is cut for: reported,
     and nothing outside the outputs and the scratch is written."""
     from huffman_amd import HuffhipError
     ctx = hf.Context()
-    batch, n = 40, 64
+    n = 64
     c = make(kv, "e4m3", 64, 16, 8, 64, 32, ctx=ctx)
     c.k.fill_(0)
     c.v.fill_(0)
