@@ -267,20 +267,28 @@ __device__ __forceinline__ bool kv_unit_of(const hf_kv_attend_args& a, const uin
     unit = blockIdx.x % 8u * eighth + blockIdx.x / 8u;
     return blockIdx.x / 8u < eighth && unit < total;
 }
+// The last of `count` numbers, which ascend, that is at most `most` (the first, if none is), for a
+// wavefront: 64 looked at at a time.  `number` gives the i-th.
+template <typename F>
+__device__ __forceinline__ uint32_t kv_last(const uint32_t count, F&& number, const uint32_t most) {
+    uint32_t at = 0, among = count;
+    while (among > 1) {
+        const uint32_t apart = (among + 63u) / 64u, mine = apart * hf_lane();
+        bool past = true;
+        if (mine < among) past = number(at + mine) > most;
+        const unsigned long long ends = __ballot(past);
+        const uint32_t k = ends ? max((int)__ffsll(ends) - 2, 0) : 63;
+        at += k * apart;
+        among = min(apart, among - k * apart);
+    }
+    return at;
+}
 // The unit's sequence in the cut that hf_k_kv_plan left: the last one with no more units before it
-// than the unit's number, 64 looked at at a time.
+// than the unit's number.
 __device__ __forceinline__ bool kv_search(const hf_kv_attend_args& a, kv_cut& cut) {
     const uint32_t total = __builtin_amdgcn_readfirstlane(a.plan[4 * (int64_t)a.s.batch + 1]);
     if (!kv_unit_of(a, total, cut.unit)) return false;
-    uint32_t b = 0, among = a.s.batch;
-    while (among > 1) {
-        const uint32_t apart = (among + 63u) / 64u, at = apart * hf_lane();
-        bool before = false;
-        if (at < among) before = a.plan[4 * (int64_t)(b + at)] <= cut.unit;
-        const uint32_t k = max((int)__popcll(__ballot(before)), 1) - 1;
-        b += k * apart;
-        among = min(apart, among - k * apart);
-    }
+    const uint32_t b = kv_last(a.s.batch, [&](const uint32_t i) { return a.plan[4 * (int64_t)i]; }, cut.unit);
     const hf_u32x4 p = *(const hf_u32x4*)(a.plan + 4 * (int64_t)b);
     cut.b = b;
     cut.n_before = __builtin_amdgcn_readfirstlane(p[0]);
@@ -857,7 +865,8 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
 
 // Joins the ranges of rows that have several: a wavefront takes a row of a head at a time, DP / 4
 // lanes along it and the ranges dealt to the groups of lanes that are left.  4 us for one
-// token, 10 for eight trees of up to 63 tokens x 32 heads in four ranges.
+// token, 10 for eight trees of up to 63 tokens x 32 heads in four ranges.  A row's sequence is searched
+// (the whole call for 4096 sequences of 3 rows, one of them long: 876 us; with the offsets walked 1420).
 template <int QT, int DP>
 __global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a, const uint32_t tile_rows) {
     typedef kv_type<QT> T;
@@ -868,16 +877,10 @@ __global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a, c
     for (uint32_t id = first_id; id < all; id += gridDim.x * 4u) {
         const int32_t row = (int32_t)(id / q_heads);
         const uint32_t out_head = id % q_heads;
-        uint32_t b = a.s.cu ? a.s.batch : (uint32_t)row;
+        uint32_t b = (uint32_t)row;
         if (a.s.cu) {
-            for (uint32_t b0 = 0; b0 < a.s.batch && b == a.s.batch; b0 += 64) {
-                const uint32_t mine = b0 + hf_lane();
-                bool hit = false;
-                if (mine < a.s.batch) hit = row >= a.s.cu[mine] && row < a.s.cu[mine + 1];
-                const unsigned long long hits = __ballot(hit);
-                if (hits) b = b0 + __ffsll(hits) - 1;
-            }
-            if (b == a.s.batch) continue;
+            b = kv_last(a.s.batch, [&](const uint32_t i) { return (uint32_t)a.s.cu[i]; }, b);
+            if (row < a.s.cu[b] || row >= a.s.cu[b + 1]) continue;  // of no sequence
         }
         const hf_u32x4 plan = *(const hf_u32x4*)(a.plan + 4 * (int64_t)b);
         const uint32_t before = plan[0], tiles = plan[1], ranges = plan[2];
