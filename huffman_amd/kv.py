@@ -128,8 +128,8 @@ class KvCache(_Module):
         if ctx is None:
             stream = torch.cuda.current_stream(self._index)
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("the captured stream has no context yet: make one before the capture "
-                                   "(Context(stream=...)) or call once on that stream")
+                raise RuntimeError("the captured stream has no context yet: give the cache one made before the "
+                                   "capture (ctx=Context(stream=...)), or call once on that stream before it")
             ctx = api._default_ctx[key] = Context(self._index, stream)
         return ctx
 
