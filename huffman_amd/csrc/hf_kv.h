@@ -110,4 +110,11 @@ __host__ __device__ __forceinline__ hf_kv_seq hf_kv_sequence(const hf_kv_seqs& s
     }
     return q;
 }
+// Whether step i of a path, draft path[i] of a sequence's n rows to place i, can be taken: it is one of the
+// rows and behind the draft of the step before.  A step is looked at for itself alone: what the steps in
+// front of it hold may be anything.
+__host__ __device__ __forceinline__ bool hf_kv_path_ok(const int32_t* path, const int32_t i, const int32_t n) {
+    const int32_t j = path[i];
+    return j >= 0 && j < n && (i == 0 || path[i - 1] < j);
+}
 #endif

@@ -408,9 +408,9 @@ __global__ __launch_bounds__(kThreads) void hf_k_kv_keep(const hf_kv_pools c, co
     bool bad = q.bad || m < 0 || m > q.n || (uint32_t)m > path_width;
     if (!bad) {
         for (int32_t i = (int32_t)threadIdx.x; i < m; i += kThreads) {
-            const int32_t j = p[i], before = i ? p[i - 1] : -1;
-            bad |= j <= before || j >= q.n;
-            bad = bad || (uint32_t)table[(uint32_t)(q.past + j) >> c.page_shift] >= c.n_pages ||
+            // (the table is read for steps that can be taken only: both places are the sequence's own)
+            bad = bad || !hf_kv_path_ok(p, i, q.n) ||
+                  (uint32_t)table[(uint32_t)(q.past + p[i]) >> c.page_shift] >= c.n_pages ||
                   (uint32_t)table[(uint32_t)(q.past + i) >> c.page_shift] >= c.n_pages;
         }
     }

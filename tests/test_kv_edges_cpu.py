@@ -1,0 +1,50 @@
+"""CPU suite of the KV cache at its edges: what the kernels and the host mirror decide before they touch memory."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+
+
+def run_on_host(tmp_path, source):
+    """Builds a program over the kernels' header for the host and runs it."""
+    if not shutil.which(HIPCC):
+        pytest.skip("no hipcc")
+    src, exe = tmp_path / "edge.hip", tmp_path / "edge"
+    src.write_text(source)
+    subprocess.run([HIPCC, "--offload-arch=gfx950", "-O1", "-std=c++17", "-I", os.path.join(ROOT, "huffman_amd", "csrc"),
+                    str(src), "-o", str(exe)], check=True, capture_output=True, timeout=300)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert out.returncode == 0 and out.stdout.startswith("ok"), (out.returncode, out.stdout)
+
+
+PATH_TEST = r'''
+#include <cstdio>
+#include "hf_kv.h"
+// every path of three steps out of a few values
+int main() {
+    const int vals[] = {-2147483647 - 1, -2147483647, -5, -3, -2, -1, 0, 1, 2, 7, 8, 9, 2147483647};
+    long taken = 0;
+    for (int a : vals) for (int b : vals) for (int c : vals) for (int n : {0, 1, 3, 8, 2147418112}) {
+        const int path[3] = {a, b, c};
+        bool all = true;
+        for (int i = 0; i < 3; ++i) {
+            const bool ok = hf_kv_path_ok(path, i, n);
+            // a step that is taken names a row, whatever stands in front of it: its page is looked up
+            if (ok && (path[i] < 0 || path[i] >= n)) { printf("step %d of %d %d %d, %d rows\n", i, a, b, c, n); return 1; }
+            all = all && ok;
+        }
+        if (all != (0 <= a && a < b && b < c && c < n)) { printf("path %d %d %d, %d rows\n", a, b, c, n); return 2; }
+        taken += all;
+    }
+    printf("ok %ld\n", taken);
+}
+'''
+
+
+def test_steps_of_a_path_are_rows_whatever_stands_in_front(tmp_path):
+    """Paths that ascend below zero: every step is judged by itself before the table is read for it."""
+    run_on_host(tmp_path, PATH_TEST)
