@@ -128,6 +128,18 @@ __device__ __forceinline__ float kv_row_sum(float a) {
     return a + __shfl_xor(a, 32);
 }
 
+// Exponent of a weight, p = exp2(score x scale + nm).  Fused, the error of scale x maximum is the same factor
+// for the whole row; where it could pass 1 / 256 of a power of two (kv_huge, of a wavefront's rows), the
+// products are rounded first, as the maximum's was.  Whether a score calls for a new maximum is decided on
+// this very number: from 2^25 on the two forms differ by a power of two and more, and a weight that passed
+// as the one could leave fp16's range as the other.
+__device__ __forceinline__ float kv_exponent(const float score, const float scale, const float nm, const bool huge) {
+    return huge ? score * scale + nm : __builtin_fmaf(score, scale, nm);
+}
+__device__ __forceinline__ bool kv_huge(const float nm) {
+    return __ballot(fabsf(nm) > 65536.0f && nm != 3.402823466e38f) != 0;
+}
+
 // Has the values' loads waited for here: left to their first use, which is in a loop that issues
 // loads of its own, the wait there would be for those too, in every turn.
 template <int N>
@@ -644,7 +656,8 @@ struct kv_unit {
 #pragma unroll
         for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e / 4][e % 4]);
         // seldom after the first step: sums and outputs to a new maximum
-        if (__ballot(__builtin_fmaf(top, a.scale_log2, nm) > T::off + T::rise)) {
+        bool huge = kv_huge(nm);
+        if (__ballot(kv_exponent(top, a.scale_log2, nm, huge) > T::off + T::rise)) {
             const float was = nm;
             nm = fminf(was, T::off - kv_row_max(top) * a.scale_log2);
             const float f = __builtin_amdgcn_exp2f(nm - was);
@@ -652,18 +665,16 @@ struct kv_unit {
             div *= f;
 #pragma unroll
             for (int c = 0; c < VD; ++c) acc[c] *= f;
+            huge = kv_huge(nm);
         }
         hf_u32x4 p;
-        // (fused: the error of scale x maximum is the same factor for the whole row; where it could
-        // pass 1 / 256 of a power of two, the products are rounded first, as the maximum's was)
-        const bool huge = __ballot(fabsf(nm) > 65536.0f && nm != 3.402823466e38f) != 0;
         float e[8];
         if (huge) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = s[i / 4][i % 4] * a.scale_log2 + nm;
+            for (int i = 0; i < 8; ++i) e[i] = kv_exponent(s[i / 4][i % 4], a.scale_log2, nm, true);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = __builtin_fmaf(s[i / 4][i % 4], a.scale_log2, nm);
+            for (int i = 0; i < 8; ++i) e[i] = kv_exponent(s[i / 4][i % 4], a.scale_log2, nm, false);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {

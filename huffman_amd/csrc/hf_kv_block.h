@@ -129,7 +129,7 @@ void hf_k_kv_attend_block(const hf_kv_attend_args a) {
         for (int i = 0; i < 16; ++i) acc[q][i] = 0.0f;
     float nm = 3.402823466e38f, sum = 0.0f, div = 0.0f;  // p = exp2(scale_log2 s + nm)
     uint32_t bad = 0;
-    bool huge = false;  // |nm| where fused exponents would not do
+    bool huge = false;  // kv_huge of nm
 
     // The staging of a wavefront: K parts for the first half of the wavefronts, V for the others.  A
     // part's place is the lane's own (fixed) plus its page and its first token's place in the page.
@@ -308,7 +308,7 @@ void hf_k_kv_attend_block(const hf_kv_attend_args a) {
             float top = s[0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-            if (__ballot(__builtin_fmaf(top, a.scale_log2, nm) > T::off + T::rise)) {
+            if (__ballot(kv_exponent(top, a.scale_log2, nm, huge) > T::off + T::rise)) {
                 top = fmaxf(top, __shfl_xor(top, 32));
                 const float was = nm;
                 nm = fminf(was, T::off - top * a.scale_log2);
@@ -317,16 +317,14 @@ void hf_k_kv_attend_block(const hf_kv_attend_args a) {
                 div *= f;
 #pragma unroll
                 for (int q = 0; q < NB; ++q) acc[q] *= f;
-                huge = __ballot(fabsf(nm) > 65536.0f && nm != 3.402823466e38f) != 0;
+                huge = kv_huge(nm);
             }
-            // (fused: the error of scale x maximum is the same factor for the whole row; where it
-            // could pass 1 / 256 of a power of two, the products are rounded first, as the maximum's was)
             if (huge) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = s[i] * a.scale_log2 + nm;
+                for (int i = 0; i < 16; ++i) s[i] = kv_exponent(s[i], a.scale_log2, nm, true);
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], a.scale_log2, nm);
+                for (int i = 0; i < 16; ++i) s[i] = kv_exponent(s[i], a.scale_log2, nm, false);
             }
             hf_u32x4 p[2];
 #pragma unroll

@@ -9,6 +9,85 @@ from tests.test_gpu_kv import dev, kv, make  # noqa: F401  (kv: a fixture)
 pytestmark = pytest.mark.gpu
 
 
+# ---- scores ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,cache", [("fp16", "fp16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("n,per", [(1, 4), (16, 4), (32, 4), (64, 4)])  # tiles of 16, 64, 128, 256 rows
+@pytest.mark.parametrize("first,second", [(5, 37), (5, 69), (5, 133)])
+@pytest.mark.parametrize("key", [(16344, 2474, 6), (20432, 1862, 9), (65440, 1969, 15), (65504, 308, 16)])
+def test_scores_past_two_to_the_25(kv, dtype, cache, n, per, first, second, key):
+    """Two tokens with scores of 2.7e8 to 1.1e9, exact in 32 bits and 32 to 128 apart, the larger one later:
+    the weights' exponents are off by up to a step of such a score, but a weight stays finite.  Both tokens hold
+    the same values, so whatever their weights are the outputs are those values."""
+    batch, heads, dim, length, page = 64, 32, 64, 192, 64
+    dt = torch.float16 if dtype == "fp16" else torch.bfloat16
+    c = make(kv, cache, 3 + batch, page, heads, dim)
+    c.k.fill_(0)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    c.v.copy_(torch.randn(c.v.shape, generator=g, device="cuda"))
+    a, b, m = key
+    # (the drafts' own tokens are in a page of each sequence's own; keys of zeros: weights of zero)
+    for at, row in ((first, (a, b, 0)), (second, (a, b, m))):
+        c.k[at // page, at % page, :, :3] = torch.tensor(row, dtype=torch.float32, device="cuda").to(dt)
+    c.v[second // page, second % page] = c.v[first // page, first % page]
+    want = c.v[first // page, first % page].float()  # [heads, dim]
+    table = dev(np.concatenate([np.tile(np.arange(3), (batch, 1)), 3 + np.arange(batch)[:, None]], 1).astype(np.int32))
+    kv_len = dev(np.full(batch, length + n, np.int32))
+    cu = dev((np.arange(batch + 1) * n).astype(np.int32))
+    q = torch.zeros(batch * n, heads * per, dim, device="cuda", dtype=dt)
+    q[..., :3] = torch.tensor([16384.0, 64.0, 8.0], device="cuda").to(dt)
+    got, lse = c.attend(q, table, kv_len, cu, max_q=n, scale=128 ** -0.5, lse=True)
+    c.ctx.sync()
+    u = torch.finfo(dt).eps / 2
+    want = want.repeat_interleave(per, 0)
+    # sums of two products each in 32 bits (the other weights are zero) and a quotient, then the type's rounding
+    assert ((got.float() - want).abs() <= want.abs() * (u + 8 * 2.0 ** -24) * 1.01).all()
+    assert torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("n,per", [(1, 4), (16, 4), (32, 4), (64, 4)])
+@pytest.mark.parametrize("below", [14, 20, 22])
+def test_many_small_weights(kv, fmt, dtype, n, per, below):
+    """One token, and 60000 whose weights are 2^-below of its own: in fp16 they are near and below its smallest
+    normal number, and carry a part of the outputs that is seen."""
+    heads, dim, length, page = 1, 64, 60000, 64
+    dt = torch.float16 if dtype == "fp16" else torch.bfloat16
+    pages = -(-(length + n) // page)
+    c = make(kv, fmt, pages, page, heads, dim, 64)
+    c.k.fill_(0)
+    c.k_scale.fill_(127)
+    c.v_scale.fill_(127)
+    c.v.fill_(0x38 if fmt == "e4m3" else 0x22)  # ones
+    c.k[0, 7, 0, 0] = 0x38 if fmt == "e4m3" else 0x02  # 1.0 in the first element
+    c.v[0, 7] = 0x40 if fmt == "e4m3" else 0x44  # twos
+    q = torch.zeros(n, heads * per, dim, device="cuda", dtype=dt)
+    q[..., 0] = 1.0
+    scale = below * float(np.log(2.0))
+    got, lse = c.attend(q, dev(np.arange(pages, dtype=np.int32)[None]), dev(np.array([length + n], np.int32)),
+                        dev(np.array([0, n], np.int32)), max_q=n, scale=scale, lse=True)
+    c.ctx.sync()
+    seen = length + 1 + np.arange(n)  # tokens of each row
+    p = 2.0 ** -float(below)
+    small = (seen - 1) * p
+    want = torch.from_numpy((2.0 + small) / (1.0 + small))[:, None, None]
+    u = torch.finfo(dt).eps / 2
+    # the reference's bound with its terms for this case: weights rounded (u, twice), their exponents, sums of
+    # 60000 terms in 32 bits (twice), and what falls under fp16's range
+    rel = 2 * u + 2 * ((dim + 8) * 2.0 ** -24 * scale * 1.5 + 2.0 ** -20) + 2 * length * 2.0 ** -24 + length * 2.0 ** -31
+    # an error of a weight moves the quotient only as far as the values differ (by 1 of at most 2): the part of it
+    # that all weights share cancels
+    assert ((got.cpu().double() - want).abs() <= u * want + 1.01 * rel * want).all()
+    # (and closer: the small weights are all alike, so their sums are off by one relative error in all, at most a
+    # rounding of a weight and the sums': the outputs see that of the small part alone)
+    part = torch.from_numpy(small / (1.0 + small) ** 2)[:, None, None]
+    step = 2.0 ** -24 / 2.0 ** (7 - below) if dtype == "fp16" and below > 21 else 2 * u  # half a subnormal's step: 2^-25
+    near = u * want + part * (2 * step + 4 * u) + 2 * length * 2.0 ** -24 * 2
+    assert ((got.cpu().double() - want).abs() <= near).all()
+    ref = torch.from_numpy(scale + np.log1p(small))[:, None]
+    assert ((lse.cpu().double() - ref).abs() <= length * 2.0 ** -24 + 2.0 ** -19 + 2.0 ** -21 * ref).all()
+
+
 # ---- lists -----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("past", [0, 1, 20])
 @pytest.mark.parametrize("path", [[-2, -1], [-5, -3], [-1, 0], [-2 ** 31, -2 ** 31 + 1], [-3, 2], [0, 2 ** 31 - 1], [-2 ** 31, 3]])
