@@ -37,6 +37,22 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def _pool_strides(k: torch.Tensor) -> Tuple[int, int, int]:
+    """Page, token and head stride of a pool in bytes.  The stride of a dimension of one says nothing and is
+    replaced by a valid one; every other stays what it is, so that a pool whose rows lie on one another
+    (an expanded tensor) is refused by the call and not taken for a dense one."""
+    size = k.element_size()
+    page, token, head = (n * size for n in k.stride()[:3])
+    row = k.shape[3] * size
+    if k.shape[2] == 1:
+        head = row
+    if k.shape[1] == 1:
+        token = row
+    if k.shape[0] == 1:
+        page = max(token, head)
+    return page, token, head
+
+
 class KvCache(_Module):
     """Two page pools and their scales (include/huffhip.h has the layout and the arithmetic).
 
@@ -87,17 +103,9 @@ class KvCache(_Module):
         if ctx is not None and ctx.device != self._index:
             raise ValueError(f"the pools are on {k.device}, the context on cuda:{ctx.device}")
         self._need = {}  # scratch of hf_kv_attend by the sizes it depends on
-        size = k.element_size()
         self._c = L.hf_kv_cache(
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if group else 0,
-            v_scale.data_ptr() if group else 0, pages, k.stride(0) * size, k.stride(1) * size,
-            k.stride(2) * size, page_size, heads, dim, group, fmt, 0)
-        if pages < 2 or page_size < 2 or heads < 2:  # strides of a dimension of one say nothing
-            row = width * size
-            fix = self._c
-            fix.head_stride = max(fix.head_stride, row) if heads > 1 else row
-            fix.token_stride = max(fix.token_stride, row) if page_size > 1 else row
-            fix.page_stride = fix.page_stride if pages > 1 else max(fix.token_stride, fix.head_stride, row)
+            v_scale.data_ptr() if group else 0, pages, *_pool_strides(k), page_size, heads, dim, group, fmt, 0)
 
     @staticmethod
     def empty(pages: int, page_size: int, heads: int, head_dim: int, fmt: int = L.HF_KV_FP8_E4M3,

@@ -108,3 +108,23 @@ def test_paths_below_zero_are_reported_and_move_nothing(kv, hf, past, path):
     assert new_len.tolist() == [past + 4, past + 2]  # (the other sequence's path stays where it is)
     for t, was in zip((c.k, c.v, c.k_scale, c.v_scale), before):
         assert torch.equal(t, was)
+
+
+# ---- arguments -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shape,dim", [((1, 16, 8, 128), 1), ((1, 16, 8, 128), 2), ((4, 16, 1, 128), 0), ((4, 16, 1, 128), 1),
+                                       ((4, 16, 8, 128), 0), ((4, 16, 8, 128), 1), ((4, 16, 8, 128), 2)])
+def test_pools_whose_rows_lie_on_one_another_are_refused(kv, shape, dim):
+    """Expanded pools, also where another dimension is one and its stride is made up."""
+    from huffman_amd import HuffhipError
+    pages, page, heads, width = shape
+    pools = [torch.zeros(shape, dtype=torch.uint8, device="cuda").narrow(dim, 0, 1).expand(shape) for _ in range(2)]
+    scales = [torch.full((pages, heads, 1, page), 127, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    c = kv.KvCache(*pools, *scales)
+    t, l = dev(np.zeros((1, 1), np.int32)), dev(np.full(1, 16, np.int32))
+    x = torch.ones(1, heads, width, device="cuda", dtype=torch.bfloat16)
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for call in (lambda: c.write(x, x, t, l), lambda: c.read(t, l), lambda: c.attend(x, t, l),
+                 lambda: c.keep(t, l, None, zero[None], zero)):
+        with pytest.raises(HuffhipError):
+            call()
+    c.ctx.sync()

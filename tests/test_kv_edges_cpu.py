@@ -4,6 +4,7 @@ import shutil
 import subprocess
 
 import pytest
+import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -48,3 +49,22 @@ int main() {
 def test_steps_of_a_path_are_rows_whatever_stands_in_front(tmp_path):
     """Paths that ascend below zero: every step is judged by itself before the table is read for it."""
     run_on_host(tmp_path, PATH_TEST)
+
+
+@pytest.mark.parametrize("shape", [(1, 16, 8, 128), (4, 16, 1, 128), (1, 16, 1, 128), (4, 1, 8, 128), (4, 16, 8, 128)])
+@pytest.mark.parametrize("dtype,size", [(torch.uint8, 1), (torch.bfloat16, 2)])
+def test_strides_of_pools(shape, dtype, size):
+    """Dense pools have dense strides, whatever a dimension of one says; a stride of zero stays one."""
+    from huffman_amd.kv import _pool_strides
+    pages, tokens, heads, row = shape
+    k = torch.zeros(shape, dtype=dtype)
+    page, token, head = _pool_strides(k)
+    row *= size
+    assert (heads == 1 or head == row) and (tokens == 1 or token == heads * row) and (pages == 1 or page == tokens * heads * row)
+    assert min(page, token, head) >= row  # what the calls ask for
+    odd = k.as_strided(shape, [1 if n == 1 else s for n, s in zip(shape, k.stride())])
+    assert _pool_strides(odd) == (page, token, head)
+    for dim in range(3):
+        if shape[dim] > 1:  # expanded along a dimension: its stride is refused, not replaced
+            one = k.narrow(dim, 0, 1).expand(shape)
+            assert one.stride(dim) == 0 and _pool_strides(one)[dim] == 0
