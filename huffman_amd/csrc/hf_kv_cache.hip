@@ -62,6 +62,14 @@ __device__ __forceinline__ void find_places(const hf_kv_pools& c, const hf_kv_se
         for (uint32_t i = threadIdx.x; i <= s.batch; i += kThreads) cu_lds[i] = s.cu[i];
         __syncthreads();
     }
+    // The workgroup's other wavefronts look at every sequence of the call, a share each: offsets that fall
+    // hand a sequence's rows to one behind it, and a sequence without rows is met by no search.
+    if (s.cu && threadIdx.x >= (uint32_t)kMaxTokens) {
+        constexpr uint32_t lookers = kThreads - kMaxTokens;
+        for (uint64_t b = (uint64_t)blockIdx.x * lookers + threadIdx.x - kMaxTokens; b < s.batch;
+             b += (uint64_t)gridDim.x * lookers)
+            if (hf_kv_sequence(s, (uint32_t)b, c.page_shift).bad) atomicOr(err, HF_KERR_CORRUPT);
+    }
     if (threadIdx.x < n) {
         const int32_t row = (int32_t)(t0 + threadIdx.x);
         uint32_t b = (uint32_t)row;

@@ -110,6 +110,55 @@ def test_paths_below_zero_are_reported_and_move_nothing(kv, hf, past, path):
         assert torch.equal(t, was)
 
 
+@pytest.mark.parametrize("call", ["write", "read"])
+@pytest.mark.parametrize("batch", [3, 1500])
+@pytest.mark.parametrize("what", ["falls", "leaves", "negative length", "long length", "fewer tokens"])
+def test_every_list_that_does_not_fit_is_reported(kv, hf, call, batch, what):
+    """Offsets that fall although the sequence behind them is long enough for the rows it then claims, offsets
+    that leave the rows, and lengths of sequences without rows, which no row of the call leads to."""
+    from huffman_amd import HuffhipError
+    ctx = hf.Context()
+    page, width = 16, 8
+    c = make(kv, "e4m3", batch * width, page, 1, 64, 64, ctx=ctx)
+    table = np.arange(batch * width, dtype=np.int32).reshape(batch, width)
+    rows = 9
+    cu = np.full(batch + 1, rows, np.int32)
+    cu[:3] = [0, 6, 6]  # 6 rows, none, 3, none ...
+    kv_len = np.full(batch, 100, np.int32)
+    x = torch.ones(rows, 1, 64, device="cuda", dtype=torch.bfloat16)
+    out = (x.clone(), x.clone())
+    torch.cuda.synchronize()
+
+    def run(kv_len, cu):
+        if call == "write":
+            c.write(x, x, dev(table), dev(kv_len), dev(cu))
+        else:
+            c.read(dev(table), dev(kv_len), dev(cu), out=out)
+        torch.cuda.synchronize()
+
+    run(kv_len, cu)
+    ctx.sync()  # as it should be: nothing to report
+    bad_len, bad_cu = kv_len.copy(), cu.copy()
+    if what == "falls":
+        bad_cu[2] = 3
+    elif what == "leaves":
+        bad_cu[3:] = rows + 4
+        bad_cu[2] = rows  # (the third sequence's rows all lie behind the tensors)
+    elif what == "negative length":
+        bad_len[1] = -1
+    elif what == "long length":
+        bad_len[1] = page * width + 1
+    else:
+        bad_cu[1:] = rows
+        bad_cu[0] = rows - 1
+        bad_len[0] = 0
+    run(bad_len, bad_cu)
+    with pytest.raises(HuffhipError):
+        ctx.sync()
+    run(kv_len, cu)
+    ctx.sync()
+
+
 # ---- arguments -------------------------------------------------------------------------------------
 @pytest.mark.parametrize("shape,dim", [((1, 16, 8, 128), 1), ((1, 16, 8, 128), 2), ((4, 16, 1, 128), 0), ((4, 16, 1, 128), 1),
                                        ((4, 16, 8, 128), 0), ((4, 16, 8, 128), 1), ((4, 16, 8, 128), 2)])
