@@ -1591,6 +1591,17 @@ int kv_check_rows(const void* p, int64_t row_stride, int64_t head_stride, int el
     return HF_OK;
 }
 
+// Whether `count` entries at p touch any of `rows` rows of `width` entries that lie `stride` apart.
+bool kv_touches(const int32_t* p, uint64_t count, const int32_t* row0, uint64_t rows, uint64_t width, uint64_t stride) {
+    if (!count || !rows || !width || !row0) return false;
+    const uintptr_t lo = (uintptr_t)p, hi = lo + 4 * count, base = (uintptr_t)row0;
+    if (hi <= base) return false;
+    // the first row that ends behind lo
+    uint64_t r = 0;
+    if (lo >= base + 4 * width) r = stride ? (lo - base - 4 * width) / (4 * stride) + 1 : rows;
+    return r < rows && base + 4 * r * stride < hi;
+}
+
 int kv_move(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch, const void* d_k,
             const void* d_v, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, int dtype,
             bool write) {
@@ -1752,8 +1763,14 @@ int hf_kv_keep(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
     hf_kv_seqs s;
     if (int rc = kv_check_cache(cache, &p)) return rc;
     if (int rc = kv_check_batch(batch, &s)) return rc;
-    if (s.batch && (!d_path_len || !d_new_len || d_new_len == s.kv_len)) return HF_ERR_ARG;
+    if (s.batch && (!d_path_len || !d_new_len)) return HF_ERR_ARG;
     if (s.batch && ((path_width && !d_path) || path_stride < path_width)) return HF_ERR_ARG;
+    // (the workgroups of a sequence's heads read its lists, and some have not when the first writes)
+    if (kv_touches(d_new_len, s.batch, s.kv_len, 1, s.batch, 0) || kv_touches(d_new_len, s.batch, d_path_len, 1, s.batch, 0) ||
+        kv_touches(d_new_len, s.batch, s.cu, 1, (uint64_t)s.batch + 1, 0) ||
+        kv_touches(d_new_len, s.batch, d_path, s.batch, path_width, (uint64_t)path_stride) ||
+        kv_touches(d_new_len, s.batch, s.table, s.batch, s.width, s.table_stride))
+        return HF_ERR_ARG;
     if (path_stride > (1ll << 31)) return HF_ERR_RANGE;
     if (!ctx) return HF_ERR_ARG;
     if (s.batch == 0) return HF_OK;

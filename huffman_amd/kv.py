@@ -281,7 +281,8 @@ class KvCache(_Module):
              new_len: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``hf_kv_keep``: of the sequences' last rows (drafts), keep those that ``path`` int32
         [batch, width] names in ascending order, ``path_len`` int32 [batch] of them; returns the
-        sequences' new lengths.  ``rows``: rows that ``cu`` covers (default: any number)."""
+        sequences' new lengths (``new_len``: no part of the call's other lists).  ``rows``: rows that
+        ``cu`` covers (default: any number)."""
         batch = table.shape[0]
         if self._ints("path", path, 2)[0] != batch or self._ints("path_len", path_len, 1)[0] != batch:
             raise ValueError("path and path_len: one row for each sequence")

@@ -680,9 +680,9 @@ int hf_kv_attend(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch
                  const hf_kv_query* query, void* d_work, uint64_t work_bytes);
 /* After a tree of drafts is judged: rows d_path[b][0 .. d_path_len[b] - 1] (ascending numbers of
  * the sequence's last rows) move, codes and scales, to the first places behind the tokens in front
- * of the drafts, and d_new_len[b] (not d_kv_len itself) = those tokens + d_path_len[b].  A path that
- * does not ascend or leaves the sequence's rows is reported as HF_ERR_CORRUPT, moves nothing and
- * gives d_new_len = d_kv_len. */
+ * of the drafts, and d_new_len[b] = those tokens + d_path_len[b] (memory of its own: HF_ERR_ARG where
+ * it touches one of the call's lists).  A path that does not ascend or leaves the sequence's rows is
+ * reported as HF_ERR_CORRUPT, moves nothing and gives d_new_len = d_kv_len. */
 int hf_kv_keep(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
                const int32_t* d_path, int64_t path_stride, uint32_t path_width,
                const int32_t* d_path_len, int32_t* d_new_len);

@@ -177,3 +177,29 @@ def test_pools_whose_rows_lie_on_one_another_are_refused(kv, shape, dim):
         with pytest.raises(HuffhipError):
             call()
     c.ctx.sync()
+
+
+def test_new_lengths_in_memory_that_the_call_reads_are_refused(kv):
+    """Every list of the call, whole or in part, may be in use when the first length is written; what lies
+    between the rows of a wider table or path is not."""
+    from huffman_amd import HuffhipError
+    c = make(kv, "e4m3", 4, 16, 2, 64, 32)
+    buf = torch.zeros(64, dtype=torch.int32, device="cuda")
+    cu, length, kept = buf[0:3], buf[3:5], buf[5:7]
+    wide_path, wide_table = buf[16:32].view(2, 8), buf[32:48].view(2, 8)
+    path, table = wide_path[:, :3], wide_table[:, :2]
+    cu.copy_(dev(np.array([0, 3, 6], np.int32)))
+    length.copy_(dev(np.array([9, 20], np.int32)))
+    kept.copy_(dev(np.array([2, 1], np.int32)))
+    path.copy_(dev(np.array([[0, 2, 9], [1, 0, 0]], np.int32)))
+    table.copy_(dev(np.array([[0, 1], [2, 3]], np.int32)))
+    torch.cuda.synchronize()
+    before = buf.clone()
+    for lo in (0, 1, 2, 3, 4, 5, 6, 15, 16, 17, 18, 23, 24, 26, 31, 32, 33, 39, 40, 41):
+        with pytest.raises(HuffhipError):
+            c.keep(table, length, cu, path, kept, new_len=buf[lo:lo + 2])
+    c.ctx.sync()
+    assert torch.equal(buf, before)
+    for lo in (7, 14, 19, 22, 27, 29, 34, 38, 42, 48):
+        assert c.keep(table, length, cu, path, kept, new_len=buf[lo:lo + 2]).tolist() == [8, 18]
+    c.ctx.sync()
