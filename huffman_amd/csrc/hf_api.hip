@@ -1723,7 +1723,8 @@ int hf_kv_attend(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch
     if (int rc = kv_check_attend(cache, batch, query->q_heads, &a.c, &a.s, &a.per)) return rc;
     if (query->dtype > HF_DT_FP16) return HF_ERR_ARG;
     if (cache->format <= HF_KV_FP16 && query->dtype != cache->format) return HF_ERR_ARG;
-    if (!(query->scale > 0.0f) || query->scale > 3.0e38f) return HF_ERR_ARG;
+    a.scale_log2 = query->scale * 1.4426950408889634f;
+    if (!(query->scale > 0.0f) || !(a.scale_log2 <= 3.402823466e38f)) return HF_ERR_ARG;
     if (a.s.rows == 0 || a.s.batch == 0) return ctx ? HF_OK : HF_ERR_ARG;
     if (query->d_mask && (uint64_t)query->mask_words * 32u < a.s.most) return HF_ERR_ARG;
     if (int rc = kv_check_rows(query->d_q, query->q_row_stride, query->q_head_stride, 2, &a.q)) return rc;
@@ -1738,7 +1739,6 @@ int hf_kv_attend(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch
     a.lse = query->d_lse;
     a.mask = query->d_mask;
     a.mask_words = query->mask_words;
-    a.scale_log2 = query->scale * 1.4426950408889634f;
     a.part = (float*)d_work;
     a.part_ml = a.part + plan.part_floats;
     a.plan = (uint32_t*)(a.part_ml + plan.ml_floats);

@@ -672,7 +672,7 @@ typedef struct hf_kv_query {
     uint32_t q_heads; /* a multiple of heads */
     uint32_t mask_words;
     uint32_t dtype;
-    float scale; /* finite, above 0 */
+    float scale; /* above 0, its product with log2(e) finite (2.35e38) */
 } hf_kv_query;
 uint64_t hf_kv_attend_work_bytes(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
                                  uint32_t q_heads);

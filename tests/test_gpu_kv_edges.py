@@ -203,3 +203,18 @@ def test_new_lengths_in_memory_that_the_call_reads_are_refused(kv):
     for lo in (7, 14, 19, 22, 27, 29, 34, 38, 42, 48):
         assert c.keep(table, length, cu, path, kept, new_len=buf[lo:lo + 2]).tolist() == [8, 18]
     c.ctx.sync()
+
+
+def test_a_scale_whose_logarithmic_form_overflows_is_refused(kv):
+    from huffman_amd import HuffhipError
+    c = make(kv, "e4m3", 4, 16, 2, 64, 32)
+    c.k.fill_(0)
+    c.v.fill_(0x38)
+    t, l = dev(np.zeros((1, 1), np.int32)), dev(np.ones(1, np.int32))
+    q = torch.zeros(1, 4, 64, device="cuda", dtype=torch.bfloat16)
+    for scale in (2.4e38, 3.0e38, 3.4e38):
+        with pytest.raises(HuffhipError):
+            c.attend(q, t, l, scale=scale)
+    for scale in (2.3e38, 1e-38, 1e-44):  # scores of zero: ones
+        assert (c.attend(q, t, l, scale=scale) == 1).all()
+    c.ctx.sync()
