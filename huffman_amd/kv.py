@@ -254,10 +254,9 @@ class KvCache(_Module):
         # captured graph, has its own.
         sizes = (table.shape, rows, max_q, cu is None, heads)
         need = self._need.get(sizes)
-        if need is None:
-            need = self._need[sizes] = L.lib().hf_kv_attend_work_bytes(handle, cache, b, heads)
-            if len(self._need) > 1000:
-                self._need = {sizes: need}
+        known = need is not None
+        if not known:
+            need = L.lib().hf_kv_attend_work_bytes(handle, cache, b, heads)
         wanted = [((need,), torch.uint8)]
         if lse:
             wanted.append(((rows, heads), torch.float32))
@@ -274,6 +273,10 @@ class KvCache(_Module):
                             _DTYPES[q.dtype], self.head_dim ** -0.5 if scale is None else scale)
         check(L.lib().hf_kv_attend(handle, cache, b, query, work.data_ptr() if need else None, need),
               "hf_kv_attend")
+        if not known:  # (of a call that was taken: what hf_kv_attend refuses needs no scratch)
+            if len(self._need) >= 1000:
+                self._need = {}
+            self._need[sizes] = need
         return (out, sums) if lse else out
 
     def keep(self, table: torch.Tensor, kv_len: torch.Tensor, cu: Optional[torch.Tensor],

@@ -218,3 +218,17 @@ def test_a_scale_whose_logarithmic_form_overflows_is_refused(kv):
     for scale in (2.3e38, 1e-38, 1e-44):  # scores of zero: ones
         assert (c.attend(q, t, l, scale=scale) == 1).all()
     c.ctx.sync()
+
+
+def test_a_refused_call_leaves_the_next_one_alone(kv):
+    """A table whose rows lie on one another is refused; the same shape in a table of its own is not."""
+    from huffman_amd import HuffhipError
+    c = make(kv, "e4m3", 64, 16, 2, 64, 32)
+    c.k.fill_(0)
+    c.v.fill_(0x38)
+    row, l = dev(np.arange(32, dtype=np.int32)[None]), dev(np.full(2, 500, np.int32))
+    q = torch.zeros(2, 4, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(HuffhipError):
+        c.attend(q, row.expand(2, 32), l)
+    assert (c.attend(q, row.repeat(2, 1), l) == 1).all()
+    c.ctx.sync()
