@@ -152,10 +152,12 @@ class KvCache(_Module):
             return [torch.empty(shape, dtype=dtype, device=self._device) for shape, dtype in tensors]
 
     def _ints(self, name: str, t: torch.Tensor, dim: int) -> torch.Size:
-        if t.dtype != torch.int32 or t.dim() != dim or t.get_device() != self._index or \
-                (t.numel() and t.stride(-1) != 1):
+        shape = t.shape
+        # (one entry may have any stride: a column of a wider list, for one sequence)
+        if t.dtype != torch.int32 or len(shape) != dim or t.get_device() != self._index or \
+                (shape[-1] > 1 and t.stride(-1) != 1):
             raise ValueError(f"{name}: int32, {dim} dimension(s), contiguous rows, on the pools' device")
-        return t.shape
+        return shape
 
     def _batch(self, table, kv_len, cu, rows: int, max_rows: int) -> bytes:
         batch, width = self._ints("table", table, 2)

@@ -232,3 +232,17 @@ def test_a_refused_call_leaves_the_next_one_alone(kv):
         c.attend(q, row.expand(2, 32), l)
     assert (c.attend(q, row.repeat(2, 1), l) == 1).all()
     c.ctx.sync()
+
+
+def test_lists_of_one_entry_may_have_any_stride(kv):
+    c = make(kv, "e4m3", 4, 16, 2, 64, 32)
+    x = torch.ones(1, 2, 64, device="cuda", dtype=torch.bfloat16)
+    state = dev(np.array([[5, 2, 1, 0]], np.int32))  # one sequence's length, page, accepted drafts and path
+    length, page, kept, path = state[:, 0], state[:, 1:2], state[:, 2], state[:, 3:4]
+    assert length.stride() == (4,)
+    c.write(x, x, page, length)
+    assert (c.read(page, length)[0] == 1).all()
+    assert (c.attend(x.repeat(1, 2, 1), page, length).shape == (1, 4, 64))
+    assert c.keep(page, length, None, path, kept).tolist() == [5]
+    assert c.keep(page.t(), length, None, path.t(), kept).tolist() == [5]
+    c.ctx.sync()
