@@ -69,6 +69,8 @@ class KvCache(_Module):
     of a sequence, the call's rows included) and ``cu`` int32 [batch + 1], the first row of each
     sequence; None: one row each.  They are read on the device, on the context's stream; what they
     say wrongly is reported by ``Context.sync``.  No call synchronises or copies to the host.
+    The cache is for inference: rows, queries and outputs that need a gradient are refused while
+    gradients are recorded.
     """
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
@@ -183,6 +185,9 @@ class KvCache(_Module):
             raise ValueError(f"{name}: [rows, {heads}, {self.head_dim}] on the pools' device")
         if t.dtype not in _DTYPES:
             raise TypeError(f"{name}: bf16, fp16 or fp32, not {t.dtype}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} needs a gradient, and no call here records one: detach it, or call under "
+                               "torch.no_grad()")
         row, head, one = t.stride()
         if one != 1 and t.numel():
             raise ValueError(f"{name}: the last dimension is contiguous")

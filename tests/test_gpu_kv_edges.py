@@ -246,3 +246,22 @@ def test_lists_of_one_entry_may_have_any_stride(kv):
     assert c.keep(page, length, None, path, kept).tolist() == [5]
     assert c.keep(page.t(), length, None, path.t(), kept).tolist() == [5]
     c.ctx.sync()
+
+
+def test_tensors_that_need_gradients_are_refused(kv):
+    """No call records what a backward pass needs."""
+    c = make(kv, "e4m3", 4, 16, 2, 64, 32)
+    t, l = dev(np.zeros((1, 1), np.int32)), dev(np.ones(1, np.int32))
+    x = torch.ones(1, 2, 64, device="cuda", dtype=torch.bfloat16)
+    q = torch.ones(1, 4, 64, device="cuda", dtype=torch.bfloat16)
+    need = lambda a: a.clone().requires_grad_()  # noqa: E731
+    for call in (lambda: c.write(need(x), x, t, l), lambda: c.write(x, need(x), t, l), lambda: c.attend(need(q), t, l),
+                 lambda: c.attend(need(q) * 1, t, l), lambda: c.attend(q, t, l, out=need(q)),
+                 lambda: c.read(t, l, out=(x.clone(), need(x)))):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with torch.inference_mode():
+        c.attend(need(q), t, l)
+    c.ctx.sync()
