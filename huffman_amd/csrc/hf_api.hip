@@ -1621,8 +1621,8 @@ int kv_move(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch, con
         if (int rc = kv_check_rows(d_v, v_row, v_head, elem, &v)) return rc;
     }
     // (rows that are written must not lie on one another)
-    const int64_t row = p.head_dim;
-    if (!write && ((p.heads > 1 && (k_head < row || v_head < row)) || (s.rows > 1 && (k_row < row || v_row < row))))
+    if (!write && !none && (hf_kv_rows_touch(s.rows, p.heads, k.row_stride, k.head_stride, p.head_dim) ||
+                            hf_kv_rows_touch(s.rows, p.heads, v.row_stride, v.head_stride, p.head_dim)))
         return HF_ERR_ARG;
     if (!ctx) return HF_ERR_ARG;
     if (none) return HF_OK;
@@ -1729,9 +1729,7 @@ int hf_kv_attend(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch
     if (query->d_mask && (uint64_t)query->mask_words * 32u < a.s.most) return HF_ERR_ARG;
     if (int rc = kv_check_rows(query->d_q, query->q_row_stride, query->q_head_stride, 2, &a.q)) return rc;
     if (int rc = kv_check_rows(query->d_out, query->out_row_stride, query->out_head_stride, 2, &a.out)) return rc;
-    const int64_t row = a.c.head_dim;
-    if ((query->q_heads > 1 && query->out_head_stride < row) || (a.s.rows > 1 && query->out_row_stride < row))
-        return HF_ERR_ARG;
+    if (hf_kv_rows_touch(a.s.rows, query->q_heads, a.out.row_stride, a.out.head_stride, a.c.head_dim)) return HF_ERR_ARG;
     if (!ctx) return HF_ERR_ARG;
     if (int rc = kv_plan_of(ctx, a.c, a.s, a.per, &plan)) return rc;
     if (plan.bytes > work_bytes || (plan.bytes && !d_work)) return HF_ERR_ARG;

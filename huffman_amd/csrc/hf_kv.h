@@ -40,6 +40,23 @@ struct hf_kv_rows {
     uint32_t head_stride;
 };
 
+// Whether rows of `dim` elements, at i row_stride + j head_stride for i < rows and j < heads, lie on one
+// another.  Beside the two nested orders any layout is fine whose rows stay apart: for every distance in
+// heads the rows nearest to it are looked at.
+inline bool hf_kv_rows_touch(const uint64_t rows, const uint64_t heads, const uint64_t row_stride,
+                             const uint64_t head_stride, const uint64_t dim) {
+    if (rows == 0 || heads == 0) return false;
+    if ((rows > 1 && row_stride < dim) || (heads > 1 && head_stride < dim)) return true;
+    if (rows == 1 || heads == 1) return false;
+    if (row_stride >= (heads - 1) * head_stride + dim || head_stride >= (rows - 1) * row_stride + dim) return false;
+    for (uint64_t j = 1; j < heads; ++j) {
+        const uint64_t at = j * head_stride, i = at / row_stride;
+        if (i < rows && at - i * row_stride < dim) return true;
+        if (i + 1 < rows && (i + 1) * row_stride - at < dim) return true;
+    }
+    return false;
+}
+
 struct hf_kv_attend_args {
     hf_kv_pools c;
     hf_kv_seqs s;

@@ -265,3 +265,29 @@ def test_tensors_that_need_gradients_are_refused(kv):
     with torch.inference_mode():
         c.attend(need(q), t, l)
     c.ctx.sync()
+
+
+def test_outputs_that_lie_on_one_another_are_refused(kv):
+    """Heads of a row on the rows behind it; layouts whose rows stay apart in any order are taken."""
+    from huffman_amd import HuffhipError
+    c = make(kv, "e4m3", 4, 16, 3, 64, 32)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for pool in (c.k, c.v):
+        pool.copy_(torch.randint(0, 0x70, pool.shape, generator=g, device="cuda", dtype=torch.uint8))
+    t, l, cu = dev(np.array([[2, 1]], np.int32)), dev(np.full(1, 20, np.int32)), dev(np.array([0, 2], np.int32))
+    q = torch.randn(2, 3, 64, generator=g, device="cuda").bfloat16()
+    want, rows = c.attend(q, t, l, cu, max_q=2), c.read(t, l, cu, rows=2)
+    flat = lambda: torch.zeros(2048, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    for strides in ((64, 64), (128, 64), (96, 64), (192, 96)):
+        out = flat().as_strided((2, 3, 64), strides + (1,))
+        good = flat()[:384].view(2, 3, 64)
+        for call in (lambda: c.attend(q, t, l, cu, max_q=2, out=out), lambda: c.read(t, l, cu, out=(out, good)),
+                     lambda: c.read(t, l, cu, out=(good, out))):
+            with pytest.raises(HuffhipError):
+                call()
+    for strides in ((192, 64), (64, 192), (64, 128), (200, 64), (192, 128), (1024, 72)):
+        out, other = (flat().as_strided((2, 3, 64), strides + (1,)) for _ in range(2))
+        assert torch.equal(c.attend(q, t, l, cu, max_q=2, out=out), want)
+        got = c.read(t, l, cu, out=(out, other))
+        assert torch.equal(got[0], rows[0]) and torch.equal(got[1], rows[1])
+    c.ctx.sync()

@@ -68,3 +68,31 @@ def test_strides_of_pools(shape, dtype, size):
         if shape[dim] > 1:  # expanded along a dimension: its stride is refused, not replaced
             one = k.narrow(dim, 0, 1).expand(shape)
             assert one.stride(dim) == 0 and _pool_strides(one)[dim] == 0
+
+
+ROWS_TEST = r'''
+#include <cstdio>
+#include <vector>
+#include "hf_kv.h"
+// strides from 0 to 40 of rows of 1, 3 and 4 elements, against every element counted
+int main() {
+    long touch = 0, apart = 0;
+    for (int rows = 0; rows < 6; ++rows) for (int heads = 0; heads < 6; ++heads) for (int dim : {1, 3, 4})
+        for (int rs = 0; rs <= 40; ++rs) for (int hs = 0; hs <= 40; ++hs) {
+            std::vector<char> hit(6 * 40 * 2 + 8);
+            bool want = false;
+            for (int i = 0; i < rows; ++i) for (int j = 0; j < heads; ++j) for (int d = 0; d < dim; ++d)
+                want = hit[i * rs + j * hs + d]++ || want;
+            if (hf_kv_rows_touch(rows, heads, rs, hs, dim) != want) {
+                printf("rows %d heads %d strides %d %d dim %d\n", rows, heads, rs, hs, dim);
+                return 1;
+            }
+            ++(want ? touch : apart);
+        }
+    printf("ok %ld %ld\n", touch, apart);
+}
+'''
+
+
+def test_rows_that_lie_on_one_another(tmp_path):
+    run_on_host(tmp_path, ROWS_TEST)
