@@ -69,6 +69,8 @@ class KvCache(_Module):
     of a sequence, the call's rows included) and ``cu`` int32 [batch + 1], the first row of each
     sequence; None: one row each.  They are read on the device, on the context's stream; what they
     say wrongly is reported by ``Context.sync``.  No call synchronises or copies to the host.
+    With ``ctx`` they run on its stream, whatever the current one is: the tensors of a call are to be
+    ready there, and its results are.
     The cache is for inference: rows, queries and outputs that need a gradient are refused while
     gradients are recorded.
     """
@@ -104,6 +106,7 @@ class KvCache(_Module):
         self._device, self._index = k.device, k.device.index
         if ctx is not None and ctx.device != self._index:
             raise ValueError(f"the pools are on {k.device}, the context on cuda:{ctx.device}")
+        self._hold(k, v, k_scale, v_scale)
         self._need = {}  # scratch of hf_kv_attend by the sizes it depends on
         self._c = L.hf_kv_cache(
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if group else 0,
@@ -152,6 +155,14 @@ class KvCache(_Module):
             return [torch.empty(shape, dtype=dtype, device=self._device) for shape, dtype in tensors]
         with torch.cuda.stream(self._ctx.stream):
             return [torch.empty(shape, dtype=dtype, device=self._device) for shape, dtype in tensors]
+
+    def _hold(self, *tensors) -> None:
+        """Tensors of a call that ran on another stream than the current one: dropped by the caller, their
+        memory is not handed out again before the call is through with it."""
+        if self._ctx is not None and _raw_stream(self._index) != self._ctx.stream.cuda_stream:
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(self._ctx.stream)
 
     def _ints(self, name: str, t: torch.Tensor, dim: int) -> torch.Size:
         shape = t.shape
@@ -208,6 +219,7 @@ class KvCache(_Module):
         b = self._batch(table, kv_len, cu, k.shape[0], 0)
         check(L.lib().hf_kv_write(self._handle(), C.addressof(self._c), b, pk, pv, kr, kh, vr, vh,
                                   _DTYPES[k.dtype]), "hf_kv_write")
+        self._hold(k, v, table, kv_len, cu)
 
     def read(self, table: torch.Tensor, kv_len: torch.Tensor, cu: Optional[torch.Tensor] = None,
              rows: Optional[int] = None, dtype: torch.dtype = torch.bfloat16,
@@ -230,6 +242,7 @@ class KvCache(_Module):
         b = self._batch(table, kv_len, cu, k.shape[0], 0)
         check(L.lib().hf_kv_read(self._handle(), C.addressof(self._c), b, pk, pv, kr, kh, vr, vh,
                                  _DTYPES[k.dtype]), "hf_kv_read")
+        self._hold(k, v, table, kv_len, cu)
         return k, v
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor,
@@ -280,6 +293,7 @@ class KvCache(_Module):
                             _DTYPES[q.dtype], self.head_dim ** -0.5 if scale is None else scale)
         check(L.lib().hf_kv_attend(handle, cache, b, query, work.data_ptr() if need else None, need),
               "hf_kv_attend")
+        self._hold(q, table, kv_len, cu, mask, out)
         if not known:  # (of a call that was taken: what hf_kv_attend refuses needs no scratch)
             if len(self._need) >= 1000:
                 self._need = {}
@@ -304,4 +318,5 @@ class KvCache(_Module):
         check(L.lib().hf_kv_keep(self._handle(), C.addressof(self._c), b, path.data_ptr(),
                                  path.stride(0) if batch > 1 else path.shape[1], path.shape[1],
                                  path_len.data_ptr(), new_len.data_ptr()), "hf_kv_keep")
+        self._hold(table, kv_len, cu, path, path_len, new_len)
         return new_len

@@ -291,3 +291,52 @@ def test_outputs_that_lie_on_one_another_are_refused(kv):
         got = c.read(t, l, cu, out=(out, other))
         assert torch.equal(got[0], rows[0]) and torch.equal(got[1], rows[1])
     c.ctx.sync()
+
+
+# ---- streams ---------------------------------------------------------------------------------------
+def test_tensors_dropped_before_another_stream_has_used_them(kv, hf):
+    """Every tensor of a call on a context's own stream, which is busy, is dropped right after the call and
+    its memory asked for again: the call works on what it was given."""
+    side = torch.cuda.Stream()
+    ctx = hf.Context(stream=side)
+    heads, dim, n = 4, 128, 512
+    c = make(kv, "bf16", 64, 16, heads, dim, ctx=ctx)
+    a = torch.randn(4096, 4096, device="cuda")
+    k, v = (torch.randn(n, heads, dim, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(n, heads, dim, device="cuda").bfloat16()
+    lists = [np.arange(32, dtype=np.int32)[None], np.array([n], np.int32), np.array([0, n], np.int32)]
+    steps = [np.arange(0, n, 2, dtype=np.int32)[None], np.array([n // 2], np.int32)]
+
+    def spoil(sizes):
+        return [torch.full((s,), 0x55, dtype=torch.uint8, device="cuda") for s in sizes for _ in range(3)]
+
+    def run(early):
+        got = []
+        for i in range(4):
+            given = [t.clone() for t in ([k, v] if i == 0 else [q] if i == 2 else [])]
+            given += [dev(x) for x in lists + (steps if i == 3 else [])]
+            torch.cuda.synchronize()
+            if early:
+                with torch.cuda.stream(side):
+                    for _ in range(8):
+                        torch.mm(a, a)
+            if i == 0:
+                c.write(*given)
+            elif i == 1:
+                got += c.read(*given, rows=n)
+            elif i == 2:
+                got += c.attend(*given, max_q=n, lse=True)
+            else:
+                got.append(c.keep(*given))
+            sizes = [t.numel() * t.element_size() for t in given]
+            if early:
+                del given
+                spoil(sizes)
+            torch.cuda.synchronize()
+        return got + [c.k.clone(), c.v.clone()]
+
+    want = run(False)
+    got = run(True)
+    ctx.sync()
+    for x, y in zip(want, got):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
