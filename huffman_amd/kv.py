@@ -140,7 +140,9 @@ class KvCache(_Module):
         ctx = api._default_ctx.get(key)
         if ctx is None:
             stream = torch.cuda.current_stream(self._index)
-            if torch.cuda.is_current_stream_capturing():
+            with torch.cuda.device(self._index):  # (the question is asked of the current device's stream)
+                capturing = torch.cuda.is_current_stream_capturing()
+            if capturing:
                 raise RuntimeError("the captured stream has no context yet: give the cache one made before the "
                                    "capture (ctx=Context(stream=...)), or call once on that stream before it")
             ctx = api._default_ctx[key] = Context(self._index, stream)

@@ -1,4 +1,5 @@
 """CPU suite of the KV cache at its edges: what the kernels and the host mirror decide before they touch memory."""
+import contextlib
 import os
 import shutil
 import subprocess
@@ -96,3 +97,33 @@ int main() {
 
 def test_rows_that_lie_on_one_another(tmp_path):
     run_on_host(tmp_path, ROWS_TEST)
+
+
+@pytest.mark.parametrize("captured", [0, 1])
+def test_the_pools_device_is_asked_for_a_capture(monkeypatch, captured):
+    """Pools on the second device, the first one current: a stream without a context is refused if the pools'
+    device records a capture on it, and only then."""
+    from huffman_amd import api, kv
+    now = [0]
+
+    @contextlib.contextmanager
+    def device(index):
+        was, now[0] = now[0], index
+        yield
+        now[0] = was
+
+    monkeypatch.setattr(api, "_default_ctx", {})
+    monkeypatch.setattr(kv, "_raw_stream", lambda index: 77)
+    monkeypatch.setattr(kv, "Context", lambda index, stream: ("context", index, stream))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index: ("stream", index))
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] == captured)
+    c = kv.KvCache.__new__(kv.KvCache)
+    c._ctx, c._index = None, 1
+    if captured == 1:
+        with pytest.raises(RuntimeError, match="capture"):
+            c.ctx
+        assert api._default_ctx == {}
+    else:
+        assert c.ctx == ("context", 1, ("stream", 1)) and list(api._default_ctx) == [(1, 77)]
+    assert now == [0]
