@@ -43,8 +43,8 @@ template <int QT>
 struct kv_type;
 template <>
 struct kv_type<HF_DT_BF16> {
-    // bit patterns: exponent field of both halves, its lowest bit, infinity, one
-    static constexpr uint32_t expo = 0x7F807F80u, unit = 0x00800080u, inf = 0x7F80u, one = 0x3F80u;
+    // bit patterns: exponent field of both halves, its lowest bit, one
+    static constexpr uint32_t expo = 0x7F807F80u, unit = 0x00800080u, one = 0x3F80u;
     static constexpr float off = 0.0f, rise = 8.0f;
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
@@ -56,7 +56,7 @@ struct kv_type<HF_DT_BF16> {
 };
 template <>
 struct kv_type<HF_DT_FP16> {
-    static constexpr uint32_t expo = 0x7C007C00u, unit = 0x04000400u, inf = 0x7C00u, one = 0x3C00u;
+    static constexpr uint32_t expo = 0x7C007C00u, unit = 0x04000400u, one = 0x3C00u;
     // p is held 2^7 up and may rise by 2^8 more, to 2^15: a p that fp16 flushes is below 2^-31 of
     // the largest, so even a long row of such tokens beside one large one keeps its weight
     static constexpr float off = 7.0f, rise = 8.0f;
@@ -107,10 +107,6 @@ struct kv_raw {
                 for (int j = 0; j < 4; ++j) w[4 * i + j] = a[j];
             }
         }
-    }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < (BYTES >= 4 ? BYTES / 4 : 1); ++i) w[i] = 0;
     }
 };
 
@@ -361,7 +357,6 @@ struct kv_unit {
     uint32_t head;
     hf_kv_seq q;
     const hf_gi32* table;
-    uint32_t groups_of_page;  // groups of eight tokens the table has pages for
     f32x4 acc[VD];
     f32x4 div;      // sums of the rounded p (all four alike)
     float nm, sum;  // p = exp2(scale_log2 s + nm); the lane's share of the sum of p
@@ -499,6 +494,33 @@ struct kv_unit {
         return on ? bits8 & ((1u << left) - 1u) : 0u;
     }
 
+    // VD elements of V, as loaded, times their scale, as 16-bit pairs.
+    static __device__ __forceinline__ void decode(const kv_raw<VB>& r, const float s, uint32_t (&w)[VD / 2]) {
+        if constexpr (bits == 16) {
+#pragma unroll
+            for (int i = 0; i < VD / 2; ++i) w[i] = r.w[i];
+        } else if constexpr (bits == 8) {
+#pragma unroll
+            for (int i = 0; i < VD / 4; ++i) {
+                w[2 * i] = kv_pair<QT, FMT, 0>(r.w[i], s);
+                w[2 * i + 1] = kv_pair<QT, FMT, 1>(r.w[i], s);
+            }
+        } else {
+            w[0] = kv_pair<QT, FMT, 0>(r.w[0], s);
+            w[1] = kv_pair<QT, FMT, 1>(r.w[0], s);
+            if constexpr (VD >= 8) {
+                w[2] = kv_pair<QT, FMT, 2>(r.w[0], s);
+                w[3] = kv_pair<QT, FMT, 3>(r.w[0], s);
+            }
+            if constexpr (VD >= 16) {
+                w[4] = kv_pair<QT, FMT, 0>(r.w[1], s);
+                w[5] = kv_pair<QT, FMT, 1>(r.w[1], s);
+                w[6] = kv_pair<QT, FMT, 2>(r.w[1], s);
+                w[7] = kv_pair<QT, FMT, 3>(r.w[1], s);
+            }
+        }
+    }
+
     // The eight tokens of the lane as operand A of the product along tokens, for each of its d.
     __device__ __forceinline__ void columns(const tile& x, const uint32_t there, hf_u32x4 (&av)[VD]) const {
         uint32_t v[8][VD / 2];
@@ -508,29 +530,7 @@ struct kv_unit {
             const uint32_t w = j < 4 ? x.vs.x : x.vs.y;
             const uint32_t sb = ((j & 3) == 3 ? w >> 1 : w << (23 - 8 * (j & 3))) & 0x7F800000u;
             const float s = __uint_as_float(sb);
-            if constexpr (bits == 16) {
-#pragma unroll
-                for (int i = 0; i < VD / 2; ++i) v[j][i] = x.v[j].w[i];
-            } else if constexpr (bits == 8) {
-#pragma unroll
-                for (int i = 0; i < VD / 4; ++i) {
-                    v[j][2 * i] = kv_pair<QT, FMT, 0>(x.v[j].w[i], s);
-                    v[j][2 * i + 1] = kv_pair<QT, FMT, 1>(x.v[j].w[i], s);
-                }
-            } else {
-                v[j][0] = kv_pair<QT, FMT, 0>(x.v[j].w[0], s);
-                v[j][1] = kv_pair<QT, FMT, 1>(x.v[j].w[0], s);
-                if constexpr (VD >= 8) {
-                    v[j][2] = kv_pair<QT, FMT, 2>(x.v[j].w[0], s);
-                    v[j][3] = kv_pair<QT, FMT, 3>(x.v[j].w[0], s);
-                }
-                if constexpr (VD >= 16) {
-                    v[j][4] = kv_pair<QT, FMT, 0>(x.v[j].w[1], s);
-                    v[j][5] = kv_pair<QT, FMT, 1>(x.v[j].w[1], s);
-                    v[j][6] = kv_pair<QT, FMT, 2>(x.v[j].w[1], s);
-                    v[j][7] = kv_pair<QT, FMT, 3>(x.v[j].w[1], s);
-                }
-            }
+            decode(x.v[j], s, v[j]);
             if (!(there >> j & 1u)) {  // nothing is known of what the page holds behind the last token
 #pragma unroll
                 for (int i = 0; i < VD / 2; ++i) v[j][i] = 0;
@@ -557,29 +557,7 @@ struct kv_unit {
                                                                       ((int64_t)(d >> a.c.group_shift) << a.c.page_shift)]
                                 << 23);
         uint32_t w[VD / 2];
-        if constexpr (bits == 16) {
-#pragma unroll
-            for (int i = 0; i < VD / 2; ++i) w[i] = r.w[i];
-        } else if constexpr (bits == 8) {
-#pragma unroll
-            for (int i = 0; i < VD / 4; ++i) {
-                w[2 * i] = kv_pair<QT, FMT, 0>(r.w[i], s);
-                w[2 * i + 1] = kv_pair<QT, FMT, 1>(r.w[i], s);
-            }
-        } else {
-            w[0] = kv_pair<QT, FMT, 0>(r.w[0], s);
-            w[1] = kv_pair<QT, FMT, 1>(r.w[0], s);
-            if constexpr (VD >= 8) {
-                w[2] = kv_pair<QT, FMT, 2>(r.w[0], s);
-                w[3] = kv_pair<QT, FMT, 3>(r.w[0], s);
-            }
-            if constexpr (VD >= 16) {
-                w[4] = kv_pair<QT, FMT, 0>(r.w[1], s);
-                w[5] = kv_pair<QT, FMT, 1>(r.w[1], s);
-                w[6] = kv_pair<QT, FMT, 2>(r.w[1], s);
-                w[7] = kv_pair<QT, FMT, 3>(r.w[1], s);
-            }
-        }
+        decode(r, s, w);
 #pragma unroll
         for (int i = 0; i < VD / 2; ++i) {
             const uint32_t x = w[i];
