@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_kv import dev, kv, make  # noqa: F401  (kv: a fixture)
+from tests import kv_reference as R
+from tests.test_gpu_kv import attend_case, dev, kv, make, rows_of, verify  # noqa: F401  (kv: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -86,6 +87,84 @@ def test_many_small_weights(kv, fmt, dtype, n, per, below):
     assert ((got.cpu().double() - want).abs() <= near).all()
     ref = torch.from_numpy(scale + np.log1p(small))[:, None]
     assert ((lse.cpu().double() - ref).abs() <= length * 2.0 ** -24 + 2.0 ** -19 + 2.0 ** -21 * ref).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2", "e2m1"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,per", [(1, 3), (20, 3), (50, 4)])
+def test_scale_bytes_at_their_ends(kv, fmt, dtype, n, per):
+    """Scale bytes of 0 and 255 among a caller's own: 2^-127, and NaN that reaches the rows that see it alone."""
+    f, dim = {"e4m3": R.E4M3, "e5m2": R.E5M2, "e2m1": R.E2M1}[fmt], 64
+    rng = np.random.default_rng(5)
+    past, page = 70, 16
+    length = past + n
+    pages = -(-length // page)
+    c = make(kv, fmt, pages, page, 1, dim, 32)
+    table, kv_len, cu = np.arange(pages, dtype=np.int32)[None], np.array([length], np.int32), np.array([0, n], np.int32)
+    x = rows_of(rng, length, 1, dim, dtype)
+    full = dev(np.array([0, length], np.int32))
+    c.write(x.cuda(), x.cuda(), dev(table), dev(kv_len), full)
+    c.ctx.sync()
+    c.k_scale[0, 0, 1, 3] = 0      # a token of the past with tiny keys
+    c.v_scale[1, 0, 0, 5] = 0      # ... and with tiny values
+    c.v_scale[2, 0, 1, 1] = 1
+    last = length - 1              # the last row alone sees NaN values
+    c.v_scale[last // page, 0, 1, last % page] = 255
+    back = c.read(dev(table), dev(kv_len), full, rows=length, dtype=torch.float32)
+    q = rows_of(rng, n, per, dim, dtype, 0.7)
+    got, lse = c.attend(q.cuda(), dev(table), dev(kv_len), dev(cu), max_q=n, lse=True)
+    c.ctx.sync()
+    k, v = R.pool_values(c.k, c.k_scale, f), R.pool_values(c.v, c.v_scale, f)
+    for t, pool in zip(back, (k, v)):
+        want = torch.from_numpy(pool.reshape(-1, 1, dim)[:length]).float()
+        assert torch.equal(t.cpu().nan_to_num(nan=12345.0), want.nan_to_num(nan=12345.0))
+    out, ref, weight = R.attend(q.double().numpy(), k, v, table, kv_len, cu, None, dim ** -0.5)
+    got = got.cpu().double().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(out)) and np.isnan(out[-1, :, 32:]).all() and not np.isnan(out[:-1]).any()
+    fin = np.isfinite(out)
+    dt = torch.float16 if dtype == "fp16" else torch.bfloat16
+    tol = R.tolerance(np.where(fin, out, 0), np.where(fin, weight, 0), q.double().numpy(), float(np.abs(k[np.isfinite(k)]).max()),
+                      length, dim ** -0.5, dt)
+    assert (np.abs(np.where(fin, got, 0) - np.where(fin, out, 0)) <= tol).all()
+    assert np.isfinite(lse.cpu().numpy()).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2", "e2m1"])
+@pytest.mark.parametrize("n,per", [(1, 3), (20, 3), (50, 4)])
+def test_fp16_queries_take_values_as_fp16_reads_them(kv, fmt, n, per):
+    """Values of a past token and of a draft beyond 65504 are infinite for fp16 queries, as hf_kv_read gives them,
+    and reach the rows that see them."""
+    f, dim, past, page = {"e4m3": R.E4M3, "e5m2": R.E5M2, "e2m1": R.E2M1}[fmt], 64, 70, 16
+    length = past + n
+    pages = -(-length // page)
+    c = make(kv, fmt, pages, page, 1, dim, 32)
+    rng = np.random.default_rng(8)
+    table, kv_len, cu = np.arange(pages, dtype=np.int32)[None], np.array([length], np.int32), np.array([0, n], np.int32)
+    x = rows_of(rng, length, 1, dim, "fp16").cuda()
+    full = dev(np.array([0, length], np.int32))
+    c.write(x, x, dev(table), dev(kv_len), full)
+    c.ctx.sync()
+    seen_by_all, group = 9, {"e4m3": 136, "e5m2": 129, "e2m1": 142}[fmt]  # a part of the values passes 65504
+    c.v_scale[0, 0, 0, seen_by_all] = group
+    draft = length - 1
+    c.v_scale[draft // page, 0, 1, draft % page] = group
+    read = c.read(dev(table), dev(kv_len), full, rows=length, dtype=torch.float16)[1]
+    q = rows_of(rng, n, per, dim, "fp16", 0.7)
+    got, lse = c.attend(q.cuda(), dev(table), dev(kv_len), dev(cu), max_q=n, lse=True)
+    c.ctx.sync()
+    k, v = R.pool_values(c.k, c.k_scale, f), R.pool_values(c.v, c.v_scale, f)
+    flat = torch.from_numpy(v.reshape(-1, 1, dim)[:length]).to(torch.float16)
+    assert torch.equal(read.cpu(), flat)
+    assert torch.isinf(flat[seen_by_all, 0, :32]).any() and torch.isinf(flat[draft, 0, 32:]).any()
+    v16 = np.zeros_like(v)
+    v16.reshape(-1, 1, dim)[:length] = flat.double().numpy()
+    out, ref, weight = R.attend(q.double().numpy(), k, v16, table, kv_len, cu, None, dim ** -0.5)
+    got = got.cpu().double().numpy()
+    fin = np.isfinite(out)
+    assert np.array_equal(got[~fin], out[~fin]) and np.isfinite(got[fin]).all()
+    tol = R.tolerance(np.where(fin, out, 0), np.where(fin, weight, 0), q.double().numpy(), float(np.nanmax(np.abs(k[np.isfinite(k)]))),
+                      length, dim ** -0.5, torch.float16)
+    assert (np.abs(np.where(fin, got, 0) - np.where(fin, out, 0)) <= tol).all()
 
 
 # ---- lists -----------------------------------------------------------------------------------------
@@ -340,3 +419,76 @@ def test_tensors_dropped_before_another_stream_has_used_them(kv, hf):
     ctx.sync()
     for x, y in zip(want, got):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+# ---- shapes ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("fmt", ["bf16", "fp16", "e4m3", "e5m2", "e2m1"])
+@pytest.mark.parametrize("dim,heads,per,new,past,mask", [
+    (160, 2, 4, [1, 1, 1], [0, 40, 700], None), (192, 1, 8, [1], [2100], None), (160, 1, 2, [70], [33], None),
+    (192, 2, 3, [9, 0, 31], [5, 0, 100], "tree"), (64, 1, 100, [3], [50], None), (32, 3, 1, [200], [0], None),
+    (128, 1, 300, [1, 1], [90, 10], None)])
+def test_attend_other_shapes(kv, fmt, dtype, dim, heads, per, new, past, mask):
+    if fmt in ("bf16", "fp16") and fmt != dtype:
+        pytest.skip("a 16-bit cache takes queries of its own type")
+    c, f, q, table, kv_len, cu, m = attend_case(kv, fmt, dtype, new, past, 16, heads, per, dim, 32, "thd", mask, 17)
+    one = max(new) == 1
+    got, lse = c.attend(q.cuda(), dev(table), dev(kv_len), None if one else dev(cu), max_q=max(new),
+                        mask=None if m is None else dev(m.view(np.int32)), lse=True)
+    c.ctx.sync()
+    verify(c, f, q, table, kv_len, cu, m, got, lse, dim ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("batch", [129, 1025, 4100])
+def test_attend_many_sequences_in_large_tiles(kv, batch):
+    """More sequences than one pass of the cut takes, most of them of no row or one, a few of up to 40: tiles of
+    64 and 256 rows."""
+    rng = np.random.default_rng(batch)
+    new = rng.integers(0, 2, batch)
+    new[rng.integers(0, batch, 20)] = rng.integers(2, 41, 20)
+    new[batch - 1] = 40
+    past = rng.integers(0, 40, batch)
+    past[[batch // 3, batch - 1]] = 3000, 1500  # these are cut into ranges
+    for per in (1, 5):
+        c, f, q, table, kv_len, cu, _ = attend_case(kv, "e4m3", "bf16", [int(n) for n in new], [int(p) for p in past], 16, 1,
+                                                    per, 64, 64, "thd", None, 1)
+        got, lse = c.attend(q.cuda(), dev(table), dev(kv_len), dev(cu), max_q=40, lse=True)
+        c.ctx.sync()
+        verify(c, f, q, table, kv_len, cu, None, got, lse, 64 ** -0.5, "bf16")
+
+
+@pytest.mark.parametrize("n,per", [(16, 4), (32, 4), (64, 4)])
+def test_large_tiles_long_and_past_four_gigabytes(kv, n, per):
+    """Tiles of 64, 128 and 256 rows on 20000 tokens in the last pages of a pool of more than 2^32 bytes: bit for
+    bit what a dense small pool gives."""
+    pages, page, heads, dim = 35000, 64, 16, 128
+    if torch.cuda.mem_get_info()[0] < 12e9:
+        pytest.skip("needs 12 GB")
+    c = kv.KvCache.empty(pages, page, heads, dim, R.E4M3, 128)
+    length = 20000 + n
+    need = -(-length // page)
+    small = kv.KvCache.empty(need, page, heads, dim, R.E4M3, 128)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(length, heads, dim, generator=g, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(n, heads * per, dim, generator=g, device="cuda").bfloat16()
+    far = (pages - 1 - np.random.default_rng(2).permutation(need)).astype(np.int32)[None]
+    near = np.arange(need, dtype=np.int32)[None]
+    l, cu, full = dev(np.array([length], np.int32)), dev(np.array([0, n], np.int32)), dev(np.array([0, length], np.int32))
+    got = []
+    for cache, table in ((c, dev(far)), (small, dev(near))):
+        cache.write(k, v, table, l, full)
+        got.append(cache.attend(q, table, l, cu, max_q=n, lse=True))
+    c.ctx.sync()
+    assert torch.equal(got[0][0].view(torch.int16), got[1][0].view(torch.int16)) and torch.equal(got[0][1], got[1][1])
+    # and one head of it against the definition
+    back = small.read(dev(near), l, full, rows=length, dtype=torch.float32)
+    small.ctx.sync()
+    kk, vv = (t[:, 3].cpu().double().numpy() for t in back)
+    qq = q[:, 3 * per + 1].cpu().double().numpy()
+    s = qq @ kk.T * dim ** -0.5
+    s[np.arange(length)[None] > 20000 + np.arange(n)[:, None]] = -np.inf
+    p = np.exp(s - s.max(-1, keepdims=True))
+    z = p.sum(-1, keepdims=True)
+    out, weight = p @ vv / z, p @ np.abs(vv) / z
+    tol = R.tolerance(out, weight, qq, float(np.abs(kk).max()), length, dim ** -0.5, torch.bfloat16)
+    assert (np.abs(got[0][0][:, 3 * per + 1].cpu().double().numpy() - out) <= tol).all()
