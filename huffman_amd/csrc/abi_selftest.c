@@ -89,6 +89,52 @@ int main(void) {
     CHECK(hf_page_codebook_download(NULL, NULL, 0, NULL, 0, NULL, NULL, NULL, NULL) == HF_ERR_ARG);
     CHECK(hf_system_codebook_chunks_static(NULL, NULL, 0, HF_MODE_HUFFMAN, 0, NULL) == HF_ERR_ARG);
 
+    /* KV cache: the checks of every argument, strides and sizes at their ends among them (without a
+       context each call ends in an error) */
+    {
+        static const int64_t strides[] = {0, 1, 127, 128, 1024, 1000, 1ll << 31, (1ll << 31) + 16, 1ll << 62, INT64_MAX,
+                                          -1, -1024, INT64_MIN};
+        static const uint32_t sizes[] = {0, 1, 7, 8, 32, 96, 256, 257, 65536, 0x7FFFFFFFu, 0x80000000u, 0xFFFFFFFFu};
+        const int ns = sizeof strides / sizeof *strides, nz = sizeof sizes / sizeof *sizes;
+        int32_t lists[64] = {0};
+        char* const mem = (char*)(uintptr_t)4096; /* never followed */
+        for (int what = 0; what < 15; ++what)
+            for (int i = 0; i < (what < 6 ? ns : nz); ++i) {
+                hf_kv_cache c = {mem, mem, (uint8_t*)mem, (uint8_t*)mem, 4, 16 * 1024, 1024, 128, 16, 8, 128, 128,
+                                 HF_KV_FP8_E4M3, 0};
+                hf_kv_batch b = {NULL, lists, lists + 8, 4, 4, 2, 2, 1};
+                hf_kv_query q = {mem, mem, NULL, NULL, 4096, 128, 4096, 128, 32, 0, HF_DT_BF16, 0.1f};
+                int64_t row = 1024, head = 128, path = 4;
+                if (what == 0) c.page_stride = strides[i];
+                if (what == 1) c.token_stride = c.head_stride = strides[i];
+                if (what == 2) b.table_stride = strides[i];
+                if (what == 3) q.q_row_stride = q.out_row_stride = row = strides[i];
+                if (what == 4) q.q_head_stride = q.out_head_stride = head = strides[i];
+                if (what == 5) path = strides[i];
+                if (what == 6) c.n_pages = sizes[i];
+                if (what == 7) c.page_size = sizes[i];
+                if (what == 8) c.heads = sizes[i];
+                if (what == 9) c.head_dim = sizes[i];
+                if (what == 10) c.group = sizes[i];
+                if (what == 11) c.format = sizes[i];
+                if (what == 12) b.table_width = sizes[i];
+                if (what == 13) {
+                    b.batch = sizes[i];
+                    b.d_cu_rows = lists + 16;
+                }
+                if (what == 14) q.q_heads = sizes[i];
+                for (int dtype = -1; dtype < 4; ++dtype) {
+                    CHECK(hf_kv_write(NULL, &c, &b, mem, mem, row, head, row, head, dtype) < 0);
+                    CHECK(hf_kv_read(NULL, &c, &b, mem, mem, row, head, row, head, dtype) < 0);
+                }
+                CHECK(hf_kv_attend(NULL, &c, &b, &q, mem, 1u << 20) < 0);
+                CHECK(hf_kv_attend_work_bytes(NULL, &c, &b, q.q_heads) == 0);
+                CHECK(hf_kv_keep(NULL, &c, &b, lists + 32, path, 3, lists + 40, lists + 48) < 0);
+            }
+        CHECK(hf_kv_write(NULL, NULL, NULL, NULL, NULL, 0, 0, 0, 0, 0) == HF_ERR_ARG);
+        CHECK(hf_kv_keep(NULL, NULL, NULL, NULL, 0, 0, NULL, NULL) == HF_ERR_ARG);
+    }
+
     hf_ctx* ctx = NULL;
     const int rc = hf_ctx_create(&ctx, 0, NULL);
     if (rc == HF_OK) {

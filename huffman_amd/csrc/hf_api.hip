@@ -1582,9 +1582,9 @@ int kv_check_batch(const hf_kv_batch* b, hf_kv_seqs* s) {
 // row tensors: whole 16-byte pieces wherever a row or a head starts
 int kv_check_rows(const void* p, int64_t row_stride, int64_t head_stride, int elem, hf_kv_rows* r) {
     if (!p) return HF_ERR_ARG;
-    if (!aligned16(p) || (row_stride * elem) % 16 || (head_stride * elem) % 16) return HF_ERR_ALIGN;
     if (row_stride < 0 || head_stride < 0) return HF_ERR_ARG;
     if (row_stride > (1ll << 31) || head_stride > (1ll << 31)) return HF_ERR_RANGE;
+    if (!aligned16(p) || (row_stride * elem) % 16 || (head_stride * elem) % 16) return HF_ERR_ALIGN;
     r->p = const_cast<void*>(p);
     r->row_stride = (uint32_t)row_stride;
     r->head_stride = (uint32_t)head_stride;
@@ -1763,13 +1763,13 @@ int hf_kv_keep(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch,
     if (int rc = kv_check_batch(batch, &s)) return rc;
     if (s.batch && (!d_path_len || !d_new_len)) return HF_ERR_ARG;
     if (s.batch && ((path_width && !d_path) || path_stride < path_width)) return HF_ERR_ARG;
+    if (path_stride > (1ll << 31)) return HF_ERR_RANGE;
     // (the workgroups of a sequence's heads read its lists, and some have not when the first writes)
     if (kv_touches(d_new_len, s.batch, s.kv_len, 1, s.batch, 0) || kv_touches(d_new_len, s.batch, d_path_len, 1, s.batch, 0) ||
         kv_touches(d_new_len, s.batch, s.cu, 1, (uint64_t)s.batch + 1, 0) ||
         kv_touches(d_new_len, s.batch, d_path, s.batch, path_width, (uint64_t)path_stride) ||
         kv_touches(d_new_len, s.batch, s.table, s.batch, s.width, s.table_stride))
         return HF_ERR_ARG;
-    if (path_stride > (1ll << 31)) return HF_ERR_RANGE;
     if (!ctx) return HF_ERR_ARG;
     if (s.batch == 0) return HF_OK;
     HF_USE_DEVICE(ctx);
