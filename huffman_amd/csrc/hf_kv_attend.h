@@ -728,7 +728,7 @@ struct kv_lds {
 };
 
 // Bound by memory and the latency of its loads: 64 sequences of up to 8001 tokens, 8 heads of 128 in
-// e4m3 (675 MB), in 151 us, 4.5 TB/s; 64 of 32 k at 5.1 TB/s, where a large read reaches 6.1.  The
+// e4m3 (675 MB), in 149 us, 4.5 TB/s; 64 of 32 k at 5.1 TB/s, where a large read reaches 6.1.  The
 // registers of a tile are loaded again as soon as they have been turned into operands (a second tile
 // in flight costs a wavefront of two and was slower, 187 us).
 template <int QT, int FMT, int DP>
@@ -854,7 +854,7 @@ void hf_k_kv_attend(const hf_kv_attend_args a) {
 
 // Joins the ranges of rows that have several: a wavefront takes a row of a head at a time, DP / 4
 // lanes along it and the ranges dealt to the groups of lanes that are left.  4 us for one
-// token, 10 for eight trees of up to 63 tokens x 32 heads in four ranges.  A row's sequence is searched
+// token, 11 for eight trees of up to 63 tokens x 32 heads in four ranges.  A row's sequence is searched
 // (the whole call for 4096 sequences of 3 rows, one of them long: 876 us; with the offsets walked 1420).
 template <int QT, int DP>
 __global__ __launch_bounds__(256) void hf_k_kv_join(const hf_kv_attend_args a, const uint32_t tile_rows) {

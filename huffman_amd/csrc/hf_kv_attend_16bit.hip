@@ -10,7 +10,11 @@ void hf_launch_kv_attend_fp4_e2m1(const hf_kv_attend_args&, int, int, hipStream_
 // 135 / 313, of 64 rows 226 / 122 / 158 / 332; 16 of 68 rows 141 / 98 / 78 / 120, of 128 rows 204 /
 // 115 / 94 / 145, of 160 rows 292 / 186 / 147 / 137; 64 sequences of 4 rows 155 / 201 / 271 / -.
 // A padded head_dim of 256 fills the registers of the 128-row kernel, which is the fastest from 8
-// rows (172 against 204 with 16) to 64 (77 against 111 with 64, 163 with 16): it has that one only.
+// rows (172 against 204 with 16) to 64 (77 against 111 with 64, 163 with 16): it has that one only.  Below
+// 8 rows it is slow: single tokens of 64 sequences of up to 8001 tokens, 4 cache heads of 160 to 256 in e4m3,
+// take 515 to 540 us whether 1, 2 or 4 query heads share them, a quarter of the rate of 128 (88 to 90).
+// The rule goes by the longest sequence of the call: a chunk of 1000 rows beside 63 single tokens takes
+// 585 us in one call, 146 + 154 in two.
 int hf_kv_attend_tile_rows(uint32_t max_q, uint32_t per, uint32_t head_dim) {
     const uint64_t rows = (uint64_t)max_q * per;
     if (head_dim > 128) return 128;

@@ -285,8 +285,8 @@ struct kv_deal {
     uint32_t pieces, per_head, inv, tokens;
 };
 
-// Bound by memory: 42 k rows of 8 x 128 bf16 to e4m3 (260 MB) in 55 us, 4.7 TB/s, what a large copy
-// reaches; 64 rows in 3.7 us, which is a launch and three dependent loads.
+// Bound by memory: 42 k rows of 8 x 128 bf16 to e4m3 (260 MB) in 57 us, 4.6 TB/s (a large copy: 4.9);
+// 64 rows in 3.9 us, which is a launch and three dependent loads.
 template <int FMT, int DT>
 __global__ __launch_bounds__(kThreads) void hf_k_kv_write(const hf_kv_pools c, const hf_kv_seqs s,
                                                           const hf_kv_rows k, const hf_kv_rows v,
@@ -341,7 +341,8 @@ __global__ __launch_bounds__(kThreads) void hf_k_kv_write(const hf_kv_pools c, c
     }
 }
 
-// Bound by memory: 41 k rows of 8 x 128 e4m3 to bf16 (254 MB) in 44 us, 5.8 TB/s.
+// Bound by memory: 41 k rows of 8 x 128 e4m3 to bf16 (254 MB) in 55 us, 4.6 TB/s (into the same outputs
+// call after call, which the last cache then holds, 44).
 template <int FMT, int DT>
 __global__ __launch_bounds__(kThreads) void hf_k_kv_read(const hf_kv_pools c, const hf_kv_seqs s,
                                                          const hf_kv_rows k, const hf_kv_rows v,
@@ -402,7 +403,7 @@ kv_deal deal_of(const hf_kv_pools& c, const uint32_t rows, const int num_cu) {
 // past + i, for i < path_len[b].  A path ascends, so a row's place is never behind its source, and
 // the rows of a later turn of the loop come from behind every place an earlier turn wrote; inside
 // a turn all loads come before all stores.  One workgroup per sequence and head: 64 trees of up to
-// 48 drafts take 4.6 us, one tree 4.1, a launch and its chain of loads.
+// 48 drafts take 5.0 us, one tree 4.1, a launch and its chain of loads.
 __global__ __launch_bounds__(kThreads) void hf_k_kv_keep(const hf_kv_pools c, const hf_kv_seqs s,
                                                          const int32_t* path, const int64_t path_stride,
                                                          const uint32_t path_width, const int32_t* path_len,

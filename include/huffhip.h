@@ -631,7 +631,9 @@ typedef struct hf_kv_batch {
     uint32_t table_width;
     uint32_t batch;
     uint32_t rows;     /* rows of the row tensors */
-    uint32_t max_rows; /* hf_kv_attend: rows of a sequence, at most (a larger bound costs speed) */
+    uint32_t max_rows; /* hf_kv_attend: rows of a sequence, at most.  It chooses the tiles: a larger bound
+                        * costs speed, and so do single tokens in a call that has a long chunk beside them
+                        * (two calls are faster) */
 } hf_kv_batch;
 
 /* Quantises the rows d_k, d_v [rows][heads][head_dim] into their places.  A group's scale exponent
