@@ -1591,6 +1591,13 @@ int kv_check_rows(const void* p, int64_t row_stride, int64_t head_stride, int el
     return HF_OK;
 }
 
+// Two row tensors of one call with elements in common (of the same strides; others are the caller's care).
+bool kv_rows_meet(uint32_t rows, uint32_t heads, uint32_t dim, int elem, const hf_kv_rows& a, const hf_kv_rows& b) {
+    return a.row_stride == b.row_stride && a.head_stride == b.head_stride &&
+           hf_kv_rows_meet(rows, heads, a.row_stride, a.head_stride, dim,
+                           ((int64_t)(uintptr_t)b.p - (int64_t)(uintptr_t)a.p) / elem);
+}
+
 // Whether `count` entries at p touch any of `rows` rows of `width` entries that lie `stride` apart.
 bool kv_touches(const int32_t* p, uint64_t count, const int32_t* row0, uint64_t rows, uint64_t width, uint64_t stride) {
     if (!count || !rows || !width || !row0) return false;
@@ -1624,6 +1631,7 @@ int kv_move(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch, con
     if (!write && !none && (hf_kv_rows_touch(s.rows, p.heads, k.row_stride, k.head_stride, p.head_dim) ||
                             hf_kv_rows_touch(s.rows, p.heads, v.row_stride, v.head_stride, p.head_dim)))
         return HF_ERR_ARG;
+    if (!write && !none && kv_rows_meet(s.rows, p.heads, p.head_dim, elem, k, v)) return HF_ERR_ARG;
     if (!ctx) return HF_ERR_ARG;
     if (none) return HF_OK;
     HF_USE_DEVICE(ctx);
@@ -1730,6 +1738,10 @@ int hf_kv_attend(hf_ctx* ctx, const hf_kv_cache* cache, const hf_kv_batch* batch
     if (int rc = kv_check_rows(query->d_q, query->q_row_stride, query->q_head_stride, 2, &a.q)) return rc;
     if (int rc = kv_check_rows(query->d_out, query->out_row_stride, query->out_head_stride, 2, &a.out)) return rc;
     if (hf_kv_rows_touch(a.s.rows, query->q_heads, a.out.row_stride, a.out.head_stride, a.c.head_dim)) return HF_ERR_ARG;
+    // (in place is fine: a row of a head is read and written by one unit; a shift is not)
+    const bool alike = (a.s.rows == 1 || a.out.row_stride == a.q.row_stride) &&
+                       (query->q_heads == 1 || a.out.head_stride == a.q.head_stride);
+    if (a.out.p == a.q.p ? !alike : kv_rows_meet(a.s.rows, query->q_heads, a.c.head_dim, 2, a.q, a.out)) return HF_ERR_ARG;
     if (!ctx) return HF_ERR_ARG;
     if (int rc = kv_plan_of(ctx, a.c, a.s, a.per, &plan)) return rc;
     if (plan.bytes > work_bytes || (plan.bytes && !d_work)) return HF_ERR_ARG;

@@ -57,6 +57,25 @@ inline bool hf_kv_rows_touch(const uint64_t rows, const uint64_t heads, const ui
     return false;
 }
 
+// Whether two row tensors of the same strides, the second `apart` elements behind the first, have an element
+// in common: for every distance in heads the two rows nearest to it are looked at.
+inline bool hf_kv_rows_meet(const int64_t rows, const int64_t heads, const int64_t row_stride,
+                            const int64_t head_stride, const int64_t dim, const int64_t apart) {
+    if (rows == 0 || heads == 0) return false;
+    const int64_t extent = (rows - 1) * row_stride + (heads - 1) * head_stride + dim;
+    if (apart >= extent || apart <= -extent) return false;
+    for (int64_t j = 1 - heads; j < heads; ++j) {
+        const int64_t rest = apart - j * head_stride;
+        int64_t i = row_stride ? rest / row_stride : 0;
+        if (i * row_stride > rest) --i;  // (down, also below zero)
+        for (int64_t at = i; at <= i + 1; ++at) {
+            const int64_t off = rest - (at <= -rows ? 1 - rows : at >= rows ? rows - 1 : at) * row_stride;
+            if (off < dim && off > -dim) return true;
+        }
+    }
+    return false;
+}
+
 struct hf_kv_attend_args {
     hf_kv_pools c;
     hf_kv_seqs s;

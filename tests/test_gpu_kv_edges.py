@@ -372,6 +372,43 @@ def test_outputs_that_lie_on_one_another_are_refused(kv):
     c.ctx.sync()
 
 
+@pytest.mark.parametrize("n,per,past", [(1, 4, 3000), (5, 4, 20), (33, 4, 40), (70, 4, 40)])
+def test_outputs_over_what_the_call_reads_or_writes(kv, n, per, past):
+    """Outputs over the queries themselves, row for row, are as anywhere else; over other rows of them, or keys
+    over values, they are refused."""
+    from huffman_amd import HuffhipError
+    c, f, q, table, kv_len, cu, _ = attend_case(kv, "e4m3", "bf16", [n, n], [past, 7], 16, 2, per, 64, 64, "thd", None, 3)
+    lists = dev(table), dev(kv_len), dev(cu)
+    q = q.cuda()
+    want = c.attend(q, *lists, max_q=n)
+    buf = torch.zeros(2 * n + 1, 2 * per, 64, device="cuda", dtype=torch.bfloat16)
+    for lo in (0, 1):
+        same = buf[lo:lo + 2 * n]
+        same.copy_(q)
+        assert c.attend(same, *lists, max_q=n, out=same) is same and torch.equal(same, want)
+    for a, b in ((0, 1), (1, 0)):
+        with pytest.raises(HuffhipError):
+            c.attend(buf[a:a + 2 * n], *lists, max_q=n, out=buf[b:b + 2 * n])
+    flat = torch.zeros(2 * n * 2 * per * 64, device="cuda", dtype=torch.bfloat16)
+    turned = flat.view(2 * per, 2 * n, 64).transpose(0, 1)  # the same memory, heads in front
+    turned.copy_(q)
+    with pytest.raises(HuffhipError):
+        c.attend(turned, *lists, max_q=n, out=flat.view(q.shape))
+    assert torch.equal(c.attend(turned, *lists, max_q=n, out=turned), want)
+    rows = torch.zeros(2 * n + 1, 3, 64, device="cuda", dtype=torch.bfloat16)
+    for k, v in ((rows[1:, :2], rows[1:, :2]), (rows[1:, :2], rows[1:, 1:]), (rows[1:, 1:], rows[1:, :2]),
+                 (rows[1:, :2], rows[:-1, :2]) if n > 1 else (rows[1:, :2], rows[1:, :2])):
+        with pytest.raises(HuffhipError):
+            c.read(*lists, out=(k, v))
+    good = c.read(*lists, rows=2 * n)
+    wide = torch.zeros(2 * n, 4, 64, device="cuda", dtype=torch.bfloat16)
+    got = c.read(*lists, out=(wide[:, 2:], wide[:, :2]))
+    assert torch.equal(got[0], good[0]) and torch.equal(got[1], good[1])
+    got = c.read(*lists, out=(wide[:, ::2], wide[:, 1::2]))
+    assert torch.equal(got[0], good[0]) and torch.equal(got[1], good[1])
+    c.ctx.sync()
+
+
 # ---- streams ---------------------------------------------------------------------------------------
 def test_tensors_dropped_before_another_stream_has_used_them(kv, hf):
     """Every tensor of a call on a context's own stream, which is busy, is dropped right after the call and

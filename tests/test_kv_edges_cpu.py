@@ -127,3 +127,37 @@ def test_the_pools_device_is_asked_for_a_capture(monkeypatch, captured):
     else:
         assert c.ctx == ("context", 1, ("stream", 1)) and list(api._default_ctx) == [(1, 77)]
     assert now == [0]
+
+
+MEET_TEST = r'''
+#include <cstdio>
+#include <cstring>
+#include "hf_kv.h"
+// two tensors of the same strides, moved against one another, against every element counted
+int main() {
+    long meet = 0, apart = 0;
+    for (int rows = 0; rows < 5; ++rows) for (int heads = 0; heads < 5; ++heads) for (int dim : {1, 3, 4})
+        for (int rs = 0; rs <= 24; ++rs) for (int hs = 0; hs <= 24; ++hs) {
+            char hit[256];
+            memset(hit, 0, sizeof hit);
+            for (int i = 0; i < rows; ++i) for (int j = 0; j < heads; ++j) memset(hit + i * rs + j * hs, 1, dim);
+            for (int off = -210; off <= 210; ++off) {
+                bool want = false;
+                for (int i = 0; i < rows; ++i) for (int j = 0; j < heads; ++j) for (int d = 0; d < dim; ++d) {
+                    const int at = i * rs + j * hs + d + off;
+                    want = want || (at >= 0 && at < 256 && hit[at]);
+                }
+                if (hf_kv_rows_meet(rows, heads, rs, hs, dim, off) != want) {
+                    printf("rows %d heads %d strides %d %d dim %d apart %d\n", rows, heads, rs, hs, dim, off);
+                    return 1;
+                }
+                ++(want ? meet : apart);
+            }
+        }
+    printf("ok %ld %ld\n", meet, apart);
+}
+'''
+
+
+def test_row_tensors_that_share_elements(tmp_path):
+    run_on_host(tmp_path, MEET_TEST)
