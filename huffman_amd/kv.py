@@ -170,7 +170,7 @@ class KvCache(_Module):
         shape = t.shape
         # (one entry may have any stride: a column of a wider list, for one sequence)
         if t.dtype != torch.int32 or len(shape) != dim or t.get_device() != self._index or \
-                (shape[-1] > 1 and t.stride(-1) != 1):
+                (shape[-1] > 1 and t.stride(-1) != 1 and t.numel()):
             raise ValueError(f"{name}: int32, {dim} dimension(s), contiguous rows, on the pools' device")
         return shape
 

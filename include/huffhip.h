@@ -590,13 +590,13 @@ int hf_container_codebook(hf_ctx* ctx, const void* d_blob, const hf_container_in
  * defined (offsets that fall: what any row of the call holds).
  * A page may belong to several sequences (a shared prefix) as long as no call writes it for two.
  *
- * All calls only enqueue work, allocate nothing and can be captured.  Row tensors are 16-byte
- * aligned with strides in elements that are multiples of 8 (fp32: of 4); pools, scales and byte
- * strides are 16-byte aligned (HF_ERR_ALIGN); rows that a call writes to lie apart, from
- * one another and from what it reads (HF_ERR_ARG; hf_kv_attend may write over its own queries, row
- * for row).  A call without rows or sequences does nothing.  heads <= 1024, 32 <= head_dim <= 256 in steps of 32,
- * group a power of two from 32 that divides head_dim, page_size a power of two in 8 .. 65536
- * (HF_ERR_ARG). */
+ * All calls only enqueue work, allocate nothing and can be captured; writing, reading and attending do
+ * nothing without rows or sequences.  Row tensors are 16-byte aligned with strides in elements that
+ * are multiples of 8 (fp32: of 4); pools, scales and byte strides are 16-byte aligned (HF_ERR_ALIGN).
+ * Rows that a call writes to lie apart, from one another and from what it reads (HF_ERR_ARG;
+ * hf_kv_attend may write over its own queries, row for row).  heads <= 1024, 32 <= head_dim <= 256 in
+ * steps of 32, group a power of two from 32 that divides head_dim, page_size a power of two in
+ * 8 .. 65536 (HF_ERR_ARG). */
 #define HF_KV_BF16 0
 #define HF_KV_FP16 1
 #define HF_KV_FP8_E4M3 2

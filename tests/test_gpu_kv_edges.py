@@ -529,3 +529,30 @@ def test_large_tiles_long_and_past_four_gigabytes(kv, n, per):
     out, weight = p @ vv / z, p @ np.abs(vv) / z
     tol = R.tolerance(out, weight, qq, float(np.abs(kk).max()), length, dim ** -0.5, torch.bfloat16)
     assert (np.abs(got[0][0][:, 3 * per + 1].cpu().double().numpy() - out) <= tol).all()
+
+
+@pytest.mark.parametrize("heads,dim,group", [(1024, 32, 32), (1024, 256, 32), (1000, 224, 32), (513, 160, 32)])
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1", "bf16"])
+def test_as_many_heads_as_there_may_be(kv, fmt, heads, dim, group):
+    """Rows of up to 32768 pieces, dealt to threads by a multiplication: written, read, kept and attended to."""
+    new, past, page = [3, 0, 2], [0, 4, 9], 8
+    c, f, q, table, kv_len, cu, _ = attend_case(kv, fmt, "bf16", new, past, page, heads, 1, dim, group, "thd", None, 2)
+    lists = dev(table), dev(kv_len), dev(cu)
+    x = rows_of(np.random.default_rng(3), 5, heads, dim, "bf16")
+    c.write(x.cuda(), (x * 2).cuda(), *lists)
+    got = c.read(*lists, rows=5)
+    c.ctx.sync()
+    if fmt == "bf16":
+        want = x.double()
+    else:
+        want = torch.from_numpy(R.dequantise(*R.quantise(x.double().numpy(), f, group), f, group))
+    assert torch.equal(got[0].cpu(), want.bfloat16()) and torch.equal(got[1].cpu(), (2 * want).bfloat16())
+    out, lse = c.attend(q.cuda(), *lists, max_q=3, lse=True)
+    c.ctx.sync()
+    verify(c, f, q, table, kv_len, cu, None, out, lse, dim ** -0.5, "bf16")
+    new_len = c.keep(*lists, dev(np.array([[1, 2], [0, 0], [1, 0]], np.int32)), dev(np.array([2, 0, 1], np.int32)))
+    assert new_len.tolist() == [2, 4, 10]
+    after = c.read(*lists, rows=5)
+    for a, b in zip(got, after):
+        assert torch.equal(b[[0, 1, 3]], a[[1, 2, 4]]) and torch.equal(b[[2, 4]], a[[2, 4]])
+    c.ctx.sync()
